@@ -451,6 +451,91 @@ int star_xattn_bwd(const void* q, const void* k, const void* v, const void* o, c
 int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, int Kn, int bias_len,
                          float* dbias, void* stream);
 
+/* ---------------------------------------------------------------- causal self-attention of packed sequences
+ * The other branch of MyGPT2Attention (src/models/my_transformer.py:476-603 with is_cross_attention = False): the
+ * attention of the semantic encoder over the frames and of the decoder over its own tokens, on sequences that lie one
+ * behind the other instead of in a padded batch, with grouped heads (query head h reads key head h / (H / Hkv)).
+ *   q [rows,H,hd], k / v [rows,Hkv,hd], o like q: 16-bit values of one type (dtype), hd contiguous, row and head
+ *        strides in elements, multiples of 8; base addresses multiples of 16 bytes.  hd in {64, 96, 128}
+ *   seqs [nseq][4] int32: first query row, queries nq, first key row, keys nk.  Query i of a sequence sees its keys
+ *        j <= i + nk - nq (the queries are the newest nq positions); a query that sees no key gets o = 0, lse = -inf
+ *   tiles [ntiles][2] int32: sequence and first query of every tile of STAR_CAUSAL_TILE queries, each exactly once, in
+ *        the order in which they are to start (longest first balances the load).  Rows in no sequence are not touched
+ *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward
+ * Softmax statistics and sums are fp32; the weights P are rounded to dtype for the product with V (as the inputs are).
+ * Nothing is masked by arithmetic on values: a key after the query never enters its maximum, sum or output, with one
+ * exception: V rows of the SAME sequence behind the query but inside its 64-key tile meet a weight of exactly 0, so an
+ * infinite or NaN V reaches up to 63 earlier queries of its own sequence. */
+#define STAR_DT_F16 2
+#define STAR_CAUSAL_TILE 128
+typedef struct {
+    int H, Hkv, hd, dtype, nseq;
+    int64_t q_sr, q_sh, k_sr, k_sh, v_sr, v_sh, o_sr, o_sh;
+    int64_t lse_stride;
+    float scale;
+} star_causal_shape;
+int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles, int ntiles,
+                    const star_causal_shape* s, void* o, float* lse, void* stream);
+/* Backward: P recomputed from lse.  do_ has o's strides; dq [rows,H,hd] and dk / dv [rows,Hkv,hd] are dense.  q_tiles as
+ * tiles above; k_tiles [nk_tiles][2]: the same for tiles of STAR_CAUSAL_TILE keys.  delta [H][lse_stride] fp32 scratch.
+ * No atomics: the gradient of a shared key head is summed over its query heads in a fixed order. */
+int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
+                    const int32_t* seqs, const int32_t* q_tiles, int nq_tiles, const int32_t* k_tiles, int nk_tiles,
+                    const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit key/value cache and attention over it
+ * A cache of B sequences x Hkv key heads x T tokens (T a multiple of STAR_KV8_BLOCK = 64), for generation and for the
+ * growing nugget memory of the streaming path.  Tokens are kept in blocks of 64 of one head.  A block that is complete
+ * is held as OCP e4m3 values times ONE scale, the smallest power of two 2^e, e >= -126, with max|x| <= 448 * 2^e over
+ * the block's finite values (1 for an all-zero block): the division by the scale is exact, so the only error is the
+ * rounding of each value to e4m3 (half a step: 2^-4 of the value; 2^(e-10) below 2^(e-6)).  An infinity or NaN is held
+ * as NaN.  The newest, incomplete block is held as it came, in dtype.  What is held depends on the tokens alone, not on
+ * how they were split into calls.
+ *   k_codes [B][Hkv][T][hd], k_scales [B][Hkv][T/64]         k_tail [B][Hkv][64][hd]  (row = token % 64)
+ *   v_codes [B][Hkv][T/64][hd][64], v_scales [B][Hkv][T/64]  v_tail [B][Hkv][hd][64]  (V is transposed inside a block)
+ *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written); tickets [B]: zero before the
+ *   first call, zero after every call.  All base addresses multiples of 16 bytes.
+ * Calls on one cache are ordered by the stream: two appends, or an append and an attention, must not overlap. */
+#define STAR_KV8_BLOCK 64
+typedef struct {
+    int B, Hkv, T, hd, dtype;
+    uint8_t* k_codes;
+    float* k_scales;
+    uint8_t* v_codes;
+    float* v_scales;
+    void* k_tail;
+    void* v_tail;
+    int32_t* lens;
+    int32_t* dropped;
+    int32_t* tickets;
+} star_kv8_cache;
+
+/* Append rows of k, v (dtype; element strides per sequence, head, row, multiples of 8; hd contiguous; 16-byte aligned).
+ *   starts, counts (either may be NULL): sequence b gives the rows starts[b * idx_stride] .. + counts[b * idx_stride] of
+ *       k + b * k_sb; NULL starts: from row 0; NULL counts: max_rows rows.  counts are clamped to [0, max_rows]
+ *   at [B] or NULL: the position of the first of them, in place of lens[b].  Only positions at or behind the first token
+ *       of the open block can be written again.  lens[b] becomes at + count, clipped to T */
+int star_kv8_append(const star_kv8_cache* c, const void* k, const void* v, int64_t k_sb, int64_t k_sh, int64_t k_sr,
+                    int64_t v_sb, int64_t v_sh, int64_t v_sr, const int32_t* starts, const int32_t* counts,
+                    int idx_stride, const int32_t* at, int max_rows, void* stream);
+
+/* o = softmax(scale q k^T + bias) v over the tokens held; q [B,H,L,hd] and o by strides as above, query head h on key
+ * head h / (H / Hkv).  q_len [B] or NULL: queries of sequence b (at most L; rows behind them give 0).
+ *   causal: query i sees the tokens j <= lens[b] - q_len[b] + i (the queries are the newest tokens, already appended)
+ *   ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask, my_transformer.py:566)
+ *   bias [B][bias_len] fp32 or NULL, added to the logits of token j < bias_len (the scorer's logits)
+ * A query that sees nothing, or only biases of -inf (or so low that bias * log2(e) overflows), gives 0.
+ * workspace: star_kv8_attn_workspace(c, H, L) bytes, used by this call only. */
+typedef struct {
+    int H, L;
+    int64_t q_sb, q_sh, q_sr, o_sb, o_sh, o_sr;
+    int bias_len, causal, ilk_diag;
+    float scale;
+} star_kv8_query;
+size_t star_kv8_attn_workspace(const star_kv8_cache* c, int H, int L);
+int star_kv8_attn(const star_kv8_cache* c, const void* q, const float* bias, const int32_t* q_len,
+                  const star_kv8_query* s, void* o, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,27 @@ class XAttnShape(C.Structure):
                 ("dropout_p", C.c_float), ("seed", C.c_uint64), ("offset", C.c_uint64), ("rng_state", C.c_void_p)]
 
 
+class CausalShape(C.Structure):
+    _fields_ = [("H", C.c_int), ("Hkv", C.c_int), ("hd", C.c_int), ("dtype", C.c_int), ("nseq", C.c_int),
+                ("q_sr", C.c_int64), ("q_sh", C.c_int64), ("k_sr", C.c_int64), ("k_sh", C.c_int64),
+                ("v_sr", C.c_int64), ("v_sh", C.c_int64), ("o_sr", C.c_int64), ("o_sh", C.c_int64),
+                ("lse_stride", C.c_int64), ("scale", C.c_float)]
+
+
+class KV8Cache(C.Structure):
+    _fields_ = [("B", C.c_int), ("Hkv", C.c_int), ("T", C.c_int), ("hd", C.c_int), ("dtype", C.c_int),
+                ("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+                ("k_tail", C.c_void_p), ("v_tail", C.c_void_p), ("lens", C.c_void_p), ("dropped", C.c_void_p),
+                ("tickets", C.c_void_p)]
+
+
+class KV8Query(C.Structure):
+    _fields_ = [("H", C.c_int), ("L", C.c_int),
+                ("q_sb", C.c_int64), ("q_sh", C.c_int64), ("q_sr", C.c_int64),
+                ("o_sb", C.c_int64), ("o_sh", C.c_int64), ("o_sr", C.c_int64),
+                ("bias_len", C.c_int), ("causal", C.c_int), ("ilk_diag", C.c_int), ("scale", C.c_float)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _I64 = C.c_int64
@@ -82,6 +103,11 @@ SIGNATURES = {
     "star_colsum_workspace": (_SZ, [_I64, _I]),
     "star_colsum": (_I, [_P, _I, _I64, _I, _I64, _P, _P, _SZ, _P]),
     "star_colsum_batched": (_I, [C.POINTER(C.c_void_p), _I, _I, _I64, _I, _I64, _P, _P, _SZ, _P]),
+    "star_causal_fwd": (_I, [_P, _P, _P, _P, _P, _I, C.POINTER(CausalShape), _P, _P, _P]),
+    "star_causal_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, C.POINTER(CausalShape), _P, _P, _P, _P, _P]),
+    "star_kv8_append": (_I, [C.POINTER(KV8Cache), _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I, _P, _I, _P]),
+    "star_kv8_attn_workspace": (_SZ, [C.POINTER(KV8Cache), _I, _I]),
+    "star_kv8_attn": (_I, [C.POINTER(KV8Cache), _P, _P, _P, C.POINTER(KV8Query), _P, _P, _SZ, _P]),
     "star_xattn_fwd": (_I, [_P, _P, _P, _P, _P, C.POINTER(XAttnShape), _P, _P, _P, _P]),
     "star_xattn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, C.POINTER(XAttnShape), _P, _P, _P, _P, _P, _P, _I, _P]),
 }

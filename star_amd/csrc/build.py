@@ -11,7 +11,8 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["error.cpp", "select.hip", "gather.hip", "harness.hip", "cif.hip", "cifagg.hip", "typeembed.hip", "gatherln.hip", "gemm.hip", "xattn.hip", "xattn_bwd4.hip"]
+SOURCES = ["error.cpp", "select.hip", "gather.hip", "harness.hip", "cif.hip", "cifagg.hip", "typeembed.hip", "gatherln.hip", "gemm.hip", "xattn.hip", "xattn_bwd4.hip",
+           "causal.hip", "kv8.hip"]
 LIB = os.path.join(HERE, "libstar_nugget.so")
 # (packed fp32 arithmetic is off: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this hardware; the
 # host pass warns that it does not know the feature, which is harmless)
@@ -76,7 +77,7 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    deps = [os.path.join(HERE, "common.h"), os.path.join(HERE, "xattn_drop.h"), os.path.join(HERE, "gemm_nt4.h"),
+    deps = [os.path.join(HERE, "common.h"), os.path.join(HERE, "xattn_drop.h"), os.path.join(HERE, "gemm_nt4.h"), os.path.join(HERE, "causal.h"),
             os.path.join(HERE, "..", "..", "include", "star_nugget.h"), os.path.join(HERE, "..", "..", "include", "star_harness.h")]
     jobs = []
     objs = []

@@ -1,0 +1,557 @@
+// Causal self-attention of packed sequences, forward and backward (star_causal_* in star_nugget.h).
+//
+//   S = scale Q K^T over the keys j <= i + nk - nq,  P = softmax(S),  O = P V
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Both directions walk tiles of 64 rows of the other side with a running maximum and sum (forward) or the stored
+// log-sum-exp (backward); no [nq, nk] tensor exists.  Two products per pair of rows forward, seven backward (the
+// gradients of the queries and of the keys are two kernels, each recomputing P and dP in the order it needs: no
+// atomics, the result does not depend on the order in which workgroups run).
+//
+// One operand of every product stays in registers, the other is read from LDS, where a 16-bit tile is read by rows or
+// transposed from the same copy (Tile in causal.h).  The softmax side has the query on the MFMA column, so maximum and
+// sum of a row are in-lane but for two shuffles, and the accumulator of S^T is, packed to 16 bits, the next operand.
+#include "causal.h"
+
+namespace star {
+
+constexpr int CT = STAR_CAUSAL_TILE;     // rows of one workgroup: 4 waves x 32
+constexpr int CK = 64;                   // rows of the tiles it walks
+
+struct SeqOf { int q0, nq, k0, nk; };
+__device__ __forceinline__ SeqOf seq_of(const int32_t* seqs, int s) {
+    return SeqOf{seqs[4 * s], seqs[4 * s + 1], seqs[4 * s + 2], seqs[4 * s + 3]};
+}
+
+// ------------------------------------------------------------------------------------------------------ forward
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                           const T* __restrict__ V, const int32_t* __restrict__ seqs,
+                                                           const int32_t* __restrict__ tiles, star_causal_shape s,
+                                                           T* __restrict__ O, float* __restrict__ lse) {
+    typedef typename Vec<T>::x8 x8;
+    typedef typename Vec<T>::x4 x4;
+    using Ti = Tile<T, HD>;
+    constexpr int KS = HD / 32, NT = HD / 16;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    constexpr int TB = CK * Ti::ROWB;
+
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    // consecutive workgroups go to consecutive XCDs: key heads first, so that the tiles and query heads that share a
+    // key head meet in one L2 when Hkv is a multiple of 8
+    const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
+    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const int i0 = tiles[2 * t + 1];                               // first query of the workgroup
+    const int off = sq.nk - sq.nq;
+    const T* Qh = Q + (int64_t)sq.q0 * s.q_sr + (int64_t)h * s.q_sh;
+    const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
+    const T* Vh = V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh;
+
+    const int w0 = i0 + 32 * wid;                                  // first query of the wave
+    int lim[2];                                                    // keys that this lane's query of block qb sees
+    x8 qf[2][KS];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+        const int i = w0 + 16 * qb + r16;
+        lim[qb] = i < sq.nq ? max(0, min(sq.nk, i + off + 1)) : 0;
+        const T* row = Qh + (int64_t)min(i, sq.nq - 1) * s.q_sr + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[qb][ks] = *(const x8*)(row + 32 * ks);
+    }
+    const int all_see = w0 + 32 <= sq.nq ? max(0, min(sq.nk, w0 + off + 1)) : 0;   // keys that every query of the wave sees
+    const int wave_end = w0 < sq.nq ? max(0, min(sq.nk, min(w0 + 32, sq.nq) + off)) : 0;
+    const int end = max(0, min(sq.nk, min(i0 + CT, sq.nq) + off)); // keys that any query of the workgroup sees
+    const float c2 = s.scale * A_LOG2E;
+
+    f32x4 oacc[2][NT];
+    float m[2], l[2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) oacc[qb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        m[qb] = M_NONE;
+        l[qb] = 0.f;
+    }
+
+    TileLoad<T, HD, CK, 256> kl, vl;
+    const int ntile = (end + CK - 1) / CK;
+    if (ntile > 0) {
+        kl.load(Kh, s.k_sr, 0, sq.nk, tid);
+        vl.load(Vh, s.v_sr, 0, sq.nk, tid);
+    }
+#pragma unroll 1
+    for (int tile = 0; tile < ntile; ++tile) {
+        uint8_t* kt = smem + (tile & 1) * 2 * TB;
+        uint8_t* vt = kt + TB;
+        kl.store(kt, tid);                                         // (the tile two before is done: barrier of the last step)
+        vl.store(vt, tid);
+        __syncthreads();
+        if (tile + 1 < ntile) {
+            kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
+            vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
+        }
+        const int key0 = tile * CK;
+        if (key0 >= wave_end) continue;                            // (wave-uniform)
+
+        f32x4 sc[2][4];
+#pragma unroll
+        for (int kt4 = 0; kt4 < 4; ++kt4) {
+            x8 kf[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kf[ks] = Ti::row8(kt, 16 * kt4, ks, lane);
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                sc[qb][kt4] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) sc[qb][kt4] = mfma16(kf[ks], qf[qb][ks], sc[qb][kt4]);
+            }
+        }
+        const bool masked = key0 + CK > all_see;
+        x8 pf[2][2];
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            float mx = M_NONE;
+#pragma unroll
+            for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = sc[qb][kt4][i] * c2;
+                    if (masked && key0 + 16 * kt4 + 4 * g + i >= lim[qb]) x = -INFINITY;
+                    sc[qb][kt4][i] = x;
+                    mx = fmaxf(mx, x);
+                }
+            if (!__all(mx <= m[qb] + M_SLACK)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m[qb], mx), a = __builtin_amdgcn_exp2f(m[qb] - mn);
+                m[qb] = mn;
+                l[qb] *= a;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) oacc[qb][nt][i] *= a;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(sc[qb][kt4][i] - m[qb]);
+                    sum += p;
+                    sc[qb][kt4][i] = p;
+                }
+            l[qb] += sum;
+            pf[qb][0] = pack_b<T>(sc[qb][0], sc[qb][1]);
+            pf[qb][1] = pack_b<T>(sc[qb][2], sc[qb][3]);
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const x8 vf = Ti::tr8(vt, 32 * hf, nt, lane);
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb) oacc[qb][nt] = mfma16(vf, pf[qb][hf], oacc[qb][nt]);
+            }
+    }
+
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+        float sum = l[qb];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        const int i = w0 + 16 * qb + r16;
+        if (i >= sq.nq) continue;
+        const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   // no visible key: 0; NaN stays NaN
+        T* orow = O + (int64_t)(sq.q0 + i) * s.o_sr + (int64_t)h * s.o_sh + 4 * g;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            x4 o4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o4[e] = (T)(oacc[qb][nt][e] * inv);
+            *(x4*)(orow + 16 * nt) = o4;
+        }
+        if (g == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = sum == 0.f ? -INFINITY : m[qb] * A_LN2 + logf(sum);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ gradient of Q
+// The forward's walk with dP^T = V dO^T beside S^T = K Q^T; dQ^T += K^T dS^T with K read transposed from the same tile.
+// Also writes delta = rowsum(dO O) for the kernel below.
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                          const T* __restrict__ V, const T* __restrict__ O,
+                                                          const T* __restrict__ dO, const float* __restrict__ lse,
+                                                          const int32_t* __restrict__ seqs,
+                                                          const int32_t* __restrict__ tiles, star_causal_shape s,
+                                                          T* __restrict__ dQ, float* __restrict__ delta) {
+    typedef typename Vec<T>::x8 x8;
+    typedef typename Vec<T>::x4 x4;
+    using Ti = Tile<T, HD>;
+    constexpr int KS = HD / 32, NT = HD / 16;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    constexpr int TB = CK * Ti::ROWB;
+
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
+    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const int i0 = tiles[2 * t + 1];
+    const int off = sq.nk - sq.nq;
+    const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
+    const T* Vh = V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh;
+
+    const int w0 = i0 + 32 * wid;
+    int lim[2];
+    float l2[2], dl[2];
+    x8 qf[2][KS], gf[2][KS];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+        const int i = w0 + 16 * qb + r16;
+        const int64_t row = sq.q0 + min(i, sq.nq - 1);
+        lim[qb] = i < sq.nq ? max(0, min(sq.nk, i + off + 1)) : 0;
+        const T* qr = Q + row * s.q_sr + (int64_t)h * s.q_sh + 8 * g;
+        const T* gr = dO + row * s.o_sr + (int64_t)h * s.o_sh + 8 * g;
+        const T* orow = O + row * s.o_sr + (int64_t)h * s.o_sh + 8 * g;
+        float sum = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            qf[qb][ks] = *(const x8*)(qr + 32 * ks);
+            gf[qb][ks] = *(const x8*)(gr + 32 * ks);
+            const x8 of = *(const x8*)(orow + 32 * ks);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += (float)gf[qb][ks][e] * (float)of[e];
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        dl[qb] = sum;
+        l2[qb] = lse[(int64_t)h * s.lse_stride + row] * A_LOG2E;
+        if (g == 0 && i < sq.nq) delta[(int64_t)h * s.lse_stride + row] = sum;
+    }
+    const int all_see = w0 + 32 <= sq.nq ? max(0, min(sq.nk, w0 + off + 1)) : 0;
+    const int wave_end = w0 < sq.nq ? max(0, min(sq.nk, min(w0 + 32, sq.nq) + off)) : 0;
+    const int end = max(0, min(sq.nk, min(i0 + CT, sq.nq) + off));
+    const float c2 = s.scale * A_LOG2E;
+
+    f32x4 acc[2][NT];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[qb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    TileLoad<T, HD, CK, 256> kl, vl;
+    const int ntile = (end + CK - 1) / CK;
+    if (ntile > 0) {
+        kl.load(Kh, s.k_sr, 0, sq.nk, tid);
+        vl.load(Vh, s.v_sr, 0, sq.nk, tid);
+    }
+#pragma unroll 1
+    for (int tile = 0; tile < ntile; ++tile) {
+        uint8_t* kt = smem + (tile & 1) * 2 * TB;
+        uint8_t* vt = kt + TB;
+        kl.store(kt, tid);
+        vl.store(vt, tid);
+        __syncthreads();
+        if (tile + 1 < ntile) {
+            kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
+            vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
+        }
+        const int key0 = tile * CK;
+        if (key0 >= wave_end) continue;
+        const bool masked = key0 + CK > all_see;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {                           // 32 keys at a time
+            f32x4 ds[2][2];
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+                f32x4 sc[2], dp[2];
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb) sc[qb] = dp[qb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const x8 kf = Ti::row8(kt, 32 * hf + 16 * k2, ks, lane);
+                    const x8 vf = Ti::row8(vt, 32 * hf + 16 * k2, ks, lane);
+#pragma unroll
+                    for (int qb = 0; qb < 2; ++qb) {
+                        sc[qb] = mfma16(kf, qf[qb][ks], sc[qb]);
+                        dp[qb] = mfma16(vf, gf[qb][ks], dp[qb]);
+                    }
+                }
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool hide = masked && key0 + 32 * hf + 16 * k2 + 4 * g + i >= lim[qb];
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][i], c2, -l2[qb]));
+                        ds[qb][k2][i] = hide ? 0.f : p * (dp[qb][i] - dl[qb]);
+                    }
+            }
+            x8 df[2];
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) df[qb] = pack_b<T>(ds[qb][0], ds[qb][1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const x8 kf = Ti::tr8(kt, 32 * hf, nt, lane);
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb) acc[qb][nt] = mfma16(kf, df[qb], acc[qb][nt]);
+            }
+        }
+    }
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+        const int i = w0 + 16 * qb + r16;
+        if (i >= sq.nq) continue;
+        T* row = dQ + ((int64_t)(sq.q0 + i) * s.H + h) * HD + 4 * g;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            x4 o4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o4[e] = (T)(acc[qb][nt][e] * s.scale);
+            *(x4*)(row + 16 * nt) = o4;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ gradients of K, V
+// One workgroup: 128 keys of one key head, 32 per wave with K, V, dK^T and dV^T in registers; it walks the queries of
+// every query head of the group in tiles of 64.  The key is on the MFMA column, so P and dS come out as the operands of
+// dV^T += dO^T P and dK^T += Q^T dS.
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 1) void causal_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                           const T* __restrict__ V, const T* __restrict__ dO,
+                                                           const float* __restrict__ lse, const float* __restrict__ delta,
+                                                           const int32_t* __restrict__ seqs,
+                                                           const int32_t* __restrict__ tiles, star_causal_shape s,
+                                                           T* __restrict__ dK, T* __restrict__ dV) {
+    typedef typename Vec<T>::x8 x8;
+    typedef typename Vec<T>::x4 x4;
+    using Ti = Tile<T, HD>;
+    constexpr int KS = HD / 32, NT = HD / 16;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    constexpr int TB = CK * Ti::ROWB, SB = 2 * TB + 2 * CK * 4;    // Q | dO | lse | delta
+
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % s.Hkv, t = blockIdx.x / s.Hkv, grp = s.H / s.Hkv;
+    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const int j0 = tiles[2 * t + 1], w0 = j0 + 32 * wid;           // first key of the workgroup, of the wave
+    const int off = sq.nk - sq.nq;
+
+    x8 kf[2][KS], vf[2][KS];
+    int see[2];                                                    // first query that sees this lane's key
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const int j = w0 + 16 * kb + r16;
+        const int64_t row = sq.k0 + min(j, sq.nk - 1);
+        see[kb] = j < sq.nk ? j - off : 0x7fffffff;
+        const T* kr = K + row * s.k_sr + (int64_t)hk * s.k_sh + 8 * g;
+        const T* vr = V + row * s.v_sr + (int64_t)hk * s.v_sh + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            kf[kb][ks] = *(const x8*)(kr + 32 * ks);
+            vf[kb][ks] = *(const x8*)(vr + 32 * ks);
+        }
+    }
+    f32x4 dk[2][NT], dv[2][NT];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) dk[kb][nt] = dv[kb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const float c2 = s.scale * A_LOG2E;
+    const int first = max(0, j0 - off) / CK;                       // query tiles before it see none of these keys
+    const int nper = max(0, (sq.nq + CK - 1) / CK - first);        // tiles per head
+    const int all_see = w0 + 32 <= sq.nk ? w0 + 31 - off : 0x7fffffff;  // from this query on every key of the wave is visible
+
+    TileLoad<T, HD, CK, 256> ql, gl;
+    float lr = 0.f;
+    auto load = [&](int n) {
+        const int h = hk * grp + n / nper, q0 = (first + n % nper) * CK;
+        ql.load(Q + (int64_t)sq.q0 * s.q_sr + (int64_t)h * s.q_sh, s.q_sr, q0, sq.nq, tid);
+        gl.load(dO + (int64_t)sq.q0 * s.o_sr + (int64_t)h * s.o_sh, s.o_sr, q0, sq.nq, tid);
+        if (tid < 2 * CK) lr = (tid < CK ? lse : delta)[(int64_t)h * s.lse_stride + sq.q0 + min(q0 + (tid & (CK - 1)), sq.nq - 1)];
+    };
+    const int ntile = nper * grp;
+    if (ntile > 0) load(0);
+#pragma unroll 1
+    for (int n = 0; n < ntile; ++n) {
+        uint8_t* qt = smem + (n & 1) * SB;
+        uint8_t* gt = qt + TB;
+        float* lt = (float*)(gt + TB);
+        ql.store(qt, tid);
+        gl.store(gt, tid);
+        if (tid < CK) lt[tid] = lr * A_LOG2E;
+        else if (tid < 2 * CK) lt[tid] = lr;
+        __syncthreads();
+        if (n + 1 < ntile) load(n + 1);
+        const int q0 = (first + n % nper) * CK;
+        if (q0 + CK <= w0 - off) continue;                         // (wave-uniform) no query of the tile sees a key of the wave
+        const bool masked = q0 < all_see || q0 + CK > sq.nq;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {                           // 32 queries at a time
+            f32x4 pp[2][2], ds[2][2];
+#pragma unroll
+            for (int q2 = 0; q2 < 2; ++q2) {
+                f32x4 sc[2], dp[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) sc[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const x8 qa = Ti::row8(qt, 32 * hf + 16 * q2, ks, lane);
+                    const x8 ga = Ti::row8(gt, 32 * hf + 16 * q2, ks, lane);
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+                        sc[kb] = mfma16(qa, kf[kb][ks], sc[kb]);
+                        dp[kb] = mfma16(ga, vf[kb][ks], dp[kb]);
+                    }
+                }
+                const f32x4 ls = *(const f32x4*)(lt + 32 * hf + 16 * q2 + 4 * g);
+                const f32x4 de = *(const f32x4*)(lt + CK + 32 * hf + 16 * q2 + 4 * g);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int qi = q0 + 32 * hf + 16 * q2 + 4 * g + i;
+                        const bool hide = masked && (qi < see[kb] || qi >= sq.nq);
+                        const float p = hide ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i], c2, -ls[i]));
+                        pp[kb][q2][i] = p;
+                        ds[kb][q2][i] = hide ? 0.f : p * (dp[kb][i] - de[i]);
+                    }
+            }
+            x8 pf[2], df[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                pf[kb] = pack_b<T>(pp[kb][0], pp[kb][1]);
+                df[kb] = pack_b<T>(ds[kb][0], ds[kb][1]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const x8 ga = Ti::tr8(gt, 32 * hf, nt, lane);
+                const x8 qa = Ti::tr8(qt, 32 * hf, nt, lane);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    dv[kb][nt] = mfma16(ga, pf[kb], dv[kb][nt]);
+                    dk[kb][nt] = mfma16(qa, df[kb], dk[kb][nt]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const int j = w0 + 16 * kb + r16;
+        if (j >= sq.nk) continue;
+        const int64_t at = ((int64_t)(sq.k0 + j) * s.Hkv + hk) * HD + 4 * g;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            x4 a, b;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = (T)(dk[kb][nt][e] * s.scale);
+                b[e] = (T)dv[kb][nt][e];
+            }
+            *(x4*)(dK + at + 16 * nt) = a;
+            *(x4*)(dV + at + 16 * nt) = b;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ host side
+static int check_causal(const star_causal_shape* s, const char* who) {
+    STAR_REQUIRE(s, "%s: null shape", who);
+    STAR_REQUIRE(s->hd == 64 || s->hd == 96 || s->hd == 128, "%s: head dim %d not in {64, 96, 128}", who, s->hd);
+    STAR_REQUIRE(s->dtype == STAR_DT_BF16 || s->dtype == STAR_DT_F16, "%s: dtype %d is neither bf16 nor fp16", who, s->dtype);
+    STAR_REQUIRE(s->Hkv >= 1 && s->H >= s->Hkv && s->H % s->Hkv == 0, "%s: %d query heads do not divide into %d key heads", who, s->H, s->Hkv);
+    STAR_REQUIRE(s->nseq >= 0 && s->lse_stride >= 0, "%s: negative size", who);
+    const int64_t st[8] = {s->q_sr, s->q_sh, s->k_sr, s->k_sh, s->v_sr, s->v_sh, s->o_sr, s->o_sh};
+    for (int i = 0; i < 8; ++i) STAR_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    return STAR_OK;
+}
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename T, int HD>
+static int launch_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+                             int ntiles, const star_causal_shape* s, void* o, float* lse, hipStream_t st) {
+    constexpr int smem = 4 * CK * Tile<T, HD>::ROWB;
+    static DevOnce once;
+    if (!reserve_lds_once(once, (const void*)causal_fwd_kernel<T, HD>, smem)) {
+        set_error("star_causal_fwd: cannot reserve %d bytes of LDS", smem);
+        return STAR_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL((causal_fwd_kernel<T, HD>), dim3((unsigned)ntiles * s->H), dim3(256), smem, st, (const T*)q, (const T*)k,
+                       (const T*)v, seqs, tiles, *s, (T*)o, lse);
+    return STAR_OK;
+}
+
+template <typename T, int HD>
+static int launch_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
+                             const int32_t* seqs, const int32_t* q_tiles, int nq_tiles, const int32_t* k_tiles,
+                             int nk_tiles, const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta,
+                             hipStream_t st) {
+    constexpr int smem_q = 4 * CK * Tile<T, HD>::ROWB, smem_k = 2 * (2 * CK * Tile<T, HD>::ROWB + 2 * CK * 4);
+    static DevOnce once_q, once_k;
+    if (!reserve_lds_once(once_q, (const void*)causal_dq_kernel<T, HD>, smem_q) ||
+        !reserve_lds_once(once_k, (const void*)causal_dkv_kernel<T, HD>, smem_k)) {
+        set_error("star_causal_bwd: cannot reserve %d bytes of LDS", smem_k);
+        return STAR_ERR_LAUNCH;
+    }
+    if (nq_tiles > 0)
+        hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3((unsigned)nq_tiles * s->H), dim3(256), smem_q, st, (const T*)q,
+                           (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, seqs, q_tiles, *s, (T*)dq, delta);
+    if (nk_tiles > 0)
+        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)nk_tiles * s->Hkv), dim3(256), smem_k, st, (const T*)q,
+                           (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, seqs, k_tiles, *s, (T*)dk,
+                           (T*)dv);
+    return STAR_OK;
+}
+
+#define CAUSAL_BY_TYPE(CALL)                                         \
+    do {                                                             \
+        if (s->dtype == STAR_DT_BF16) {                              \
+            if (s->hd == 64) { using T = __bf16; constexpr int HD = 64; rc = CALL; }       \
+            else if (s->hd == 96) { using T = __bf16; constexpr int HD = 96; rc = CALL; }  \
+            else { using T = __bf16; constexpr int HD = 128; rc = CALL; }                  \
+        } else {                                                     \
+            if (s->hd == 64) { using T = _Float16; constexpr int HD = 64; rc = CALL; }      \
+            else if (s->hd == 96) { using T = _Float16; constexpr int HD = 96; rc = CALL; } \
+            else { using T = _Float16; constexpr int HD = 128; rc = CALL; }                 \
+        }                                                            \
+    } while (0)
+
+}  // namespace star
+
+extern "C" int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+                               int ntiles, const star_causal_shape* s, void* o, float* lse, void* stream) {
+    using namespace star;
+    int rc = check_causal(s, "star_causal_fwd");
+    if (rc) return rc;
+    STAR_REQUIRE(ntiles >= 0 && (int64_t)ntiles * s->H < (1ll << 31), "star_causal_fwd: %d tiles x %d heads", ntiles, s->H);
+    if (ntiles == 0) return STAR_OK;
+    STAR_REQUIRE(q && k && v && seqs && tiles && o && lse, "star_causal_fwd: null pointer");
+    STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "star_causal_fwd: tensors must be 16-byte aligned");
+    CAUSAL_BY_TYPE((launch_causal_fwd<T, HD>(q, k, v, seqs, tiles, ntiles, s, o, lse, (hipStream_t)stream)));
+    if (rc) return rc;
+    STAR_LAUNCH_CHECK("star_causal_fwd");
+    return STAR_OK;
+}
+
+extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_,
+                               const float* lse, const int32_t* seqs, const int32_t* q_tiles, int nq_tiles,
+                               const int32_t* k_tiles, int nk_tiles, const star_causal_shape* s, void* dq, void* dk,
+                               void* dv, float* delta, void* stream) {
+    using namespace star;
+    int rc = check_causal(s, "star_causal_bwd");
+    if (rc) return rc;
+    STAR_REQUIRE(nq_tiles >= 0 && nk_tiles >= 0 && (int64_t)nq_tiles * s->H < (1ll << 31) && (int64_t)nk_tiles * s->H < (1ll << 31),
+                 "star_causal_bwd: %d and %d tiles x %d heads", nq_tiles, nk_tiles, s->H);
+    if (nq_tiles == 0 && nk_tiles == 0) return STAR_OK;
+    STAR_REQUIRE(q && k && v && o && do_ && lse && seqs && (q_tiles || !nq_tiles) && (k_tiles || !nk_tiles) && dq && dk && dv && delta,
+                 "star_causal_bwd: null pointer");
+    STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(do_) && aligned16(dq) && aligned16(dk) && aligned16(dv),
+                 "star_causal_bwd: tensors must be 16-byte aligned");
+    CAUSAL_BY_TYPE((launch_causal_bwd<T, HD>(q, k, v, o, do_, lse, seqs, q_tiles, nq_tiles, k_tiles, nk_tiles, s, dq, dk, dv,
+                                             delta, (hipStream_t)stream)));
+    if (rc) return rc;
+    STAR_LAUNCH_CHECK("star_causal_bwd");
+    return STAR_OK;
+}

@@ -6,15 +6,17 @@ the STAR checkout (src/models/...).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import XAttnShape, check, lib, ptr, stream_ptr
+from ._lib import CausalShape, KV8Cache, KV8Query, XAttnShape, check, lib, ptr, stream_ptr
 
 DT_BF16, DT_F32 = 0, 1
 
@@ -1551,6 +1553,378 @@ def xattn(q, k, v, bias=None, key_len=None, ilk_diag: int = -1, scale: Optional[
         raise ValueError(f"xattn: dropout_p = {dropout_p} not in [0, 1)")
     return _XAttn.apply(q, k, v, bias, key_len, int(ilk_diag), float(scale), bool(need_probs), float(dropout_p),
                         dropout_rng, kv_grad)
+
+
+# ----------------------------------------------------------------------------- self-attention of packed sequences
+DT_F16 = 2
+_DT16 = {torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+CAUSAL_TILE = 128                 # STAR_CAUSAL_TILE
+
+
+def _on(dev):
+    """The device of the tensors as the current one (and with it the stream that stream_ptr() gives)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _same_device(what, **ts):
+    dev = None
+    for name, t in ts.items():
+        if t is None:
+            continue
+        _need_cuda(t)
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, the others on {dev}")
+        dev = t.device
+    return dev
+
+
+def _check_rows(what, name, t):
+    """What the 16-byte loads of the kernels need of a [.., hd] operand."""
+    if t.dtype not in _DT16:
+        raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16 or float16 is required")
+    if t.shape[-1] not in (64, 96, 128):
+        raise ValueError(f"{what}: head dim {t.shape[-1]} not in (64, 96, 128)")
+    if t.numel() and t.stride(-1) != 1:
+        raise ValueError(f"{what}: {name} must have a contiguous head dimension")
+    if t.data_ptr() % 16 or any(st % 8 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        raise ValueError(f"{what}: {name} must be 16-byte aligned in every row")
+
+
+class PackedSeqs:
+    """Host-known lengths of a batch of sequences, prepared once for causal_attn and kv8_append: where every sequence
+    lies and the list of tiles, longest first, that the kernels start in that order.  Built from host lists, so using it
+    costs no device->host sync (HIP-graph safe).
+
+    lengths: keys of every sequence.  q_lengths: its queries where there are fewer (they are the newest positions: query
+    i sees the keys j <= i + lengths[s] - q_lengths[s]); more queries than keys are allowed, the first then see nothing.
+    Sequences lie one behind the other; with padded_to=T sequence s starts at row s * T instead (a padded [B,T] batch,
+    flattened), for the queries too."""
+
+    def __init__(self, lengths: Sequence[int], device, q_lengths: Optional[Sequence[int]] = None,
+                 padded_to: Optional[int] = None):
+        nk = np.asarray(list(lengths), dtype=np.int64).reshape(-1)
+        nq = nk if q_lengths is None else np.asarray(list(q_lengths), dtype=np.int64).reshape(-1)
+        if nq.size != nk.size:
+            raise ValueError(f"PackedSeqs: {nq.size} query lengths for {nk.size} sequences")
+        if nk.size and min(nk.min(), nq.min()) < 0:
+            raise ValueError("PackedSeqs: negative length")
+        if padded_to is not None and nk.size and max(nk.max(), nq.max()) > padded_to:
+            raise ValueError(f"PackedSeqs: a length exceeds padded_to = {padded_to}")
+
+        def place(n):
+            if padded_to is not None:
+                return np.arange(n.size, dtype=np.int64) * int(padded_to)
+            return np.concatenate([np.zeros(1, np.int64), np.cumsum(n)[:-1]]) if n.size else n
+
+        q0, k0 = place(nq), place(nk)
+        # rows that tensors have to have, and rows that belong to a sequence
+        self.q_rows = int((q0 + nq).max()) if nk.size else 0
+        self.k_rows = int((k0 + nk).max()) if nk.size else 0
+        self.q_used, self.k_used = int(nq.sum()), int(nk.sum())
+        if max(self.q_rows, self.k_rows) >= 2 ** 31:
+            raise ValueError("PackedSeqs: more than 2^31 - 1 rows")
+        self.n, self.max_q, self.max_k = int(nk.size), int(nq.max(initial=0)), int(nk.max(initial=0))
+
+        def tiles(n, work):
+            per = -(-n // CAUSAL_TILE)
+            seq = np.repeat(np.arange(n.size, dtype=np.int64), per)
+            first = (np.arange(seq.size, dtype=np.int64) - np.repeat(np.cumsum(per) - per, per)) * CAUSAL_TILE
+            order = np.argsort(-work(seq, first), kind="stable")
+            return np.stack([seq[order], first[order]], 1)
+
+        qt = tiles(nq, lambda s, i: np.clip(np.minimum(i + CAUSAL_TILE, nq[s]) + nk[s] - nq[s], 0, nk[s]))
+        kt = tiles(nk, lambda s, j: nq[s] - np.clip(j - (nk[s] - nq[s]), 0, nq[s]))
+        seqs = np.stack([q0, nq, k0, nk], 1)
+        flat = np.concatenate([seqs.ravel(), qt.ravel(), kt.ravel()]).astype(np.int32)
+        buf = torch.from_numpy(flat).to(device)
+        self.device = buf.device
+        a, b = seqs.size, seqs.size + qt.size
+        self.seqs, self.q_tiles, self.k_tiles = buf[:a].view(-1, 4), buf[a:b].view(-1, 2), buf[b:].view(-1, 2)
+        self.starts, self.counts = self.seqs[:, 2], self.seqs[:, 3]
+
+
+def _causal_shape(q, k, v, o, plan, scale):
+    s = CausalShape()
+    s.H, s.Hkv, s.hd, s.dtype, s.nseq = q.shape[1], k.shape[1], q.shape[2], _DT16[q.dtype], plan.n
+    s.q_sr, s.q_sh, s.k_sr, s.k_sh = q.stride(0), q.stride(1), k.stride(0), k.stride(1)
+    s.v_sr, s.v_sh, s.o_sr, s.o_sh = v.stride(0), v.stride(1), o.stride(0), o.stride(1)
+    # (the stride of a dimension of size 1 is never used, and may be anything)
+    if q.shape[1] == 1:
+        s.q_sh = s.o_sh = 0
+    if k.shape[1] == 1:
+        s.k_sh = s.v_sh = 0
+    if q.shape[0] == 1:
+        s.q_sr = s.o_sr = 0
+    if k.shape[0] == 1:
+        s.k_sr = s.v_sr = 0
+    s.lse_stride, s.scale = q.shape[0], float(scale)
+    return s
+
+
+def _rows_like(rows, used, heads, hd, t):
+    """[rows, heads, hd] for a kernel that writes the rows of the sequences; rows in no sequence are 0."""
+    make = torch.empty if rows == used else torch.zeros
+    return make((rows, heads, hd), dtype=t.dtype, device=t.device)
+
+
+class _CausalAttn(torch.autograd.Function):
+    """softmax(scale Q K^T, j <= i + nk - nq) V of packed sequences."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, plan, scale):
+        q, k, v = q.detach(), k.detach(), v.detach()
+        with _on(q.device):
+            o = _rows_like(q.shape[0], plan.q_used, q.shape[1], q.shape[2], q)
+            lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+            if plan.q_used != q.shape[0]:
+                lse.fill_(-math.inf)
+            s = _causal_shape(q, k, v, o, plan, scale)
+            check(lib().star_causal_fwd(ptr(q), ptr(k), ptr(v), ptr(plan.seqs), ptr(plan.q_tiles), plan.q_tiles.shape[0], s,
+                                        ptr(o), ptr(lse), stream_ptr()), "star_causal_fwd")
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.plan, ctx.scale = plan, scale
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        if g is None:
+            return None, None, None, None, None
+        q, k, v, o, lse = ctx.saved_tensors
+        plan = ctx.plan
+        with _on(q.device):
+            g = g.to(q.dtype).contiguous()
+            if g.data_ptr() % 16:
+                g = g.clone()
+            dq = _rows_like(q.shape[0], plan.q_used, q.shape[1], q.shape[2], q)
+            dk = _rows_like(k.shape[0], plan.k_used, k.shape[1], k.shape[2], k)
+            dv = _rows_like(k.shape[0], plan.k_used, k.shape[1], k.shape[2], v)
+            delta = torch.empty_like(lse)
+            s = _causal_shape(q, k, v, o, plan, ctx.scale)
+            check(lib().star_causal_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(g), ptr(lse), ptr(plan.seqs),
+                                        ptr(plan.q_tiles), plan.q_tiles.shape[0], ptr(plan.k_tiles), plan.k_tiles.shape[0],
+                                        s, ptr(dq), ptr(dk), ptr(dv), ptr(delta), stream_ptr()), "star_causal_bwd")
+        return dq, dk, dv, None, None
+
+
+def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_lse: bool = False):
+    """Causal attention of packed sequences (the self-attention branch of my_transformer.py:490-603), forward and
+    backward.  q [rows,H,hd], k and v [rows,Hkv,hd], bfloat16 or float16, hd in (64, 96, 128), hd contiguous and rows
+    16-byte aligned (views of one qkv projection are fine); H a multiple of Hkv, query head h reads key head
+    h // (H // Hkv).  plan says where the sequences lie and what a query sees.  scale defaults to hd ** -0.5.
+    Returns o [rows,H,hd]; with need_lse also the natural log-sum-exp of every row's logits, fp32 [H,rows] (not
+    differentiable).  A query that sees no key gives 0 and -inf, and rows in no sequence give 0 and -inf and have zero
+    gradients.  Sums and softmax statistics are fp32; the softmax weights are rounded to the inputs' type for the
+    product with v, and their gradient for the products with q and k.  An infinite or NaN v row reaches up to 63 earlier
+    queries of its own sequence (they share a tile); k and v rows of other sequences or in no sequence reach nobody."""
+    dev = _same_device("causal_attn", q=q, k=k, v=v)
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"causal_attn: [rows, heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError(f"causal_attn: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"causal_attn: q, k and v must share one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"causal_attn: {q.shape[1]} query heads do not divide into {k.shape[1]} key heads")
+    if plan.device != dev:
+        raise ValueError(f"causal_attn: the plan is on {plan.device}, the tensors on {dev}")
+    if q.shape[0] < plan.q_rows or k.shape[0] < plan.k_rows:
+        raise ValueError(f"causal_attn: the plan needs {plan.q_rows} query and {plan.k_rows} key rows, got {q.shape[0]} and {k.shape[0]}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check_rows("causal_attn", name, t)
+    o, lse = _CausalAttn.apply(q, k, v, plan, q.shape[2] ** -0.5 if scale is None else float(scale))
+    return (o, lse) if need_lse else o
+
+
+# ----------------------------------------------------------------------------- 8-bit key/value cache
+KV8_BLOCK = 64                    # STAR_KV8_BLOCK
+
+
+class KVCache8:
+    """Keys and values of a batch of sequences in 8 bits, for generation: e4m3 values with one power-of-two scale for
+    each 64 tokens of a head, the newest incomplete 64 in 16 bits (the format is specified in star_nugget.h; what is held
+    does not depend on how the tokens were split into calls).  kv8_append fills it, kv8_attn reads it.
+
+    lens [batch] int32 lives on the device and counts the tokens held; tokens that find no room are dropped and counted
+    (`overflow()`).  Calls on one cache must be ordered on one stream.  Captured calls replay on the cache as it then is."""
+
+    _PARTS = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "lens")
+
+    def __init__(self, batch: int, kv_heads: int, max_tokens: int, head_dim: int, device, dtype=torch.bfloat16):
+        if min(batch, kv_heads, max_tokens) < 1:
+            raise ValueError(f"KVCache8: {batch} sequences x {kv_heads} heads x {max_tokens} tokens")
+        T = -(-int(max_tokens) // KV8_BLOCK) * KV8_BLOCK
+        z = lambda dt, *shape: torch.zeros(shape, dtype=dt, device=device)  # noqa: E731
+        self._take(k_codes=z(torch.uint8, batch, kv_heads, T, head_dim).view(torch.float8_e4m3fn),
+                   k_scales=z(torch.float32, batch, kv_heads, T // KV8_BLOCK),
+                   v_codes=z(torch.uint8, batch, kv_heads, T // KV8_BLOCK, head_dim, KV8_BLOCK).view(torch.float8_e4m3fn),
+                   v_scales=z(torch.float32, batch, kv_heads, T // KV8_BLOCK),
+                   k_tail=z(dtype, batch, kv_heads, KV8_BLOCK, head_dim), v_tail=z(dtype, batch, kv_heads, head_dim, KV8_BLOCK),
+                   lens=z(torch.int32, batch))
+
+    @classmethod
+    def from_tensors(cls, **parts):
+        """A cache on existing tensors, those of `tensors()` (not copied)."""
+        self = cls.__new__(cls)
+        self._take(**parts)
+        return self
+
+    def _take(self, **parts):
+        if set(parts) != set(self._PARTS):
+            raise ValueError(f"KVCache8: expected the tensors {self._PARTS}, got {tuple(sorted(parts))}")
+        dev = _same_device("KVCache8", **parts)
+        if parts["k_codes"].dim() != 4:
+            raise ValueError(f"KVCache8: k_codes [batch, heads, tokens, hd] expected, got {tuple(parts['k_codes'].shape)}")
+        B, H, T, hd = parts["k_codes"].shape
+        nb, dt, f8, f32 = T // KV8_BLOCK, parts["k_tail"].dtype, torch.float8_e4m3fn, torch.float32
+        want = dict(k_codes=(f8, (B, H, T, hd)), k_scales=(f32, (B, H, nb)), v_codes=(f8, (B, H, nb, hd, KV8_BLOCK)),
+                    v_scales=(f32, (B, H, nb)), k_tail=(dt, (B, H, KV8_BLOCK, hd)), v_tail=(dt, (B, H, hd, KV8_BLOCK)),
+                    lens=(torch.int32, (B,)))
+        if T % KV8_BLOCK or min(B, H, T) < 1 or hd not in (64, 96, 128):
+            raise ValueError(f"KVCache8: {B} sequences x {H} heads x {T} tokens x {hd}")
+        if dt not in _DT16:
+            raise TypeError(f"KVCache8: dtype {dt}; bfloat16 or float16 is required")
+        for n, (d, shape) in want.items():
+            if parts[n].dtype != d or tuple(parts[n].shape) != shape:
+                raise ValueError(f"KVCache8: {n} must be {d} {shape}, got {parts[n].dtype} {tuple(parts[n].shape)}")
+            if not parts[n].is_contiguous() or parts[n].data_ptr() % 16:
+                raise ValueError(f"KVCache8: {n} must be contiguous and 16-byte aligned")
+        for n, t in parts.items():
+            setattr(self, n, t)
+        self.batch, self.kv_heads, self.capacity, self.head_dim, self.dtype, self.device = B, H, T, hd, dt, dev
+        self._dropped = torch.zeros(B, dtype=torch.int32, device=dev)
+        self._tickets = torch.zeros(B, dtype=torch.int32, device=dev)
+        c = self._c = KV8Cache()
+        c.B, c.Hkv, c.T, c.hd, c.dtype = B, H, T, hd, _DT16[dt]
+        for n in self._PARTS:
+            setattr(c, n, parts[n].data_ptr())
+        c.dropped, c.tickets = self._dropped.data_ptr(), self._tickets.data_ptr()
+
+    def tensors(self):
+        """The cache's own buffers, by name (to save it, or for from_tensors)."""
+        return {n: getattr(self, n) for n in self._PARTS}
+
+    def reset(self, rows=None):
+        """Forget the tokens of the given sequences (bool [batch] or index tensor; default all)."""
+        sel = slice(None) if rows is None else rows
+        self.lens[sel] = 0
+        self._dropped[sel] = 0
+
+    def overflow(self):
+        """[batch] int32: tokens that found no room.  Non-zero = the sequence's end is missing."""
+        return self._dropped
+
+    def values(self):
+        """(k, v) [batch, heads, capacity, hd] fp32: the values that the cache stands for; 0 behind lens."""
+        B, H, T, hd = self.k_codes.shape
+        pos = torch.arange(T, device=self.device)
+        tail = (pos[None] // KV8_BLOCK == self.lens[:, None] // KV8_BLOCK)[:, None, :, None]
+        live = (pos[None] < self.lens[:, None])[:, None, :, None]
+        k = self.k_codes.float() * self.k_scales.repeat_interleave(KV8_BLOCK, 2)[..., None]
+        v = (self.v_codes.float() * self.v_scales[..., None, None]).transpose(3, 4).reshape(B, H, T, hd)
+        k = torch.where(tail, self.k_tail.float()[:, :, pos % KV8_BLOCK], k)
+        v = torch.where(tail, self.v_tail.float().transpose(2, 3)[:, :, pos % KV8_BLOCK], v)
+        return torch.where(live, k, 0.0), torch.where(live, v, 0.0)
+
+
+def _i32(what, t, n, dev):
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what} must be [{n}], got {tuple(t.shape)}")
+    if t.is_floating_point():
+        raise TypeError(f"{what} must hold integers, got {t.dtype}")
+    return t.to(torch.int32).contiguous()
+
+
+@torch.no_grad()
+def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = None, at=None):
+    """Append keys and values to an 8-bit cache.
+
+    k, v [batch, kv_heads, n, hd] (any strides with hd contiguous): n new tokens of every sequence, or the first
+    counts[b] of them (device integers).  Or, with a plan of `batch` sequences, packed rows [rows, kv_heads, hd]: the
+    keys that the plan gives each sequence.  at [batch] (device integers): write at these positions instead of behind
+    the last token -- 0 fills anew, a position in the incomplete block takes tokens back; other positions, whose block is
+    complete, must not be given.  Nothing is differentiated through a cache.  One launch, no host sync."""
+    dev = _same_device("kv8_append", k=k, v=v, counts=counts, at=at, cache=cache.lens)
+    B, H, hd = cache.batch, cache.kv_heads, cache.head_dim
+    if k.shape != v.shape:
+        raise ValueError(f"kv8_append: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    if k.dtype != cache.dtype or v.dtype != cache.dtype:
+        raise TypeError(f"kv8_append: the cache takes {cache.dtype}, got {k.dtype} and {v.dtype}")
+    if plan is None:
+        if k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (B, H, hd):
+            raise ValueError(f"kv8_append: [{B}, {H}, n, {hd}] expected, got {tuple(k.shape)}")
+        st = [k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2)]
+        dims = [B, H, k.shape[2]] * 2
+        counts, starts, step, most = _i32("kv8_append: counts", counts, B, dev), None, 1, k.shape[2]
+    else:
+        if counts is not None:
+            raise ValueError("kv8_append: counts go with a batch, a plan has its own")
+        if k.dim() != 3 or (k.shape[1], k.shape[2]) != (H, hd):
+            raise ValueError(f"kv8_append: [rows, {H}, {hd}] expected, got {tuple(k.shape)}")
+        if plan.n != B or plan.device != dev:
+            raise ValueError(f"kv8_append: a plan of {plan.n} sequences on {plan.device} for a cache of {B} on {dev}")
+        if k.shape[0] < plan.k_rows:
+            raise ValueError(f"kv8_append: the plan needs {plan.k_rows} rows, got {k.shape[0]}")
+        st = [0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0)]
+        dims = [1, H, k.shape[0]] * 2
+        counts, starts, step, most = plan.counts, plan.starts, 4, plan.max_k
+    if most == 0 and at is None:
+        return
+    if k.numel():
+        for name, t in (("k", k), ("v", v)):
+            _check_rows("kv8_append", name, t)
+    st = [s if n > 1 else 0 for s, n in zip(st, dims)]
+    at = _i32("kv8_append: at", at, B, dev)
+    with _on(dev):
+        check(lib().star_kv8_append(cache._c, ptr(k), ptr(v), *st, ptr(starts), ptr(counts), step, ptr(at), most,
+                                    stream_ptr()), "star_kv8_append")
+
+
+def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int = -1, bias=None,
+             scale: Optional[float] = None):
+    """Attention of a few new tokens over an 8-bit cache: q [batch, H, L, hd] in the cache's dtype, H a multiple of the
+    cache's heads.  causal: the queries are the newest tokens, already appended -- query i sees the tokens j <=
+    lens[b] - q_len[b] + i; ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask of xattn).  q_len [batch]
+    (device integers): queries of every sequence, the rows behind them give 0; default L.  bias [batch, n <= capacity]
+    is added to the logits of token j < n.  scale defaults to hd ** -0.5.  A query that sees nothing gives 0.
+    Returns [batch, H, L, hd] (memory order [batch, L, H, hd], as xattn).  Inference only: call it under no_grad.
+    The values that the cache stands for are used as they are; softmax and sums are fp32, the softmax weights are rounded
+    to 16 bits for the product with v.  An infinite or NaN v of a token reaches every query of the sequence that sees a
+    token of its block."""
+    dev = _same_device("kv8_attn", q=q, q_len=q_len, bias=bias, cache=cache.lens)
+    B, hd = cache.batch, cache.head_dim
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"kv8_attn: [{B}, a multiple of {cache.kv_heads}, L, {hd}] expected, got {tuple(q.shape)}")
+    if q.dtype != cache.dtype:
+        raise TypeError(f"kv8_attn: the cache holds {cache.dtype}, q is {q.dtype}")
+    if torch.is_grad_enabled() and (q.requires_grad or (bias is not None and bias.requires_grad)):
+        raise _lib.StarNuggetError("kv8_attn has no backward: call it under torch.no_grad()")
+    H, L = q.shape[1], q.shape[2]
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[0] != B or bias.shape[1] > cache.capacity:
+            raise ValueError(f"kv8_attn: bias [{B}, at most {cache.capacity}] expected, got {tuple(bias.shape)}")
+        bias = bias.detach().to(torch.float32).contiguous()
+    with _on(dev):
+        o = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev).permute(0, 2, 1, 3)
+        if L == 0:
+            return o
+        _check_rows("kv8_attn", "q", q)
+        s = KV8Query()
+        s.H, s.L = H, L
+        s.q_sb, s.q_sh, s.q_sr = (st if n > 1 else 0 for st, n in zip(q.stride()[:3], q.shape[:3]))
+        s.o_sb, s.o_sh, s.o_sr = L * H * hd, hd, H * hd
+        s.bias_len = 0 if bias is None else bias.shape[1]
+        s.causal, s.ilk_diag, s.scale = int(bool(causal)), int(ilk_diag), hd ** -0.5 if scale is None else float(scale)
+        q_len = _i32("kv8_attn: q_len", q_len, B, dev)
+        need = lib().star_kv8_attn_workspace(cache._c, H, L)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        check(lib().star_kv8_attn(cache._c, ptr(q), ptr(bias), ptr(q_len), s, ptr(o), ptr(ws), need, stream_ptr()),
+              "star_kv8_attn")
+    return o
 
 
 def test_override(which: int, value: int) -> int:
