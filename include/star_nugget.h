@@ -493,10 +493,11 @@ int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, 
  * how they were split into calls.
  *   k_codes [B][Hkv][T][hd], k_scales [B][Hkv][T/64]         k_tail [B][Hkv][64][hd]  (row = token % 64)
  *   v_codes [B][Hkv][T/64][hd][64], v_scales [B][Hkv][T/64]  v_tail [B][Hkv][hd][64]  (V is transposed inside a block)
- *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written); tickets [B]: zero before the
- *   first call, zero after every call.  All base addresses multiples of 16 bytes.
+ *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written);
+ *   tickets [B * STAR_KV8_TICKET_STRIDE]: zero before the first call, zero after every call.  All base addresses multiples of 16 bytes.
  * Calls on one cache are ordered by the stream: two appends, or an append and an attention, must not overlap. */
 #define STAR_KV8_BLOCK 64
+#define STAR_KV8_TICKET_STRIDE 32
 typedef struct {
     int B, Hkv, T, hd, dtype;
     uint8_t* k_codes;

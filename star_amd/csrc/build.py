@@ -20,6 +20,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-val
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extras (STAR_XATTN_FLAGS etc. override for experiments)
 EXTRA = {"xattn.hip": os.environ.get("STAR_XATTN_FLAGS", "-mllvm -amdgpu-mfma-vgpr-form=1").split(),
+         "causal.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+         "kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
          "gemm.hip": os.environ.get("STAR_GEMM_FLAGS", "-fno-slp-vectorize").split()}
 
 

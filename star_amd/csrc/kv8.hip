@@ -48,12 +48,15 @@ struct AppendArgs {
 
 // Workgroup (x, 2 * head + {K, V}, b): the blocks x, x + gridDim.x, ... that this call completes; x = 0, which holds the
 // first of them (the only one that reads the open block), afterwards writes the rows of the new open block.
+// A block goes through registers once: a thread has N chunks of 8 values of one token, the largest magnitude is found
+// over the workgroup, the codes of K leave as they are and those of V are turned by 4 x 4 bytes through an LDS tile
+// whose pitch (HD + 4) spreads both its rows and its columns over all banks.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int CH = HD / 8, N = KB * CH / 256;                   // 16-byte chunks of a row, chunks per thread
-    constexpr int VP = KB + 8;                                      // LDS pitch of a transposed row
-    __shared__ __attribute__((aligned(16))) T vt[HD * VP];
+    constexpr int VP = HD + 4;
+    __shared__ __attribute__((aligned(16))) uint8_t vt[KB * VP];
     __shared__ float wmax[4];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int b = blockIdx.z, h = blockIdx.y >> 1;
@@ -76,29 +79,22 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 
     for (int blk = first + blockIdx.x; blk < last; blk += gridDim.x) {
         const int held = max(0, at - blk * KB);                     // tokens of the block that lie in the open block's rows
+        // rows across the lanes where V's open block (transposed) is read, chunks across the lanes else
+        const bool turned = is_v && held > 0;
         x8 x[N];
+        int row[N], ch[N];
         float m = 0.f;
-        if (!is_v) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int row = (tid + 256 * i) / CH, ch = (tid + 256 * i) % CH;
-                x[i] = *(const x8*)((row < held ? tail + row * HD : src + (int64_t)(blk * KB + row - at) * sr) + 8 * ch);
+        for (int i = 0; i < N; ++i) {
+            const int q = tid + 256 * i;
+            row[i] = turned ? q % KB : q / CH;
+            ch[i] = turned ? q / KB : q % CH;
+            if (row[i] >= held) x[i] = *(const x8*)(src + (int64_t)(blk * KB + row[i] - at) * sr + 8 * ch[i]);
+            else if (!is_v) x[i] = *(const x8*)(tail + row[i] * HD + 8 * ch[i]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = tail[(8 * ch[i] + e) * KB + row[i]];
             }
-        } else {
-            // assemble the block transposed: the open block's rows lie so already, the new rows are turned here
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int row = (tid + 256 * i) / CH, ch = (tid + 256 * i) % CH;
-                if (row >= held) {
-                    const x8 y = *(const x8*)(src + (int64_t)(blk * KB + row - at) * sr + 8 * ch);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) vt[(8 * ch + e) * VP + row] = y[e];
-                }
-            }
-            for (int i = tid; i < HD * held; i += 256) vt[(i / held) * VP + i % held] = tail[(i / held) * KB + i % held];
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = *(const x8*)(vt + ((tid + 256 * i) / 8) * VP + 8 * ((tid + 256 * i) % 8));
         }
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -110,32 +106,65 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
         __syncthreads();                                            // (also: every read of the open block's rows is done)
         m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
         const float sc = block_scale(m), inv = 1.0f / sc;           // (exact: powers of two between 2^-126 and 2^120)
+        uint8_t* out = codes + (int64_t)blk * KB * HD;
+        if (!is_v) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) *(u32x2*)(codes + (int64_t)blk * KB * HD + 8 * (tid + 256 * i)) = codes8(x[i], inv);
+            for (int i = 0; i < N; ++i) *(u32x2*)(out + row[i] * HD + 8 * ch[i]) = codes8(x[i], inv);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const u32x2 w = codes8(x[i], inv);
+                *(uint32_t*)(vt + row[i] * VP + 8 * ch[i]) = w[0];
+                *(uint32_t*)(vt + row[i] * VP + 8 * ch[i] + 4) = w[1];
+            }
+            __syncthreads();
+            for (int q = tid; q < 2 * HD; q += 256) {               // 8 tokens x 4 dimensions each
+                const int t8 = q & 7, d4 = q >> 3;
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = *(const uint32_t*)(vt + (8 * t8 + i) * VP + 4 * d4);
+                u32x2 o[4];
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint32_t lo01 = __builtin_amdgcn_perm(w[4 * p + 1], w[4 * p], 0x05010400), lo23 = __builtin_amdgcn_perm(w[4 * p + 3], w[4 * p + 2], 0x05010400);
+                    const uint32_t hi01 = __builtin_amdgcn_perm(w[4 * p + 1], w[4 * p], 0x07030602), hi23 = __builtin_amdgcn_perm(w[4 * p + 3], w[4 * p + 2], 0x07030602);
+                    o[0][p] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100);
+                    o[1][p] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302);
+                    o[2][p] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100);
+                    o[3][p] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) *(u32x2*)(out + (4 * d4 + k) * KB + 8 * t8) = o[k];
+            }
+        }
         if (tid == 0) scales[blk] = sc;
         __syncthreads();                                            // wmax and vt are free again
     }
     if (blockIdx.x == 0) {
-        const int from = max(at, last * KB), cnt = end - from;      // new rows of the open block
-        for (int i = tid; i < cnt * CH; i += 256) {
-            const int row = i / CH, ch = i % CH, r = from - last * KB + row;
+        const int from = max(at, last * KB), cnt = end - from, r0 = from - last * KB;   // new rows of the open block
+        const bool turned = is_v && cnt > 8;
+        for (int q = tid; q < (turned ? KB : cnt) * CH; q += 256) {
+            const int row = turned ? q % KB : q / CH, ch = turned ? q / KB : q % CH;
+            if (row >= cnt) continue;
             const x8 y = *(const x8*)(src + (int64_t)(from + row - at) * sr + 8 * ch);
-            if (!is_v) *(x8*)(tail + r * HD + 8 * ch) = y;
+            if (!is_v) *(x8*)(tail + (r0 + row) * HD + 8 * ch) = y;
             else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) tail[(8 * ch + e) * KB + r] = y[e];
+                for (int e = 0; e < 8; ++e) tail[(8 * ch + e) * KB + r0 + row] = y[e];
             }
         }
     }
-    // lens is read by every workgroup of the sequence and changed by the last of them
+    // lens is read by every workgroup of the sequence and changed by the last of them to get here: a workgroup's count
+    // goes out after its own read has come back (the value has steered everything above), so no fence is needed.  The
+    // counters of two sequences lie in different cache lines.
     __syncthreads();
     if (tid == 0) {
-        __threadfence();
         const int total = (int)(gridDim.x * gridDim.y);
-        if (atomicAdd(&c.tickets[b], 1) == total - 1) {
+        int32_t* ticket = c.tickets + (int64_t)b * STAR_KV8_TICKET_STRIDE;
+        if (__hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == total - 1) {
             c.lens[b] = end;
             if (want > n) c.dropped[b] += want - n;
-            c.tickets[b] = 0;
+            *ticket = 0;
         }
     }
 }

@@ -1739,7 +1739,7 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
 
 
 # ----------------------------------------------------------------------------- 8-bit key/value cache
-KV8_BLOCK = 64                    # STAR_KV8_BLOCK
+KV8_BLOCK, KV8_TICKET_STRIDE = 64, 32        # STAR_KV8_BLOCK, STAR_KV8_TICKET_STRIDE
 
 
 class KVCache8:
@@ -1795,7 +1795,7 @@ class KVCache8:
             setattr(self, n, t)
         self.batch, self.kv_heads, self.capacity, self.head_dim, self.dtype, self.device = B, H, T, hd, dt, dev
         self._dropped = torch.zeros(B, dtype=torch.int32, device=dev)
-        self._tickets = torch.zeros(B, dtype=torch.int32, device=dev)
+        self._tickets = torch.zeros(B * KV8_TICKET_STRIDE, dtype=torch.int32, device=dev)
         c = self._c = KV8Cache()
         c.B, c.Hkv, c.T, c.hd, c.dtype = B, H, T, hd, _DT16[dt]
         for n in self._PARTS:
