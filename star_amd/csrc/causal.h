@@ -29,35 +29,36 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
 // two accumulator blocks (rows 4g+i of two 16-row tiles) -> the 8 contraction slots of a B operand.  The contraction
 // order is then (tile 0 rows 4g..4g+3, tile 1 rows 4g..4g+3); tile_tr8 reads the A side in the same order.
 template <typename T>
+__device__ __forceinline__ typename Vec<T>::x4 pack4(const f32x4& t) {
+    return (typename Vec<T>::x4){(T)t[0], (T)t[1], (T)t[2], (T)t[3]};
+}
+template <typename X4>
+__device__ __forceinline__ auto join8(const X4& a, const X4& b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+template <typename T>
 __device__ __forceinline__ typename Vec<T>::x8 pack_b(const f32x4& t0, const f32x4& t1) {
-    typename Vec<T>::x8 r;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { r[j] = (T)t0[j]; r[4 + j] = (T)t1[j]; }
-    return r;
+    return join8(pack4<T>(t0), pack4<T>(t1));
 }
 
-// An LDS tile of ROWS rows of HD 16-bit values.  Rows are 128 or 256 bytes (HD = 96 leaves the last 64 bytes unused)
-// and their 16-byte chunks are permuted by the row, so that both ways of reading it are free of bank conflicts:
-//   row8   16 rows x 4 chunks of one wave, for operands that contract over HD
-//   tr8    ds_read_b64_tr_b16: 4 rows x 16 columns per 16 lanes, transposed, for operands that contract over rows
+// An LDS tile of rows of HD 16-bit values, read in two ways, each from one address per lane plus constants:
+//   row8   16 rows x 4 chunks of 16 bytes of one wave, for operands that contract over HD
+//   tr8    ds_read_b64_tr_b16: 8 rows x 32 bytes of one half wave, transposed, for operands that contract over rows
+// A row is HD * 2 + 16 bytes, an odd number of 16-byte chunks, so the 16 rows of row8 begin in 16 different chunks of the
+// 256-byte bank cycle.  Row r of each 16 lies in place 2 (r % 8) + r / 8, so the 8 neighbouring rows of tr8 begin 32
+// bytes apart or more: both are free of bank conflicts.
 template <typename T, int HD>
 struct Tile {
-    static constexpr int ROWB = HD == 64 ? 128 : 256;
+    static constexpr int ROWB = HD * 2 + 16;
     static constexpr int CHUNKS = HD / 8;
-    __device__ static __forceinline__ int swz(int r) {
-        if constexpr (HD == 64) return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 2) & 1);
-        else return (r & 7) << 1;
-    }
+    __device__ static __forceinline__ int place(int r) { return (r & ~15) + ((r & 7) << 1) + ((r >> 3) & 1); }
     // rows row0 + r16, values 32 ks + 8 g ..
     __device__ static __forceinline__ typename Vec<T>::x8 row8(const uint8_t* tile, int row0, int ks, int lane) {
         const int r = lane & 15, g = lane >> 4;
-        return *(const typename Vec<T>::x8*)(tile + (row0 + r) * ROWB + (((4 * ks + g) ^ swz(r)) << 4));
+        return *(const typename Vec<T>::x8*)(tile + place(r) * ROWB + 16 * g + row0 * ROWB + 64 * ks);
     }
     // column 16 nt + r16 of rows row0 + 4g .. + 3 and row0 + 16 + 4g .. + 3
     __device__ static __forceinline__ typename Vec<T>::x8 tr8(const uint8_t* tile, int row0, int nt, int lane) {
         const int r = lane & 15, g = lane >> 4;
-        const int row = 4 * g + (r >> 2);
-        const uint8_t* p = tile + (row0 + row) * ROWB + (((2 * nt + ((r >> 1) & 1)) ^ swz(row)) << 4) + 8 * (r & 1);
+        const uint8_t* p = tile + place(4 * g + (r >> 2)) * ROWB + 8 * (r & 3) + row0 * ROWB + 32 * nt;
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p));
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p + 16 * ROWB));
         return __builtin_bit_cast(typename Vec<T>::x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -65,17 +66,36 @@ struct Tile {
 };
 
 // A tile on its way from global memory through registers: load() asks for it, store() puts it into LDS after the
-// tile before it has been used.  Rows at or past `limit` read row limit - 1 (their weights are exact zeros).
+// tile before it has been used.  Rows at or past `limit` read row limit - 1 (their weights are exact zeros).  A thread's
+// place in a whole tile is a 32-bit byte offset (ROWS * sr * 2 < 2^32, checked on the host) from the tile's scalar
+// address, found once.
 template <typename T, int HD, int ROWS, int NTH>
 struct TileLoad {
     static constexpr int CHUNKS = HD / 8, TOTAL = ROWS * CHUNKS, N = (TOTAL + NTH - 1) / NTH;
+    static constexpr bool EVEN = NTH % CHUNKS == 0;                // chunk i then lies i * NTH / CHUNKS whole rows further
     u32x4 v[N];
-    __device__ __forceinline__ void load(const T* __restrict__ g, int64_t sr, int row0, int limit, int tid) {
+    uint32_t at[EVEN ? 1 : N];
+    __device__ __forceinline__ void place(int64_t sr, int tid) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = tid + i * NTH;
-            const int row = min(row0 + c / CHUNKS, limit - 1);
-            v[i] = *(const u32x4*)(g + (int64_t)row * sr + (c % CHUNKS) * 8);
+        for (int i = 0; i < (EVEN ? 1 : N); ++i) {
+            const int c = min(tid + i * NTH, TOTAL - 1);
+            at[i] = (uint32_t)(c / CHUNKS) * (uint32_t)(sr * 2) + (uint32_t)(c % CHUNKS) * 16;
+        }
+    }
+    __device__ __forceinline__ void load(const T* __restrict__ g, int64_t sr, int row0, int limit, int tid) {
+        const char* p = (const char*)(g + (int64_t)row0 * sr);
+        if (row0 + ROWS <= limit) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if constexpr (EVEN) v[i] = *(const u32x4*)(p + i * (NTH / CHUNKS) * (sr * 2) + at[0]);
+                else v[i] = *(const u32x4*)(p + at[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = min(tid + i * NTH, TOTAL - 1);
+                v[i] = *(const u32x4*)(p + (int64_t)min(c / CHUNKS, limit - 1 - row0) * (sr * 2) + (c % CHUNKS) * 16);
+            }
         }
     }
     __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
@@ -83,7 +103,7 @@ struct TileLoad {
         for (int i = 0; i < N; ++i) {
             const int c = tid + i * NTH, row = c / CHUNKS;
             if (TOTAL % NTH == 0 || c < TOTAL)
-                *(u32x4*)(tile + row * Tile<T, HD>::ROWB + (((c % CHUNKS) ^ Tile<T, HD>::swz(row & 15)) << 4)) = v[i];
+                *(u32x4*)(tile + Tile<T, HD>::place(row) * Tile<T, HD>::ROWB + (c % CHUNKS) * 16) = v[i];
         }
     }
 };

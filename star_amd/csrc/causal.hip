@@ -77,6 +77,8 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
 
     TileLoad<T, HD, CK, 256> kl, vl;
     const int ntile = (end + CK - 1) / CK;
+    kl.place(s.k_sr, tid);
+    vl.place(s.v_sr, tid);
     if (ntile > 0) {
         kl.load(Kh, s.k_sr, 0, sq.nk, tid);
         vl.load(Vh, s.v_sr, 0, sq.nk, tid);
@@ -108,20 +110,24 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
                 for (int ks = 0; ks < KS; ++ks) sc[qb][kt4] = mfma16(kf[ks], qf[qb][ks], sc[qb][kt4]);
             }
         }
-        const bool masked = key0 + CK > all_see;
+        if (key0 + CK > all_see) {                                 // (wave-uniform) some query does not see the whole tile
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+                for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[qb][kt4][i] = key0 + 16 * kt4 + 4 * g + i < lim[qb] ? sc[qb][kt4][i] : -INFINITY;
+        }
         x8 pf[2][2];
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-            float mx = M_NONE;
+            float mx = sc[qb][0][0];                               // of the raw products: the scale is positive
 #pragma unroll
             for (int kt4 = 0; kt4 < 4; ++kt4)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = sc[qb][kt4][i] * c2;
-                    if (masked && key0 + 16 * kt4 + 4 * g + i >= lim[qb]) x = -INFINITY;
-                    sc[qb][kt4][i] = x;
-                    mx = fmaxf(mx, x);
-                }
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[qb][kt4][i]);
+            mx *= c2;
             if (!__all(mx <= m[qb] + M_SLACK)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -138,7 +144,7 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
             for (int kt4 = 0; kt4 < 4; ++kt4)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(sc[qb][kt4][i] - m[qb]);
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][kt4][i], c2, -m[qb]));
                     sum += p;
                     sc[qb][kt4][i] = p;
                 }
@@ -243,6 +249,8 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 
     TileLoad<T, HD, CK, 256> kl, vl;
     const int ntile = (end + CK - 1) / CK;
+    kl.place(s.k_sr, tid);
+    vl.place(s.v_sr, tid);
     if (ntile > 0) {
         kl.load(Kh, s.k_sr, 0, sq.nk, tid);
         vl.load(Vh, s.v_sr, 0, sq.nk, tid);
@@ -260,10 +268,10 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
         }
         const int key0 = tile * CK;
         if (key0 >= wave_end) continue;
-        const bool masked = key0 + CK > all_see;
+        const bool masked = key0 + CK > all_see;                   // (wave-uniform)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {                           // 32 keys at a time
-            f32x4 ds[2][2];
+            x4 ds[2][2];
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 f32x4 sc[2], dp[2];
@@ -283,14 +291,29 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
                 for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const bool hide = masked && key0 + 32 * hf + 16 * k2 + 4 * g + i >= lim[qb];
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][i], c2, -l2[qb]));
-                        ds[qb][k2][i] = hide ? 0.f : p * (dp[qb][i] - dl[qb]);
+                        sc[qb][i] = __builtin_fmaf(sc[qb][i], c2, -l2[qb]);
+                        dp[qb][i] -= dl[qb];
                     }
+                if (masked) {
+#pragma unroll
+                    for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool vis = key0 + 32 * hf + 16 * k2 + 4 * g + i < lim[qb];
+                            sc[qb][i] = vis ? sc[qb][i] : -INFINITY;
+                            dp[qb][i] = vis ? dp[qb][i] : 0.f;
+                        }
+                }
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dp[qb][i] *= __builtin_amdgcn_exp2f(sc[qb][i]);
+                    ds[qb][k2] = pack4<T>(dp[qb]);
+                }
             }
             x8 df[2];
 #pragma unroll
-            for (int qb = 0; qb < 2; ++qb) df[qb] = pack_b<T>(ds[qb][0], ds[qb][1]);
+            for (int qb = 0; qb < 2; ++qb) df[qb] = join8(ds[qb][0], ds[qb][1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const x8 kf = Ti::tr8(kt, 32 * hf, nt, lane);
@@ -315,44 +338,52 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------------ gradients of K, V
-// One workgroup: 128 keys of one key head, 32 per wave with K, V, dK^T and dV^T in registers; it walks the queries of
-// every query head of the group in tiles of 64.  The key is on the MFMA column, so P and dS come out as the operands of
+// One workgroup: 128 keys of one key head, 32 per wave with K, dK^T and dV^T in registers and V in LDS (with V in
+// registers too only one wave would fit a SIMD, and nothing would cover its LDS and exponential latencies); it walks the
+// queries of its query heads in tiles of 32.  The key is on the MFMA column, so P and dS come out as the operands of
 // dV^T += dO^T P and dK^T += Q^T dS.
+// A launch with few key tiles is cut by query heads (`parts` > 1): part p takes heads p * grp / parts .. of the group and
+// leaves fp32 sums, which causal_dkv_sum_kernel adds up in order.
+constexpr int CQ = 32;
 template <typename T, int HD>
-__global__ __launch_bounds__(256, 1) void causal_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                            const T* __restrict__ V, const T* __restrict__ dO,
                                                            const float* __restrict__ lse, const float* __restrict__ delta,
                                                            const int32_t* __restrict__ seqs,
                                                            const int32_t* __restrict__ tiles, star_causal_shape s,
-                                                           T* __restrict__ dK, T* __restrict__ dV) {
+                                                           int parts, float* __restrict__ sums, T* __restrict__ dK,
+                                                           T* __restrict__ dV) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
     using Ti = Tile<T, HD>;
     constexpr int KS = HD / 32, NT = HD / 16;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    constexpr int TB = CK * Ti::ROWB, SB = 2 * TB + 2 * CK * 4;    // Q | dO | lse | delta
+    constexpr int VB = CT * Ti::ROWB, TB = CQ * Ti::ROWB, SB = 2 * TB + 2 * CQ * 4;   // V | 2 x (Q | dO | lse | delta)
 
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % s.Hkv, t = blockIdx.x / s.Hkv, grp = s.H / s.Hkv;
+    const int hk = blockIdx.x % s.Hkv, part = blockIdx.x / s.Hkv % parts, t = blockIdx.x / s.Hkv / parts;
+    const int heads = s.H / s.Hkv / parts, h0 = hk * (s.H / s.Hkv) + part * heads;
     const SeqOf sq = seq_of(seqs, tiles[2 * t]);
     const int j0 = tiles[2 * t + 1], w0 = j0 + 32 * wid;           // first key of the workgroup, of the wave
     const int off = sq.nk - sq.nq;
+    uint8_t* vt = smem + 32 * wid * Ti::ROWB;                      // the wave's rows of V
 
-    x8 kf[2][KS], vf[2][KS];
+    x8 kf[2][KS];
     int see[2];                                                    // first query that sees this lane's key
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
         const int j = w0 + 16 * kb + r16;
-        const int64_t row = sq.k0 + min(j, sq.nk - 1);
         see[kb] = j < sq.nk ? j - off : 0x7fffffff;
-        const T* kr = K + row * s.k_sr + (int64_t)hk * s.k_sh + 8 * g;
-        const T* vr = V + row * s.v_sr + (int64_t)hk * s.v_sh + 8 * g;
+        const T* kr = K + (int64_t)(sq.k0 + min(j, sq.nk - 1)) * s.k_sr + (int64_t)hk * s.k_sh + 8 * g;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            kf[kb][ks] = *(const x8*)(kr + 32 * ks);
-            vf[kb][ks] = *(const x8*)(vr + 32 * ks);
-        }
+        for (int ks = 0; ks < KS; ++ks) kf[kb][ks] = *(const x8*)(kr + 32 * ks);
+    }
+    {
+        TileLoad<T, HD, CT, 256> vl;
+        vl.place(s.v_sr, tid);
+        vl.load(V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh, s.v_sr, j0, sq.nk, tid);
+        vl.store(smem, tid);
     }
     f32x4 dk[2][NT], dv[2][NT];
 #pragma unroll
@@ -360,80 +391,104 @@ __global__ __launch_bounds__(256, 1) void causal_dkv_kernel(const T* __restrict_
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) dk[kb][nt] = dv[kb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const float c2 = s.scale * A_LOG2E;
-    const int first = max(0, j0 - off) / CK;                       // query tiles before it see none of these keys
-    const int nper = max(0, (sq.nq + CK - 1) / CK - first);        // tiles per head
+    const int first = max(0, j0 - off) / CQ;                       // query tiles before it see none of these keys
+    const int nper = max(0, (sq.nq + CQ - 1) / CQ - first);        // tiles per head
     const int all_see = w0 + 32 <= sq.nk ? w0 + 31 - off : 0x7fffffff;  // from this query on every key of the wave is visible
 
-    TileLoad<T, HD, CK, 256> ql, gl;
+    TileLoad<T, HD, CQ, 256> ql, gl;
     float lr = 0.f;
-    auto load = [&](int n) {
-        const int h = hk * grp + n / nper, q0 = (first + n % nper) * CK;
-        ql.load(Q + (int64_t)sq.q0 * s.q_sr + (int64_t)h * s.q_sh, s.q_sr, q0, sq.nq, tid);
-        gl.load(dO + (int64_t)sq.q0 * s.o_sr + (int64_t)h * s.o_sh, s.o_sr, q0, sq.nq, tid);
-        if (tid < 2 * CK) lr = (tid < CK ? lse : delta)[(int64_t)h * s.lse_stride + sq.q0 + min(q0 + (tid & (CK - 1)), sq.nq - 1)];
+    int lh = h0, lq = first * CQ;                                  // head and first query of the next tile to load
+    auto load = [&]() {
+        ql.load(Q + (int64_t)sq.q0 * s.q_sr + (int64_t)lh * s.q_sh, s.q_sr, lq, sq.nq, tid);
+        gl.load(dO + (int64_t)sq.q0 * s.o_sr + (int64_t)lh * s.o_sh, s.o_sr, lq, sq.nq, tid);
+        if (tid < 2 * CQ) lr = (tid < CQ ? lse : delta)[(int64_t)lh * s.lse_stride + sq.q0 + min(lq + (tid & (CQ - 1)), sq.nq - 1)];
+        lq += CQ;
+        if (lq >= sq.nq) { lq = first * CQ; ++lh; }
     };
-    const int ntile = nper * grp;
-    if (ntile > 0) load(0);
+    ql.place(s.q_sr, tid);
+    gl.place(s.o_sr, tid);
+    const int ntile = nper * heads;
+    int q0 = first * CQ;
+    if (ntile > 0) load();
 #pragma unroll 1
     for (int n = 0; n < ntile; ++n) {
-        uint8_t* qt = smem + (n & 1) * SB;
+        uint8_t* qt = smem + VB + (n & 1) * SB;
         uint8_t* gt = qt + TB;
         float* lt = (float*)(gt + TB);
         ql.store(qt, tid);
         gl.store(gt, tid);
-        if (tid < CK) lt[tid] = lr * A_LOG2E;
-        else if (tid < 2 * CK) lt[tid] = lr;
+        if (tid < CQ) lt[tid] = lr * A_LOG2E;
+        else if (tid < 2 * CQ) lt[tid] = lr;
         __syncthreads();
-        if (n + 1 < ntile) load(n + 1);
-        const int q0 = (first + n % nper) * CK;
-        if (q0 + CK <= w0 - off) continue;                         // (wave-uniform) no query of the tile sees a key of the wave
-        const bool masked = q0 < all_see || q0 + CK > sq.nq;
+        if (n + 1 < ntile) load();
+        const int qa0 = q0;
+        q0 += CQ;
+        if (q0 >= sq.nq) q0 = first * CQ;
+        if (qa0 + CQ <= w0 - off) continue;                        // (wave-uniform) no query of the tile sees a key of the wave
+        const bool masked = qa0 < all_see || qa0 + CQ > sq.nq;
+        x4 pp[2][2], ds[2][2];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {                           // 32 queries at a time
-            f32x4 pp[2][2], ds[2][2];
+        for (int q2 = 0; q2 < 2; ++q2) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4 sc[2], dp[2];
 #pragma unroll
-            for (int q2 = 0; q2 < 2; ++q2) {
-                f32x4 sc[2], dp[2];
+            for (int kb = 0; kb < 2; ++kb) sc[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) sc[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int ks = 0; ks < KS; ++ks) {
+                const x8 qa = Ti::row8(qt, 16 * q2, ks, lane);
+                const x8 ga = Ti::row8(gt, 16 * q2, ks, lane);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const x8 qa = Ti::row8(qt, 32 * hf + 16 * q2, ks, lane);
-                    const x8 ga = Ti::row8(gt, 32 * hf + 16 * q2, ks, lane);
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) {
-                        sc[kb] = mfma16(qa, kf[kb][ks], sc[kb]);
-                        dp[kb] = mfma16(ga, vf[kb][ks], dp[kb]);
-                    }
+                for (int kb = 0; kb < 2; ++kb) {
+                    sc[kb] = mfma16(qa, kf[kb][ks], sc[kb]);
+                    dp[kb] = mfma16(ga, Ti::row8(vt, 16 * kb, ks, lane), dp[kb]);
                 }
-                const f32x4 ls = *(const f32x4*)(lt + 32 * hf + 16 * q2 + 4 * g);
-                const f32x4 de = *(const f32x4*)(lt + CK + 32 * hf + 16 * q2 + 4 * g);
+            }
+            const f32x4 ls = *(const f32x4*)(lt + 16 * q2 + 4 * g);
+            const f32x4 de = *(const f32x4*)(lt + CQ + 16 * q2 + 4 * g);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[kb][i] = __builtin_fmaf(sc[kb][i], c2, -ls[i]);
+                    dp[kb][i] -= de[i];
+                }
+            if (masked) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int qi = q0 + 32 * hf + 16 * q2 + 4 * g + i;
-                        const bool hide = masked && (qi < see[kb] || qi >= sq.nq);
-                        const float p = hide ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i], c2, -ls[i]));
-                        pp[kb][q2][i] = p;
-                        ds[kb][q2][i] = hide ? 0.f : p * (dp[kb][i] - de[i]);
+                        const int qi = qa0 + 16 * q2 + 4 * g + i;
+                        const bool vis = qi >= see[kb] && qi < sq.nq;
+                        sc[kb][i] = vis ? sc[kb][i] : -INFINITY;
+                        dp[kb][i] = vis ? dp[kb][i] : 0.f;
                     }
             }
-            x8 pf[2], df[2];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                pf[kb] = pack_b<T>(pp[kb][0], pp[kb][1]);
-                df[kb] = pack_b<T>(ds[kb][0], ds[kb][1]);
-            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const x8 ga = Ti::tr8(gt, 32 * hf, nt, lane);
-                const x8 qa = Ti::tr8(qt, 32 * hf, nt, lane);
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    dv[kb][nt] = mfma16(ga, pf[kb], dv[kb][nt]);
-                    dk[kb][nt] = mfma16(qa, df[kb], dk[kb][nt]);
+                for (int i = 0; i < 4; ++i) {
+                    sc[kb][i] = __builtin_amdgcn_exp2f(sc[kb][i]);
+                    dp[kb][i] *= sc[kb][i];
                 }
+                pp[kb][q2] = pack4<T>(sc[kb]);
+                ds[kb][q2] = pack4<T>(dp[kb]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        x8 pf[2], df[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            pf[kb] = join8(pp[kb][0], pp[kb][1]);
+            df[kb] = join8(ds[kb][0], ds[kb][1]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const x8 ga = Ti::tr8(gt, 0, nt, lane);
+            const x8 qa = Ti::tr8(qt, 0, nt, lane);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                dv[kb][nt] = mfma16(ga, pf[kb], dv[kb][nt]);
+                dk[kb][nt] = mfma16(qa, df[kb], dk[kb][nt]);
             }
         }
     }
@@ -442,6 +497,16 @@ __global__ __launch_bounds__(256, 1) void causal_dkv_kernel(const T* __restrict_
         const int j = w0 + 16 * kb + r16;
         if (j >= sq.nk) continue;
         const int64_t at = ((int64_t)(sq.k0 + j) * s.Hkv + hk) * HD + 4 * g;
+        if (parts > 1) {
+            float* sk = sums + (int64_t)part * 2 * s.k_rows * s.Hkv * HD + at;
+            float* sv = sk + s.k_rows * s.Hkv * HD;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                *(f32x4*)(sk + 16 * nt) = dk[kb][nt];
+                *(f32x4*)(sv + 16 * nt) = dv[kb][nt];
+            }
+            continue;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             x4 a, b;
@@ -456,15 +521,53 @@ __global__ __launch_bounds__(256, 1) void causal_dkv_kernel(const T* __restrict_
     }
 }
 
+// parts fp32 sums of a key tile -> dK, dV
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ seqs,
+                                                            const int32_t* __restrict__ tiles, star_causal_shape s, int parts,
+                                                            T* __restrict__ dK, T* __restrict__ dV) {
+    typedef typename Vec<T>::x4 x4;
+    const int hk = blockIdx.x % s.Hkv, t = blockIdx.x / s.Hkv;
+    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const int j0 = tiles[2 * t + 1], rows = min(CT, sq.nk - j0);
+    const int64_t one = s.k_rows * s.Hkv * HD;
+    for (int c = threadIdx.x; c < 2 * rows * (HD / 4); c += 256) {
+        const int which = c / (rows * (HD / 4)), cc = c % (rows * (HD / 4));
+        const int64_t at = ((int64_t)(sq.k0 + j0 + cc / (HD / 4)) * s.Hkv + hk) * HD + 4 * (cc % (HD / 4));
+        f32x4 sum = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < parts; ++p) sum += *(const f32x4*)(sums + (2 * p + which) * one + at);
+        x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)(which ? sum[e] : sum[e] * s.scale);
+        *(x4*)((which ? dV : dK) + at) = o;
+    }
+}
+
+// Parts of the query heads of a group: 1 when the key tiles alone make two workgroups for each of the 512 places (two a
+// CU), or when a sequence is short (under four tiles of keys on average) and its walk with it; otherwise the fewest that
+// make them.
+static int dkv_parts(const star_causal_shape* s, int nk_tiles) {
+    const int grp = s->H / s->Hkv;
+    int parts = 1;
+    if (nk_tiles >= 4 * s->nseq)
+        while (parts < grp && (int64_t)nk_tiles * s->Hkv * parts < 1024) {
+            do ++parts; while (grp % parts);
+        }
+    return parts;
+}
+
 // ------------------------------------------------------------------------------------------------------ host side
 static int check_causal(const star_causal_shape* s, const char* who) {
     STAR_REQUIRE(s, "%s: null shape", who);
     STAR_REQUIRE(s->hd == 64 || s->hd == 96 || s->hd == 128, "%s: head dim %d not in {64, 96, 128}", who, s->hd);
     STAR_REQUIRE(s->dtype == STAR_DT_BF16 || s->dtype == STAR_DT_F16, "%s: dtype %d is neither bf16 nor fp16", who, s->dtype);
     STAR_REQUIRE(s->Hkv >= 1 && s->H >= s->Hkv && s->H % s->Hkv == 0, "%s: %d query heads do not divide into %d key heads", who, s->H, s->Hkv);
-    STAR_REQUIRE(s->nseq >= 0 && s->lse_stride >= 0, "%s: negative size", who);
+    STAR_REQUIRE(s->nseq >= 0 && s->lse_stride >= 0 && s->k_rows >= 0, "%s: negative size", who);
     const int64_t st[8] = {s->q_sr, s->q_sh, s->k_sr, s->k_sh, s->v_sr, s->v_sh, s->o_sr, s->o_sh};
     for (int i = 0; i < 8; ++i) STAR_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    for (int i = 0; i < 8; i += 2)
+        STAR_REQUIRE(st[i] >= 0 && st[i] < (1ll << 23), "%s: row stride %lld not in [0, 2^23)", who, (long long)st[i]);
+    STAR_REQUIRE(s->scale > 0.f && s->scale < INFINITY, "%s: scale must be positive and finite", who);
     return STAR_OK;
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -483,12 +586,18 @@ static int launch_causal_fwd(const void* q, const void* k, const void* v, const 
     return STAR_OK;
 }
 
+static int64_t causal_bwd_bytes(const star_causal_shape* s, int nk_tiles) {
+    const int parts = dkv_parts(s, nk_tiles);
+    return parts == 1 ? 0 : (int64_t)parts * 2 * s->k_rows * s->Hkv * s->hd * 4;
+}
+
 template <typename T, int HD>
 static int launch_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
                              const int32_t* seqs, const int32_t* q_tiles, int nq_tiles, const int32_t* k_tiles,
                              int nk_tiles, const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta,
-                             hipStream_t st) {
-    constexpr int smem_q = 4 * CK * Tile<T, HD>::ROWB, smem_k = 2 * (2 * CK * Tile<T, HD>::ROWB + 2 * CK * 4);
+                             float* sums, hipStream_t st) {
+    constexpr int smem_q = 4 * CK * Tile<T, HD>::ROWB;
+    constexpr int smem_k = CT * Tile<T, HD>::ROWB + 2 * (2 * CQ * Tile<T, HD>::ROWB + 2 * CQ * 4);
     static DevOnce once_q, once_k;
     if (!reserve_lds_once(once_q, (const void*)causal_dq_kernel<T, HD>, smem_q) ||
         !reserve_lds_once(once_k, (const void*)causal_dkv_kernel<T, HD>, smem_k)) {
@@ -498,10 +607,15 @@ static int launch_causal_bwd(const void* q, const void* k, const void* v, const 
     if (nq_tiles > 0)
         hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3((unsigned)nq_tiles * s->H), dim3(256), smem_q, st, (const T*)q,
                            (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, seqs, q_tiles, *s, (T*)dq, delta);
-    if (nk_tiles > 0)
-        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)nk_tiles * s->Hkv), dim3(256), smem_k, st, (const T*)q,
-                           (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, seqs, k_tiles, *s, (T*)dk,
-                           (T*)dv);
+    if (nk_tiles > 0) {
+        const int parts = dkv_parts(s, nk_tiles);
+        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)nk_tiles * s->Hkv * parts), dim3(256), smem_k, st,
+                           (const T*)q, (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, seqs, k_tiles, *s,
+                           parts, sums, (T*)dk, (T*)dv);
+        if (parts > 1)
+            hipLaunchKernelGGL((causal_dkv_sum_kernel<T, HD>), dim3((unsigned)nk_tiles * s->Hkv), dim3(256), 0, st,
+                               (const float*)sums, seqs, k_tiles, *s, parts, (T*)dk, (T*)dv);
+    }
     return STAR_OK;
 }
 
@@ -535,10 +649,15 @@ extern "C" int star_causal_fwd(const void* q, const void* k, const void* v, cons
     return STAR_OK;
 }
 
+extern "C" size_t star_causal_bwd_workspace(const star_causal_shape* s, int nk_tiles) {
+    using namespace star;
+    return check_causal(s, "star_causal_bwd_workspace") || nk_tiles < 0 ? 0 : (size_t)causal_bwd_bytes(s, nk_tiles);
+}
+
 extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_,
                                const float* lse, const int32_t* seqs, const int32_t* q_tiles, int nq_tiles,
                                const int32_t* k_tiles, int nk_tiles, const star_causal_shape* s, void* dq, void* dk,
-                               void* dv, float* delta, void* stream) {
+                               void* dv, float* delta, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace star;
     int rc = check_causal(s, "star_causal_bwd");
     if (rc) return rc;
@@ -549,8 +668,13 @@ extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, cons
                  "star_causal_bwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(do_) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                  "star_causal_bwd: tensors must be 16-byte aligned");
+    const int64_t need = causal_bwd_bytes(s, nk_tiles);
+    if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !aligned16(workspace))) {
+        set_error("star_causal_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);
+        return STAR_ERR_WORKSPACE;
+    }
     CAUSAL_BY_TYPE((launch_causal_bwd<T, HD>(q, k, v, o, do_, lse, seqs, q_tiles, nq_tiles, k_tiles, nk_tiles, s, dq, dk, dv,
-                                             delta, (hipStream_t)stream)));
+                                             delta, (float*)workspace, (hipStream_t)stream)));
     if (rc) return rc;
     STAR_LAUNCH_CHECK("star_causal_bwd");
     return STAR_OK;

@@ -1657,7 +1657,7 @@ def _causal_shape(q, k, v, o, plan, scale):
         s.q_sr = s.o_sr = 0
     if k.shape[0] == 1:
         s.k_sr = s.v_sr = 0
-    s.lse_stride, s.scale = q.shape[0], float(scale)
+    s.lse_stride, s.k_rows, s.scale = q.shape[0], k.shape[0], float(scale)
     return s
 
 
@@ -1703,9 +1703,12 @@ class _CausalAttn(torch.autograd.Function):
             dv = _rows_like(k.shape[0], plan.k_used, k.shape[1], k.shape[2], v)
             delta = torch.empty_like(lse)
             s = _causal_shape(q, k, v, o, plan, ctx.scale)
+            need = lib().star_causal_bwd_workspace(s, plan.k_tiles.shape[0])
+            ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
             check(lib().star_causal_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(g), ptr(lse), ptr(plan.seqs),
                                         ptr(plan.q_tiles), plan.q_tiles.shape[0], ptr(plan.k_tiles), plan.k_tiles.shape[0],
-                                        s, ptr(dq), ptr(dk), ptr(dv), ptr(delta), stream_ptr()), "star_causal_bwd")
+                                        s, ptr(dq), ptr(dk), ptr(dv), ptr(delta), ptr(ws), need, stream_ptr()),
+                  "star_causal_bwd")
         return dq, dk, dv, None, None
 
 
@@ -1728,13 +1731,16 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
         raise TypeError(f"causal_attn: q, k and v must share one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
         raise ValueError(f"causal_attn: {q.shape[1]} query heads do not divide into {k.shape[1]} key heads")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"causal_attn: scale = {scale}; a positive number is required")
     if plan.device != dev:
         raise ValueError(f"causal_attn: the plan is on {plan.device}, the tensors on {dev}")
     if q.shape[0] < plan.q_rows or k.shape[0] < plan.k_rows:
         raise ValueError(f"causal_attn: the plan needs {plan.q_rows} query and {plan.k_rows} key rows, got {q.shape[0]} and {k.shape[0]}")
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check_rows("causal_attn", name, t)
-    o, lse = _CausalAttn.apply(q, k, v, plan, q.shape[2] ** -0.5 if scale is None else float(scale))
+    o, lse = _CausalAttn.apply(q, k, v, plan, scale)
     return (o, lse) if need_lse else o
 
 

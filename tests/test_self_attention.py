@@ -619,12 +619,20 @@ def test_the_library_checks_sizes_before_any_launch():
     s = _lib.CausalShape(H=4, Hkv=3, hd=64, dtype=0)
     assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"divide" in L.star_last_error()
     s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=1)
-    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 1, 16, 1, s, 16, 16, 16, 16, None) == -1 and b"dtype" in L.star_last_error()
+    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 1, 16, 1, s, 16, 16, 16, 16, None, 0, None) == -1 and b"dtype" in L.star_last_error()
     s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, q_sr=4)
     assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"multiples of 8" in L.star_last_error()
-    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0)
+    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, q_sr=1 << 23, scale=1)
+    assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"row stride" in L.star_last_error()
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, scale=scale)
+        assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"scale" in L.star_last_error()
+    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, scale=1)
     assert L.star_causal_fwd(16, 24, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"aligned" in L.star_last_error()
     assert L.star_causal_fwd(None, None, None, None, None, 0, s, None, None, None) == 0
+    s = _lib.CausalShape(H=4, Hkv=1, hd=64, dtype=0, nseq=1, k_rows=2000, scale=1)
+    assert L.star_causal_bwd_workspace(s, 16) > 0 and L.star_causal_bwd_workspace(s, 3) == 0
+    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, s, 16, 16, 16, 16, None, 0, None) == -3 and b"workspace" in L.star_last_error()
     c = _lib.KV8Cache(B=1, Hkv=2, T=100, hd=64, dtype=0)
     assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 0, 0, None, None, 1, None, 1, None) == -1 and b"capacity 100" in L.star_last_error()
     c = _lib.KV8Cache(B=1, Hkv=2, T=128, hd=64, dtype=0)
@@ -658,6 +666,8 @@ def test_causal_attn_refusals(ops):
             ops.causal_attn(*args, plan)
     with pytest.raises(ValueError, match="plan is on cpu"):
         ops.causal_attn(q, q, q, ops.PackedSeqs([10], "cpu"))
+    with pytest.raises(ValueError, match="scale"):
+        ops.causal_attn(q, q, q, plan, scale=0.0)
     assert ops.causal_attn(q[:0], q[:0], q[:0], ops.PackedSeqs([], DEV)).shape == (0, 4, 64)
     x = q.clone().requires_grad_()
     g, = torch.autograd.grad(ops.causal_attn(x, x, x, plan).sum(), x, create_graph=True)
