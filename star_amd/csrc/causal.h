@@ -42,23 +42,22 @@ __device__ __forceinline__ typename Vec<T>::x8 pack_b(const f32x4& t0, const f32
 // An LDS tile of rows of HD 16-bit values, read in two ways, each from one address per lane plus constants:
 //   row8   16 rows x 4 chunks of 16 bytes of one wave, for operands that contract over HD
 //   tr8    ds_read_b64_tr_b16: 8 rows x 32 bytes of one half wave, transposed, for operands that contract over rows
-// A row is HD * 2 + 16 bytes, an odd number of 16-byte chunks, so the 16 rows of row8 begin in 16 different chunks of the
-// 256-byte bank cycle.  Row r of each 16 lies in place 2 (r % 8) + r / 8, so the 8 neighbouring rows of tr8 begin 32
-// bytes apart or more: both are free of bank conflicts.
+// A row is HD * 2 + 32 bytes, twice an odd number of 16-byte chunks, so 8 neighbouring rows begin 32 bytes apart or more
+// in the 256-byte bank cycle, which is what tr8 reads at once, and rows r and r + 8 begin alike, which row8 never meets:
+// a wave's 16-byte reads go 16 lanes at a time, 8 rows of one chunk with the other 8 of its neighbour.
 template <typename T, int HD>
 struct Tile {
-    static constexpr int ROWB = HD * 2 + 16;
+    static constexpr int ROWB = HD * 2 + 32;
     static constexpr int CHUNKS = HD / 8;
-    __device__ static __forceinline__ int place(int r) { return (r & ~15) + ((r & 7) << 1) + ((r >> 3) & 1); }
     // rows row0 + r16, values 32 ks + 8 g ..
     __device__ static __forceinline__ typename Vec<T>::x8 row8(const uint8_t* tile, int row0, int ks, int lane) {
         const int r = lane & 15, g = lane >> 4;
-        return *(const typename Vec<T>::x8*)(tile + place(r) * ROWB + 16 * g + row0 * ROWB + 64 * ks);
+        return *(const typename Vec<T>::x8*)(tile + r * ROWB + 16 * g + row0 * ROWB + 64 * ks);
     }
     // column 16 nt + r16 of rows row0 + 4g .. + 3 and row0 + 16 + 4g .. + 3
     __device__ static __forceinline__ typename Vec<T>::x8 tr8(const uint8_t* tile, int row0, int nt, int lane) {
         const int r = lane & 15, g = lane >> 4;
-        const uint8_t* p = tile + place(4 * g + (r >> 2)) * ROWB + 8 * (r & 3) + row0 * ROWB + 32 * nt;
+        const uint8_t* p = tile + (4 * g + (r >> 2)) * ROWB + 8 * (r & 3) + row0 * ROWB + 32 * nt;
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p));
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, p + 16 * ROWB));
         return __builtin_bit_cast(typename Vec<T>::x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -103,7 +102,7 @@ struct TileLoad {
         for (int i = 0; i < N; ++i) {
             const int c = tid + i * NTH, row = c / CHUNKS;
             if (TOTAL % NTH == 0 || c < TOTAL)
-                *(u32x4*)(tile + Tile<T, HD>::place(row) * Tile<T, HD>::ROWB + (c % CHUNKS) * 16) = v[i];
+                *(u32x4*)(tile + row * Tile<T, HD>::ROWB + (c % CHUNKS) * 16) = v[i];
         }
     }
 };
