@@ -6,14 +6,12 @@ the STAR checkout (src/models/...).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import CausalShape, KV8Cache, KV8Query, XAttnShape, check, lib, ptr, stream_ptr
@@ -1561,9 +1559,20 @@ _DT16 = {torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 CAUSAL_TILE = 128                 # STAR_CAUSAL_TILE
 
 
-def _on(dev):
-    """The device of the tensors as the current one (and with it the stream that stream_ptr() gives)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(fn, what, dev, *args):
+    """fn(*args, the current stream of dev), with dev as the current device for the launch."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def _same_device(what, **ts):
@@ -1571,23 +1580,33 @@ def _same_device(what, **ts):
     for name, t in ts.items():
         if t is None:
             continue
-        _need_cuda(t)
-        if dev is not None and t.device != dev:
+        if not t.is_cuda:
+            _need_cuda(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise ValueError(f"{what}: {name} is on {t.device}, the others on {dev}")
-        dev = t.device
     return dev
 
 
-def _check_rows(what, name, t):
-    """What the 16-byte loads of the kernels need of a [.., hd] operand."""
+def _row_strides(what, name, t):
+    """The strides of a [.., hd] operand but for hd's, after checking what the kernels' 16-byte loads need of it.  That
+    of a dimension of size 1, which is never used and may be anything, is given as 0."""
     if t.dtype not in _DT16:
         raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16 or float16 is required")
-    if t.shape[-1] not in (64, 96, 128):
-        raise ValueError(f"{what}: head dim {t.shape[-1]} not in (64, 96, 128)")
-    if t.numel() and t.stride(-1) != 1:
+    *shape, hd = t.shape
+    *strides, one = t.stride()
+    if hd not in (64, 96, 128):
+        raise ValueError(f"{what}: head dim {hd} not in (64, 96, 128)")
+    if one != 1 and t.numel():
         raise ValueError(f"{what}: {name} must have a contiguous head dimension")
-    if t.data_ptr() % 16 or any(st % 8 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+    strides = [st if n > 1 else 0 for st, n in zip(strides, shape)]
+    bits = t.data_ptr()
+    for st in strides:
+        bits |= st * 2
+    if bits & 15:
         raise ValueError(f"{what}: {name} must be 16-byte aligned in every row")
+    return strides
 
 
 class PackedSeqs:
@@ -1641,24 +1660,7 @@ class PackedSeqs:
         a, b = seqs.size, seqs.size + qt.size
         self.seqs, self.q_tiles, self.k_tiles = buf[:a].view(-1, 4), buf[a:b].view(-1, 2), buf[b:].view(-1, 2)
         self.starts, self.counts = self.seqs[:, 2], self.seqs[:, 3]
-
-
-def _causal_shape(q, k, v, o, plan, scale):
-    s = CausalShape()
-    s.H, s.Hkv, s.hd, s.dtype, s.nseq = q.shape[1], k.shape[1], q.shape[2], _DT16[q.dtype], plan.n
-    s.q_sr, s.q_sh, s.k_sr, s.k_sh = q.stride(0), q.stride(1), k.stride(0), k.stride(1)
-    s.v_sr, s.v_sh, s.o_sr, s.o_sh = v.stride(0), v.stride(1), o.stride(0), o.stride(1)
-    # (the stride of a dimension of size 1 is never used, and may be anything)
-    if q.shape[1] == 1:
-        s.q_sh = s.o_sh = 0
-    if k.shape[1] == 1:
-        s.k_sh = s.v_sh = 0
-    if q.shape[0] == 1:
-        s.q_sr = s.o_sr = 0
-    if k.shape[0] == 1:
-        s.k_sr = s.v_sr = 0
-    s.lse_stride, s.k_rows, s.scale = q.shape[0], k.shape[0], float(scale)
-    return s
+        self.n_q_tiles, self.n_k_tiles = len(qt), len(kt)
 
 
 def _rows_like(rows, used, heads, hd, t):
@@ -1667,49 +1669,48 @@ def _rows_like(rows, used, heads, hd, t):
     return make((rows, heads, hd), dtype=t.dtype, device=t.device)
 
 
+def _causal_forward(q, k, v, plan, s):
+    o = _rows_like(s.lse_stride, plan.q_used, s.H, s.hd, q)
+    lse = torch.empty((s.H, s.lse_stride), dtype=torch.float32, device=q.device)
+    if plan.q_used != s.lse_stride:
+        lse.fill_(-math.inf)
+    _launch(lib().star_causal_fwd, "star_causal_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.seqs.data_ptr(),
+            plan.q_tiles.data_ptr(), plan.n_q_tiles, s, o.data_ptr(), lse.data_ptr())
+    return o, lse
+
+
 class _CausalAttn(torch.autograd.Function):
     """softmax(scale Q K^T, j <= i + nk - nq) V of packed sequences."""
 
     @staticmethod
-    def forward(ctx, q, k, v, plan, scale):
-        q, k, v = q.detach(), k.detach(), v.detach()
-        with _on(q.device):
-            o = _rows_like(q.shape[0], plan.q_used, q.shape[1], q.shape[2], q)
-            lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-            if plan.q_used != q.shape[0]:
-                lse.fill_(-math.inf)
-            s = _causal_shape(q, k, v, o, plan, scale)
-            check(lib().star_causal_fwd(ptr(q), ptr(k), ptr(v), ptr(plan.seqs), ptr(plan.q_tiles), plan.q_tiles.shape[0], s,
-                                        ptr(o), ptr(lse), stream_ptr()), "star_causal_fwd")
+    def forward(ctx, q, k, v, plan, s, need_lse):
+        o, lse = _causal_forward(q, k, v, plan, s)
         ctx.save_for_backward(q, k, v, o, lse)
-        ctx.plan, ctx.scale = plan, scale
+        ctx.plan, ctx.s = plan, s
+        if not need_lse:
+            return o
         ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
         return o, lse
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        if g is None:
-            return None, None, None, None, None
+    def backward(ctx, g, _=None):
+        if torch.is_grad_enabled():
+            raise _lib.StarNuggetError("causal_attn has no second derivative (backward with create_graph=True)")
         q, k, v, o, lse = ctx.saved_tensors
-        plan = ctx.plan
-        with _on(q.device):
-            g = g.to(q.dtype).contiguous()
-            if g.data_ptr() % 16:
-                g = g.clone()
-            dq = _rows_like(q.shape[0], plan.q_used, q.shape[1], q.shape[2], q)
-            dk = _rows_like(k.shape[0], plan.k_used, k.shape[1], k.shape[2], k)
-            dv = _rows_like(k.shape[0], plan.k_used, k.shape[1], k.shape[2], v)
-            delta = torch.empty_like(lse)
-            s = _causal_shape(q, k, v, o, plan, ctx.scale)
-            need = lib().star_causal_bwd_workspace(s, plan.k_tiles.shape[0])
-            ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-            check(lib().star_causal_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(g), ptr(lse), ptr(plan.seqs),
-                                        ptr(plan.q_tiles), plan.q_tiles.shape[0], ptr(plan.k_tiles), plan.k_tiles.shape[0],
-                                        s, ptr(dq), ptr(dk), ptr(dv), ptr(delta), ptr(ws), need, stream_ptr()),
-                  "star_causal_bwd")
-        return dq, dk, dv, None, None
+        plan, s, dev = ctx.plan, ctx.s, q.device
+        g = g.to(q.dtype).contiguous()
+        if g.data_ptr() % 16:
+            g = g.clone()
+        dq = _rows_like(s.lse_stride, plan.q_used, s.H, s.hd, q)
+        dk, dv = (_rows_like(s.k_rows, plan.k_used, s.Hkv, s.hd, t) for t in (k, v))
+        delta = torch.empty_like(lse)
+        need = lib().star_causal_bwd_workspace(s, plan.n_k_tiles) if s.H != s.Hkv else 0
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        _launch(lib().star_causal_bwd, "star_causal_bwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                g.data_ptr(), lse.data_ptr(), plan.seqs.data_ptr(), plan.q_tiles.data_ptr(), plan.n_q_tiles,
+                plan.k_tiles.data_ptr(), plan.n_k_tiles, s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+                ptr(ws), need)
+        return dq, dk, dv, None, None, None
 
 
 def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_lse: bool = False):
@@ -1725,22 +1726,31 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     dev = _same_device("causal_attn", q=q, k=k, v=v)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"causal_attn: [rows, heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape != v.shape or q.shape[2] != k.shape[2]:
+    rows, H, hd = q.shape
+    k_rows, Hkv, _ = k.shape
+    if k.shape != v.shape or hd != k.shape[2]:
         raise ValueError(f"causal_attn: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
     if not q.dtype == k.dtype == v.dtype:
         raise TypeError(f"causal_attn: q, k and v must share one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"causal_attn: {q.shape[1]} query heads do not divide into {k.shape[1]} key heads")
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    if Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"causal_attn: {H} query heads do not divide into {Hkv} key heads")
+    scale = hd ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"causal_attn: scale = {scale}; a positive number is required")
     if plan.device != dev:
         raise ValueError(f"causal_attn: the plan is on {plan.device}, the tensors on {dev}")
-    if q.shape[0] < plan.q_rows or k.shape[0] < plan.k_rows:
-        raise ValueError(f"causal_attn: the plan needs {plan.q_rows} query and {plan.k_rows} key rows, got {q.shape[0]} and {k.shape[0]}")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_rows("causal_attn", name, t)
-    o, lse = _CausalAttn.apply(q, k, v, plan, scale)
+    if rows < plan.q_rows or k_rows < plan.k_rows:
+        raise ValueError(f"causal_attn: the plan needs {plan.q_rows} query and {plan.k_rows} key rows, got {rows} and {k_rows}")
+    s = CausalShape()
+    s.q_sr, s.q_sh = _row_strides("causal_attn", "q", q)
+    s.k_sr, s.k_sh = _row_strides("causal_attn", "k", k)
+    s.v_sr, s.v_sh = _row_strides("causal_attn", "v", v)
+    s.o_sr, s.o_sh = H * hd, hd
+    s.H, s.Hkv, s.hd, s.dtype, s.nseq = H, Hkv, hd, _DT16[q.dtype], plan.n
+    s.lse_stride, s.k_rows, s.scale = rows, k_rows, scale
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CausalAttn.apply(q, k, v, plan, s, need_lse)
+    o, lse = _causal_forward(q, k, v, plan, s)
     return (o, lse) if need_lse else o
 
 
@@ -1802,6 +1812,7 @@ class KVCache8:
         self.batch, self.kv_heads, self.capacity, self.head_dim, self.dtype, self.device = B, H, T, hd, dt, dev
         self._dropped = torch.zeros(B, dtype=torch.int32, device=dev)
         self._tickets = torch.zeros(B * KV8_TICKET_STRIDE, dtype=torch.int32, device=dev)
+        self._workspace = {}                       # bytes of kv8_attn's workspace by (heads, queries)
         c = self._c = KV8Cache()
         c.B, c.Hkv, c.T, c.hd, c.dtype = B, H, T, hd, _DT16[dt]
         for n in self._PARTS:
@@ -1835,7 +1846,7 @@ class KVCache8:
         return torch.where(live, k, 0.0), torch.where(live, v, 0.0)
 
 
-def _i32(what, t, n, dev):
+def _i32(what, t, n):
     if t is None:
         return None
     if t.dim() != 1 or t.shape[0] != n:
@@ -1845,7 +1856,6 @@ def _i32(what, t, n, dev):
     return t.to(torch.int32).contiguous()
 
 
-@torch.no_grad()
 def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = None, at=None):
     """Append keys and values to an 8-bit cache.
 
@@ -1863,9 +1873,9 @@ def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = 
     if plan is None:
         if k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (B, H, hd):
             raise ValueError(f"kv8_append: [{B}, {H}, n, {hd}] expected, got {tuple(k.shape)}")
-        st = [k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2)]
-        dims = [B, H, k.shape[2]] * 2
-        counts, starts, step, most = _i32("kv8_append: counts", counts, B, dev), None, 1, k.shape[2]
+        counts, starts, step, most = _i32("kv8_append: counts", counts, B), None, 1, k.shape[2]
+        if k.numel():
+            st = _row_strides("kv8_append", "k", k) + _row_strides("kv8_append", "v", v)
     else:
         if counts is not None:
             raise ValueError("kv8_append: counts go with a batch, a plan has its own")
@@ -1875,19 +1885,17 @@ def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = 
             raise ValueError(f"kv8_append: a plan of {plan.n} sequences on {plan.device} for a cache of {B} on {dev}")
         if k.shape[0] < plan.k_rows:
             raise ValueError(f"kv8_append: the plan needs {plan.k_rows} rows, got {k.shape[0]}")
-        st = [0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0)]
-        dims = [1, H, k.shape[0]] * 2
         counts, starts, step, most = plan.counts, plan.starts, 4, plan.max_k
+        if k.numel():
+            (kr, kh), (vr, vh) = _row_strides("kv8_append", "k", k), _row_strides("kv8_append", "v", v)
+            st = 0, kh, kr, 0, vh, vr
     if most == 0 and at is None:
         return
-    if k.numel():
-        for name, t in (("k", k), ("v", v)):
-            _check_rows("kv8_append", name, t)
-    st = [s if n > 1 else 0 for s, n in zip(st, dims)]
-    at = _i32("kv8_append: at", at, B, dev)
-    with _on(dev):
-        check(lib().star_kv8_append(cache._c, ptr(k), ptr(v), *st, ptr(starts), ptr(counts), step, ptr(at), most,
-                                    stream_ptr()), "star_kv8_append")
+    if not k.numel():
+        st = (0,) * 6
+    at = _i32("kv8_append: at", at, B)
+    _launch(lib().star_kv8_append, "star_kv8_append", dev, cache._c, k.data_ptr(), v.data_ptr(), *st, ptr(starts), ptr(counts),
+            step, ptr(at), most)
 
 
 def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int = -1, bias=None,
@@ -1914,22 +1922,20 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
         if bias.dim() != 2 or bias.shape[0] != B or bias.shape[1] > cache.capacity:
             raise ValueError(f"kv8_attn: bias [{B}, at most {cache.capacity}] expected, got {tuple(bias.shape)}")
         bias = bias.detach().to(torch.float32).contiguous()
-    with _on(dev):
-        o = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev).permute(0, 2, 1, 3)
-        if L == 0:
-            return o
-        _check_rows("kv8_attn", "q", q)
-        s = KV8Query()
-        s.H, s.L = H, L
-        s.q_sb, s.q_sh, s.q_sr = (st if n > 1 else 0 for st, n in zip(q.stride()[:3], q.shape[:3]))
-        s.o_sb, s.o_sh, s.o_sr = L * H * hd, hd, H * hd
-        s.bias_len = 0 if bias is None else bias.shape[1]
-        s.causal, s.ilk_diag, s.scale = int(bool(causal)), int(ilk_diag), hd ** -0.5 if scale is None else float(scale)
-        q_len = _i32("kv8_attn: q_len", q_len, B, dev)
-        need = lib().star_kv8_attn_workspace(cache._c, H, L)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        check(lib().star_kv8_attn(cache._c, ptr(q), ptr(bias), ptr(q_len), s, ptr(o), ptr(ws), need, stream_ptr()),
-              "star_kv8_attn")
+    o = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev).permute(0, 2, 1, 3)
+    if L == 0:
+        return o
+    s = KV8Query()
+    s.q_sb, s.q_sh, s.q_sr = _row_strides("kv8_attn", "q", q)
+    s.H, s.L, s.o_sb, s.o_sh, s.o_sr = H, L, L * H * hd, hd, H * hd
+    s.bias_len = 0 if bias is None else bias.shape[1]
+    s.causal, s.ilk_diag, s.scale = int(bool(causal)), int(ilk_diag), hd ** -0.5 if scale is None else float(scale)
+    q_len = _i32("kv8_attn: q_len", q_len, B)
+    need = cache._workspace.get((H, L))
+    if need is None:
+        need = cache._workspace[H, L] = lib().star_kv8_attn_workspace(cache._c, H, L)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _launch(lib().star_kv8_attn, "star_kv8_attn", dev, cache._c, q.data_ptr(), ptr(bias), ptr(q_len), s, o.data_ptr(), ptr(ws), need)
     return o
 
 
