@@ -184,7 +184,10 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
 
 // ------------------------------------------------------------------------------------------------------ gradient of Q
 // The forward's walk with dP^T = V dO^T beside S^T = K Q^T; dQ^T += K^T dS^T with K read transposed from the same tile.
-// Also writes delta = rowsum(dO O) for the kernel below.
+// Also writes delta = rowsum(dO O) for the kernel below.  o has been rounded to 16 bits, which weighs most where a row
+// sees few keys and |o| is not small against |V|: with o's delta the error of dQ and dK was 1.55 times that of rounding
+// the exact gradients once.  A workgroup that sees at most two tiles of keys therefore walks them twice, first for
+// delta = sum_j P dP in 32 bits; its walk is the shortest there is.
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                           const T* __restrict__ V, const T* __restrict__ O,
@@ -234,7 +237,6 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
         sum += __shfl_xor(sum, 32, 64);
         dl[qb] = sum;
         l2[qb] = lse[(int64_t)h * s.lse_stride + row] * A_LOG2E;
-        if (g == 0 && i < sq.nq) delta[(int64_t)h * s.lse_stride + row] = sum;
     }
     const int all_see = w0 + 32 <= sq.nq ? max(0, min(sq.nk, w0 + off + 1)) : 0;
     const int wave_end = w0 < sq.nq ? max(0, min(sq.nk, min(w0 + 32, sq.nq) + off)) : 0;
@@ -255,19 +257,58 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
         kl.load(Kh, s.k_sr, 0, sq.nk, tid);
         vl.load(Vh, s.v_sr, 0, sq.nk, tid);
     }
+    if (ntile <= 2) {                                              // both tiles stay in LDS, each in its own half
+        float d[2] = {0.f, 0.f};
 #pragma unroll 1
-    for (int tile = 0; tile < ntile; ++tile) {
-        uint8_t* kt = smem + (tile & 1) * 2 * TB;
-        uint8_t* vt = kt + TB;
-        kl.store(kt, tid);
-        vl.store(vt, tid);
-        __syncthreads();
-        if (tile + 1 < ntile) {
-            kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
-            vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
+        for (int tile = 0; tile < ntile; ++tile) {
+            uint8_t* kt = smem + tile * 2 * TB;
+            uint8_t* vt = kt + TB;
+            kl.store(kt, tid);
+            vl.store(vt, tid);
+            __syncthreads();
+            if (tile + 1 < ntile) {
+                kl.load(Kh, s.k_sr, CK, sq.nk, tid);
+                vl.load(Vh, s.v_sr, CK, sq.nk, tid);
+            }
+#pragma unroll 1
+            for (int k4 = 0; k4 < 4; ++k4) {
+                f32x4 sc[2], dp[2];
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb) sc[qb] = dp[qb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const x8 kf = Ti::row8(kt, 16 * k4, ks, lane);
+                    const x8 vf = Ti::row8(vt, 16 * k4, ks, lane);
+#pragma unroll
+                    for (int qb = 0; qb < 2; ++qb) {
+                        sc[qb] = mfma16(kf, qf[qb][ks], sc[qb]);
+                        dp[qb] = mfma16(vf, gf[qb][ks], dp[qb]);
+                    }
+                }
+#pragma unroll
+                for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][i], c2, -l2[qb])) * dp[qb][i];
+                        d[qb] += tile * CK + 16 * k4 + 4 * g + i < lim[qb] ? p : 0.f;
+                    }
+            }
         }
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            d[qb] += __shfl_xor(d[qb], 16, 64);
+            d[qb] += __shfl_xor(d[qb], 32, 64);
+            dl[qb] = d[qb];
+        }
+    }
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+        const int i = w0 + 16 * qb + r16;
+        if (g == 0 && i < sq.nq) delta[(int64_t)h * s.lse_stride + sq.q0 + i] = dl[qb];
+    }
+    auto step = [&](int tile, const uint8_t* kt, const uint8_t* vt) {
         const int key0 = tile * CK;
-        if (key0 >= wave_end) continue;
+        if (key0 >= wave_end) return;
         const bool masked = key0 + CK > all_see;                   // (wave-uniform)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {                           // 32 keys at a time
@@ -320,6 +361,24 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 #pragma unroll
                 for (int qb = 0; qb < 2; ++qb) acc[qb][nt] = mfma16(kf, df[qb], acc[qb][nt]);
             }
+        }
+    };
+    if (ntile <= 2) {
+#pragma unroll 1
+        for (int tile = 0; tile < ntile; ++tile) step(tile, smem + tile * 2 * TB, smem + tile * 2 * TB + TB);
+    } else {
+#pragma unroll 1
+        for (int tile = 0; tile < ntile; ++tile) {
+            uint8_t* kt = smem + (tile & 1) * 2 * TB;
+            uint8_t* vt = kt + TB;
+            kl.store(kt, tid);
+            vl.store(vt, tid);
+            __syncthreads();
+            if (tile + 1 < ntile) {
+                kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
+                vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
+            }
+            step(tile, kt, vt);
         }
     }
 #pragma unroll

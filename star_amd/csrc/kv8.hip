@@ -231,6 +231,10 @@ __device__ __forceinline__ f16x8 widen<_Float16>(uint32_t lo, uint32_t hi, float
 template <typename T> struct VHalf { static constexpr float by = 1.f; };
 template <> struct VHalf<_Float16> { static constexpr float by = 0.5f; };
 
+// The codes are read once: past the caches (four sequences of up to 131072 tokens, 1.0 GB: 183 -> 161 us)
+template <typename V>
+__device__ __forceinline__ V once(const V* p) { return __builtin_nontemporal_load(p); }
+
 // Wave w of a workgroup takes the blocks w, w + 4, ... of its part for RT * 16 rows (a row is one query of one head of
 // the group); the four softmax states are joined through LDS at the end.  Token of the MFMA: row rho of K tile t is
 // token 16 * (rho / 4) + 4 t + rho % 4, so lane group g ends up with the weights of the tokens 16 g .. 16 g + 15, which
@@ -373,11 +377,11 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int cc = 0; cc < C64; ++cc) kr[t][cc] = *(const u32x4*)(kb + (krow + 4 * t) * HD + 64 * cc + 16 * g);
-            if constexpr (ODD) ko[t] = *(const u32x2*)(kb + (krow + 4 * t) * HD + 64 * C64 + 8 * g);
+            for (int cc = 0; cc < C64; ++cc) kr[t][cc] = once((const u32x4*)(kb + (krow + 4 * t) * HD + 64 * cc + 16 * g));
+            if constexpr (ODD) ko[t] = once((const u32x2*)(kb + (krow + 4 * t) * HD + 64 * C64 + 8 * g));
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) vr[nt] = *(const u32x4*)(vb + (16 * nt + r16) * KB + 16 * g);
+        for (int nt = 0; nt < NT; ++nt) vr[nt] = once((const u32x4*)(vb + (16 * nt + r16) * KB + 16 * g));
         ks_ = ksc[blk];
         vs_ = vsc[blk];
     };
@@ -507,9 +511,9 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
     }
 }
 
-// One wave per row that was cut into parts.
+// A row that was cut into few parts: one wave adds them up.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void kv8_join_few_kernel(AttnArgs a) {
     const int lane = threadIdx.x & 63;
     const star_kv8_cache& c = a.c;
     const int grp = a.s.H / c.Hkv, rows = grp * a.s.L;
@@ -530,6 +534,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
     float ll = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 2
     for (int p = 0; p < np; ++p) {
         const int64_t at = at0 + p * stride;
         const float f = __builtin_amdgcn_exp2f(ml[2 * at] - mm);
@@ -541,6 +546,66 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs a) {
     T* orow = (T*)a.o + (int64_t)b * a.s.o_sb + (int64_t)(hk * grp + rho % grp) * a.s.o_sh + (int64_t)(rho / grp) * a.s.o_sr;
     orow[lane] = (T)(o0 * inv);
     if (lane + 64 < HD) orow[64 + lane] = (T)(o1 * inv);
+}
+
+// Many parts: one workgroup a row, the parts' factors first, one per thread, then every thread adds the
+// parts of four values, PG of them at a time with all loads in flight.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs a) {
+    constexpr int D4 = HD / 4, PG = 256 / D4;                       // threads of a part, parts at a time
+    constexpr int MOST = 256;
+    __shared__ float fsh[MOST], red[8];
+    __shared__ __attribute__((aligned(16))) float osh[PG * HD];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const star_kv8_cache& c = a.c;
+    const int grp = a.s.H / c.Hkv, rows = grp * a.s.L;
+    const int64_t item = blockIdx.x;
+    const int b = (int)(item / ((int64_t)c.Hkv * rows)), hk = (int)(item / rows % c.Hkv), rho = (int)(item % rows);
+    const int per = cut(a, lane).per;
+    const int np = parts_of(blocks_of(a, b), per);
+    if (np == 1) return;
+    int base = 0;
+    for (int b0 = 0; b0 < b; b0 += 64) base += b0 + lane < b ? parts_of(blocks_of(a, b0 + lane), per) : 0;
+    base = wave_sum(base);
+    const float* ml = a.part + (int64_t)a.slots * c.Hkv * rows * HD;
+    const int64_t stride = (int64_t)c.Hkv * rows, at0 = (int64_t)base * stride + (int64_t)hk * rows + rho;
+    float mm = M_NONE;
+    for (int p = tid; p < np; p += 256) mm = fmaxf(mm, ml[2 * (at0 + p * stride)]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
+    if (lane == 0) red[wid] = mm;
+    __syncthreads();
+    mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const int d4 = tid % D4, pg = tid / D4;
+    f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float ll = 0.f;
+    for (int p0 = 0; p0 < np; p0 += MOST) {
+        const int cnt = min(np - p0, MOST);
+        __syncthreads();
+        if (tid < cnt) {
+            const int64_t at = at0 + (p0 + tid) * stride;
+            const float f = __builtin_amdgcn_exp2f(ml[2 * at] - mm);
+            fsh[tid] = f;
+            ll += f * ml[2 * at + 1];
+        }
+        __syncthreads();
+        if (pg < PG) {
+#pragma unroll 4
+            for (int p = pg; p < cnt; p += PG) o += fsh[p] * *(const f32x4*)(a.part + (at0 + (p0 + p) * stride) * HD + 4 * d4);
+        }
+    }
+    ll = wave_sum(ll);
+    if (lane == 0) red[4 + wid] = ll;
+    if (pg < PG) *(f32x4*)(osh + pg * HD + 4 * d4) = o;
+    __syncthreads();
+    if (tid >= HD) return;
+    ll = (red[4] + red[5]) + (red[6] + red[7]);
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < PG; ++p) sum += osh[p * HD + tid];
+    const float inv = (ll > 0.f ? 1.0f / ll : ll) / VHalf<T>::by;
+    T* orow = (T*)a.o + (int64_t)b * a.s.o_sb + (int64_t)(hk * grp + rho % grp) * a.s.o_sh + (int64_t)(rho / grp) * a.s.o_sr;
+    orow[tid] = (T)(sum * inv);
 }
 
 // ------------------------------------------------------------------------------------------------------ host side
@@ -559,12 +624,14 @@ static int check_cache(const star_kv8_cache* c, const char* who) {
 
 // rows of one workgroup: 16 while they suffice, else as many as keep the codes' conversion cheap against the products
 static int row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// (sequence, part) pairs that the grid has room for.  512 workgroups (two a CU) run at once: few sequences are cut into
+// parts that fill these places once; where the sequences alone make half of them or more, there is room for three times
+// as many parts besides, so that a sequence much longer than the others does not run alone at the end.
 static int attn_slots(const star_kv8_cache* c, int H, int L) {
     const int rows = H / c->Hkv * L, nrg = cdiv(rows, 16 * row_tiles(rows));
-    const int64_t target = 256 * 4;                                 // workgroups: four per CU
-    const int64_t most = (int64_t)c->B * cdiv(c->T / KB, MIN_PART);
-    const int64_t s = target / ((int64_t)c->Hkv * nrg);
-    return (int)max((int64_t)c->B, s < most ? s : most);
+    const int64_t places = 512 / ((int64_t)c->Hkv * nrg), most = (int64_t)c->B * cdiv(c->T / KB, MIN_PART);
+    const int64_t s = places >= 2 * c->B ? places : c->B + 3 * (places > 1 ? places : 1);
+    return (int)(s < most ? s : most);
 }
 
 #define KV8_BY_TYPE(DT, HDIM, CALL)                                                        \
@@ -586,8 +653,11 @@ static void launch_attn(const AttnArgs& a, int rt, hipStream_t st) {
     if (rt == 1) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 1>), grid, dim3(256), 0, st, a);
     else if (rt == 2) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 2>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 4>), grid, dim3(256), 0, st, a);
-    if (a.slots > a.c.B)
-        hipLaunchKernelGGL((kv8_join_kernel<T, HD>), dim3((unsigned)(((int64_t)a.c.B * a.s.H * a.s.L + 3) / 4)), dim3(256), 0, st, a);
+    if (a.slots == a.c.B) return;
+    // (measured at 32 heads: 2 parts on average 4.9 us by waves, 8.3 by workgroups; 32 parts 19 and 7.4)
+    const int64_t rows = (int64_t)a.c.B * a.s.H * a.s.L;
+    if (a.slots <= 8 * a.c.B) hipLaunchKernelGGL((kv8_join_few_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_join_kernel<T, HD>), dim3((unsigned)rows), dim3(256), 0, st, a);
 }
 
 }  // namespace star
