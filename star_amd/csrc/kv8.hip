@@ -77,68 +77,97 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     uint8_t* codes = (is_v ? c.v_codes : c.k_codes) + bh * c.T * HD;
     float* scales = (is_v ? c.v_scales : c.k_scales) + bh * (c.T / KB);
 
-    for (int blk = first + blockIdx.x; blk < last; blk += gridDim.x) {
-        const int held = max(0, at - blk * KB);                     // tokens of the block that lie in the open block's rows
-        // rows across the lanes where V's open block (transposed) is read, chunks across the lanes else
-        const bool turned = is_v && held > 0;
-        x8 x[N];
-        int row[N], ch[N];
-        float m = 0.f;
+    // chunk i of this thread: a row's chunks across the lanes, or (turned) the rows of a chunk
+    auto row_of = [&](int i, bool turned) { return turned ? (tid + 256 * i) % KB : (tid + 256 * i) / CH; };
+    auto ch_of = [&](int i, bool turned) { return turned ? (tid + 256 * i) / KB : (tid + 256 * i) % CH; };
+    // (32-bit byte offsets from a scalar address: 63 rows of sr < 2^23 values)
+    auto load = [&](x8 (&x)[N], int blk) {
+        const char* from = (const char*)(src + (int64_t)(blk * KB - at) * sr);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = *(const x8*)(from + ((uint32_t)row_of(i, false) * (uint32_t)sr + 8 * ch_of(i, false)) * 2);
+    };
+    // the block that was open: its first `held` tokens lie in the open block's rows, V transposed
+    auto load_opened = [&](x8 (&x)[N], int blk) {
+        const int held = at - blk * KB;
+        const char* from = (const char*)src - (int64_t)held * sr * 2;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int q = tid + 256 * i;
-            row[i] = turned ? q % KB : q / CH;
-            ch[i] = turned ? q / KB : q % CH;
-            if (row[i] >= held) x[i] = *(const x8*)(src + (int64_t)(blk * KB + row[i] - at) * sr + 8 * ch[i]);
-            else if (!is_v) x[i] = *(const x8*)(tail + row[i] * HD + 8 * ch[i]);
+            const int row = row_of(i, is_v), ch = ch_of(i, is_v);
+            if (row >= held) x[i] = *(const x8*)(from + ((uint32_t)row * (uint32_t)sr + 8 * ch) * 2);
+            else if (!is_v) x[i] = *(const x8*)((const char*)tail + (uint32_t)(row * HD + 8 * ch) * 2);
             else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = tail[(8 * ch[i] + e) * KB + row[i]];
+                for (int e = 0; e < 8; ++e) x[i][e] = *(const T*)((const char*)tail + (uint32_t)((8 * ch + e) * KB + row) * 2);
             }
         }
+    };
+    auto write = [&](const x8 (&x)[N], int blk, bool turned) {
+        float m = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs((float)x[i][e]));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        __syncthreads();                                            // wmax and vt are free
         if (lane == 0) wmax[wid] = m;
         __syncthreads();                                            // (also: every read of the open block's rows is done)
         m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
         const float sc = block_scale(m), inv = 1.0f / sc;           // (exact: powers of two between 2^-126 and 2^120)
         uint8_t* out = codes + (int64_t)blk * KB * HD;
+        if (tid == 0) scales[blk] = sc;
         if (!is_v) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) *(u32x2*)(out + row[i] * HD + 8 * ch[i]) = codes8(x[i], inv);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const u32x2 w = codes8(x[i], inv);
-                *(uint32_t*)(vt + row[i] * VP + 8 * ch[i]) = w[0];
-                *(uint32_t*)(vt + row[i] * VP + 8 * ch[i] + 4) = w[1];
-            }
-            __syncthreads();
-            for (int q = tid; q < 2 * HD; q += 256) {               // 8 tokens x 4 dimensions each
-                const int t8 = q & 7, d4 = q >> 3;
-                uint32_t w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = *(const uint32_t*)(vt + (8 * t8 + i) * VP + 4 * d4);
-                u32x2 o[4];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint32_t lo01 = __builtin_amdgcn_perm(w[4 * p + 1], w[4 * p], 0x05010400), lo23 = __builtin_amdgcn_perm(w[4 * p + 3], w[4 * p + 2], 0x05010400);
-                    const uint32_t hi01 = __builtin_amdgcn_perm(w[4 * p + 1], w[4 * p], 0x07030602), hi23 = __builtin_amdgcn_perm(w[4 * p + 3], w[4 * p + 2], 0x07030602);
-                    o[0][p] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100);
-                    o[1][p] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302);
-                    o[2][p] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100);
-                    o[3][p] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) *(u32x2*)(out + (4 * d4 + k) * KB + 8 * t8) = o[k];
-            }
+            for (int i = 0; i < N; ++i) *(u32x2*)(out + row_of(i, false) * HD + 8 * ch_of(i, false)) = codes8(x[i], inv);
+            return;
         }
-        if (tid == 0) scales[blk] = sc;
-        __syncthreads();                                            // wmax and vt are free again
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const u32x2 w = codes8(x[i], inv);
+            uint8_t* to = vt + row_of(i, turned) * VP + 8 * ch_of(i, turned);
+            *(uint32_t*)to = w[0];
+            *(uint32_t*)(to + 4) = w[1];
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int q = tid; q < 2 * HD; q += 256) {                   // 8 tokens x 4 dimensions each
+            const int t8 = q & 7, d4 = q >> 3;
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = *(const uint32_t*)(vt + (8 * t8 + i) * VP + 4 * d4);
+            uint8_t* to = out + 4 * d4 * KB + 8 * t8;
+            u32x2 o0, o1, o2, o3;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t lo01 = __builtin_amdgcn_perm(w[4 * p + 1], w[4 * p], 0x05010400), lo23 = __builtin_amdgcn_perm(w[4 * p + 3], w[4 * p + 2], 0x05010400);
+                const uint32_t hi01 = __builtin_amdgcn_perm(w[4 * p + 1], w[4 * p], 0x07030602), hi23 = __builtin_amdgcn_perm(w[4 * p + 3], w[4 * p + 2], 0x07030602);
+                o0[p] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100);
+                o1[p] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302);
+                o2[p] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100);
+                o3[p] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302);
+            }
+            *(u32x2*)to = o0;
+            *(u32x2*)(to + KB) = o1;
+            *(u32x2*)(to + 2 * KB) = o2;
+            *(u32x2*)(to + 3 * KB) = o3;
+        }
+    };
+    int blk = first + blockIdx.x;
+    if (blk < last && blk * KB < at) {
+        x8 x[N];
+        load_opened(x, blk);
+        write(x, blk, is_v);
+        blk += gridDim.x;
+    }
+    if (blk < last) {
+        x8 x[N], next[N];
+        load(x, blk);
+        for (; blk < last; blk += gridDim.x) {
+            if (blk + (int)gridDim.x < last) load(next, blk + gridDim.x);
+            write(x, blk, false);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = next[i];
+        }
     }
     if (blockIdx.x == 0) {
         const int from = max(at, last * KB), cnt = end - from, r0 = from - last * KB;   // new rows of the open block
@@ -674,8 +703,12 @@ extern "C" int star_kv8_append(const star_kv8_cache* c, const void* k, const voi
     const int64_t sd[6] = {k_sb, k_sh, k_sr, v_sb, v_sh, v_sr};
     for (int i = 0; i < 6; ++i) STAR_REQUIRE(sd[i] % 8 == 0, "star_kv8_append: strides must be multiples of 8 elements");
     AppendArgs a{*c, k, v, k_sb, k_sh, k_sr, v_sb, v_sh, v_sr, starts, counts, at, idx_stride, max_rows};
-    // a call of n rows completes at most (n + 63) / 64 blocks, and never more than the cache has
-    const int gx = max(1, min(min(cdiv((int64_t)max_rows + KB - 1, KB), c->T / KB), 4096));
+    STAR_REQUIRE(k_sr >= 0 && k_sr < (1ll << 23) && v_sr >= 0 && v_sr < (1ll << 23), "star_kv8_append: row strides %lld, %lld not in [0, 2^23)",
+                 (long long)k_sr, (long long)v_sr);
+    // A call of n rows completes at most (n + 63) / 64 blocks, and never more than the cache has.  4096 workgroups in all
+    // (16 a CU) take them in turn, the next block's rows on their way while one is written: 32 prompts of up to 4000
+    // tokens 168 us with a workgroup for every block, 110 with these
+    const int gx = max(1, min(min(cdiv((int64_t)max_rows + KB - 1, KB), c->T / KB), 4096 / (2 * c->Hkv * c->B)));
     const dim3 grid(gx, 2 * c->Hkv, c->B);
     KV8_BY_TYPE(c->dtype, c->hd, hipLaunchKernelGGL((kv8_append_kernel<T, HD>), grid, dim3(256), 0, (hipStream_t)stream, a));
     STAR_LAUNCH_CHECK("star_kv8_append");
