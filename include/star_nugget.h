@@ -470,6 +470,7 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
 #define STAR_CAUSAL_TILE 128
 typedef struct {
     int H, Hkv, hd, dtype, nseq;
+    int max_q;                  /* queries of the longest sequence */
     int64_t q_sr, q_sh, k_sr, k_sh, v_sr, v_sh, o_sr, o_sh;
     int64_t lse_stride;
     int64_t k_rows;             /* rows of k, v, dk and dv */

@@ -182,6 +182,166 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
     }
 }
 
+// The same for sequences of at most 16 * QB queries each (a chunk of a stream, a speculated run of tokens): the waves of
+// a workgroup share the queries and take the 64-key tiles in turn, each with K straight from memory in registers (its
+// rows are the operand) and V through an LDS tile of its own, so no wave waits for another before the four softmax states
+// are joined at the end.  Bound by the latency of two dependent trips to memory per 256 keys: one utterance of 375 frames,
+// 16 queries, 8 heads of 128 takes 8.4 us, 13.1 with the kernel above, whose waves would share keys and leave three of
+// four without a query.
+template <typename T, int HD, int QB>
+__global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                           const T* __restrict__ V, const int32_t* __restrict__ seqs,
+                                                           const int32_t* __restrict__ tiles, star_causal_shape s,
+                                                           T* __restrict__ O, float* __restrict__ lse) {
+    typedef typename Vec<T>::x8 x8;
+    using Ti = Tile<T, HD>;
+    constexpr int KS = HD / 32, NT = HD / 16, OP = HD + 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ float msh[4 * 16 * QB], lsh[4 * 16 * QB];
+
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
+    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const int off = sq.nk - sq.nq, end = max(0, sq.nk);            // (the last query sees every key)
+    const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
+    const T* Vh = V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh;
+    int lim[QB];
+    x8 qf[QB][KS];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int i = 16 * qb + r16;
+        lim[qb] = i < sq.nq ? max(0, min(sq.nk, i + off + 1)) : 0;
+        const T* row = Q + (int64_t)(sq.q0 + min(i, sq.nq - 1)) * s.q_sr + (int64_t)h * s.q_sh + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[qb][ks] = *(const x8*)(row + 32 * ks);
+    }
+    const int all_see = sq.nq == 16 * QB ? max(0, off + 1) : 0;
+    const float c2 = s.scale * A_LOG2E;
+    f32x4 acc[QB][NT];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[qb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        m[qb] = M_NONE;
+        l[qb] = 0.f;
+    }
+    uint8_t* vt = smem + wid * CK * Ti::ROWB;
+#pragma unroll 1
+    for (int key0 = wid * CK; key0 < end; key0 += 4 * CK) {
+        TileLoad<T, HD, CK, 64> vl;
+        vl.place(s.v_sr, lane);
+        vl.load(Vh, s.v_sr, key0, sq.nk, lane);
+        f32x4 sc[QB][4];
+#pragma unroll
+        for (int kt4 = 0; kt4 < 4; ++kt4) {
+            const T* row = Kh + (int64_t)min(key0 + 16 * kt4 + r16, sq.nk - 1) * s.k_sr + 8 * g;
+            x8 kf[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const x8*)(row + 32 * ks);
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+                sc[qb][kt4] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) sc[qb][kt4] = mfma16(kf[ks], qf[qb][ks], sc[qb][kt4]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();                           // (the reads of the tile before are behind: LDS is in order)
+        vl.store(vt, lane);
+        __builtin_amdgcn_wave_barrier();
+        if (key0 + CK > all_see) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[qb][kt4][i] = key0 + 16 * kt4 + 4 * g + i < lim[qb] ? sc[qb][kt4][i] : -INFINITY;
+        }
+        x8 pf[QB][2];
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            float mx = sc[qb][0][0];
+#pragma unroll
+            for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[qb][kt4][i]);
+            mx *= c2;
+            if (!__all(mx <= m[qb] + M_SLACK)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m[qb], mx), a = __builtin_amdgcn_exp2f(m[qb] - mn);
+                m[qb] = mn;
+                l[qb] *= a;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[qb][nt][i] *= a;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][kt4][i], c2, -m[qb]));
+                    sum += p;
+                    sc[qb][kt4][i] = p;
+                }
+            l[qb] += sum;
+            pf[qb][0] = pack_b<T>(sc[qb][0], sc[qb][1]);
+            pf[qb][1] = pack_b<T>(sc[qb][2], sc[qb][3]);
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const x8 vf = Ti::tr8(vt, 32 * hf, nt, lane);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) acc[qb][nt] = mfma16(vf, pf[qb][hf], acc[qb][nt]);
+            }
+    }
+    // join the four waves
+    float* osh = (float*)smem;                                     // [4][16 * QB][OP], over the tiles
+    __syncthreads();
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        float sum = l[qb];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        const int row = (wid * QB + qb) * 16 + r16;
+        if (g == 0) {
+            msh[row] = m[qb];
+            lsh[row] = sum;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) *(f32x4*)(osh + row * OP + 16 * nt + 4 * g) = acc[qb][nt];
+    }
+    __syncthreads();
+    constexpr int PER = HD / 16;
+    for (int row = tid >> 4; row < min(sq.nq, 16 * QB); row += 16) {
+        const int d0 = (tid & 15) * PER;
+        float mm = M_NONE, ll = 0.f, o[PER];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, msh[w * 16 * QB + row]);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(msh[w * 16 * QB + row] - mm);
+            ll += f * lsh[w * 16 * QB + row];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[e] += f * osh[(w * 16 * QB + row) * OP + d0 + e];
+        }
+        const float inv = ll > 0.f ? 1.0f / ll : ll;               // no visible key: 0; NaN stays NaN
+        T* orow = O + (int64_t)(sq.q0 + row) * s.o_sr + (int64_t)h * s.o_sh + d0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) orow[e] = (T)(o[e] * inv);
+        if ((tid & 15) == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + row] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------ gradient of Q
 // The forward's walk with dP^T = V dO^T beside S^T = K Q^T; dQ^T += K^T dS^T with K read transposed from the same tile.
 // Also writes delta = rowsum(dO O) for the kernel below.  o has been rounded to 16 bits, which weighs most where a row
@@ -621,7 +781,7 @@ static int check_causal(const star_causal_shape* s, const char* who) {
     STAR_REQUIRE(s->hd == 64 || s->hd == 96 || s->hd == 128, "%s: head dim %d not in {64, 96, 128}", who, s->hd);
     STAR_REQUIRE(s->dtype == STAR_DT_BF16 || s->dtype == STAR_DT_F16, "%s: dtype %d is neither bf16 nor fp16", who, s->dtype);
     STAR_REQUIRE(s->Hkv >= 1 && s->H >= s->Hkv && s->H % s->Hkv == 0, "%s: %d query heads do not divide into %d key heads", who, s->H, s->Hkv);
-    STAR_REQUIRE(s->nseq >= 0 && s->lse_stride >= 0 && s->k_rows >= 0, "%s: negative size", who);
+    STAR_REQUIRE(s->nseq >= 0 && s->max_q >= 0 && s->lse_stride >= 0 && s->k_rows >= 0, "%s: negative size", who);
     const int64_t st[8] = {s->q_sr, s->q_sh, s->k_sr, s->k_sh, s->v_sr, s->v_sh, s->o_sr, s->o_sh};
     for (int i = 0; i < 8; ++i) STAR_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
     for (int i = 0; i < 8; i += 2)
@@ -631,9 +791,25 @@ static int check_causal(const star_causal_shape* s, const char* who) {
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+template <typename T, int HD, int QB>
+static int launch_causal_few(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+                             int ntiles, const star_causal_shape* s, void* o, float* lse, hipStream_t st) {
+    constexpr int tile = 4 * CK * Tile<T, HD>::ROWB, join = 4 * 16 * QB * (HD + 4) * 4, smem = tile > join ? tile : join;
+    static DevOnce once;
+    if (!reserve_lds_once(once, (const void*)causal_few_kernel<T, HD, QB>, smem)) {
+        set_error("star_causal_fwd: cannot reserve %d bytes of LDS", smem);
+        return STAR_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL((causal_few_kernel<T, HD, QB>), dim3((unsigned)ntiles * s->H), dim3(256), smem, st, (const T*)q, (const T*)k,
+                       (const T*)v, seqs, tiles, *s, (T*)o, lse);
+    return STAR_OK;
+}
+
 template <typename T, int HD>
 static int launch_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
                              int ntiles, const star_causal_shape* s, void* o, float* lse, hipStream_t st) {
+    if (s->max_q <= 16) return launch_causal_few<T, HD, 1>(q, k, v, seqs, tiles, ntiles, s, o, lse, st);
+    if (s->max_q <= 32) return launch_causal_few<T, HD, 2>(q, k, v, seqs, tiles, ntiles, s, o, lse, st);
     constexpr int smem = 4 * CK * Tile<T, HD>::ROWB;
     static DevOnce once;
     if (!reserve_lds_once(once, (const void*)causal_fwd_kernel<T, HD>, smem)) {

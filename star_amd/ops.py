@@ -1746,7 +1746,7 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     s.k_sr, s.k_sh = _row_strides("causal_attn", "k", k)
     s.v_sr, s.v_sh = _row_strides("causal_attn", "v", v)
     s.o_sr, s.o_sh = H * hd, hd
-    s.H, s.Hkv, s.hd, s.dtype, s.nseq = H, Hkv, hd, _DT16[q.dtype], plan.n
+    s.H, s.Hkv, s.hd, s.dtype, s.nseq, s.max_q = H, Hkv, hd, _DT16[q.dtype], plan.n, plan.max_q
     s.lse_stride, s.k_rows, s.scale = rows, k_rows, scale
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CausalAttn.apply(q, k, v, plan, s, need_lse)

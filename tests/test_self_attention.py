@@ -81,6 +81,9 @@ SHAPES = [  # keys, queries (None: the same), H, Hkv, hd, dtype
     ([700, 65, 0], [1, 64, 0], 4, 4, 64, BF),
     ([40, 3, 0], [100, 130, 5], 2, 2, 128, BF),            # more queries than keys: the first see nothing
     ([1000], None, 12, 4, 128, BF),
+    ([3, 700, 64, 0, 257], [16, 1, 9, 2, 16], 4, 2, 128, BF),  # few queries each: the waves share them
+    ([520, 5, 1], [30, 17, 1], 2, 1, 64, FP),
+    ([100, 300], [32, 20], 3, 3, 96, BF),
 ]
 
 
