@@ -589,11 +589,10 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     uint8_t* vt = smem + 32 * wid * Ti::ROWB;                      // the wave's rows of V
 
     x8 kf[2][KS];
-    int see[2];                                                    // first query that sees this lane's key
+    const int see = w0 + r16 - off;                                // first query that sees this lane's key of block 0
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
         const int j = w0 + 16 * kb + r16;
-        see[kb] = j < sq.nk ? j - off : 0x7fffffff;
         const T* kr = K + (int64_t)(sq.k0 + min(j, sq.nk - 1)) * s.k_sr + (int64_t)hk * s.k_sh + 8 * g;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kf[kb][ks] = *(const x8*)(kr + 32 * ks);
@@ -612,7 +611,7 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     const float c2 = s.scale * A_LOG2E;
     const int first = max(0, j0 - off) / CQ;                       // query tiles before it see none of these keys
     const int nper = max(0, (sq.nq + CQ - 1) / CQ - first);        // tiles per head
-    const int all_see = w0 + 32 <= sq.nk ? w0 + 31 - off : 0x7fffffff;  // from this query on every key of the wave is visible
+    const int all_see = w0 + 31 - off;                             // from this query on every key of the wave is visible
 
     TileLoad<T, HD, CQ, 256> ql, gl;
     float lr = 0.f;
@@ -620,7 +619,10 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     auto load = [&]() {
         ql.load(Q + (int64_t)sq.q0 * s.q_sr + (int64_t)lh * s.q_sh, s.q_sr, lq, sq.nq, tid);
         gl.load(dO + (int64_t)sq.q0 * s.o_sr + (int64_t)lh * s.o_sh, s.o_sr, lq, sq.nq, tid);
-        if (tid < 2 * CQ) lr = (tid < CQ ? lse : delta)[(int64_t)lh * s.lse_stride + sq.q0 + min(lq + (tid & (CQ - 1)), sq.nq - 1)];
+        if (wid < 2 && lane < CQ) {
+            const float* p = (wid == 0 ? lse : delta) + (int64_t)lh * s.lse_stride + sq.q0 + lq;
+            lr = p[min(lane, sq.nq - 1 - lq)];
+        }
         lq += CQ;
         if (lq >= sq.nq) { lq = first * CQ; ++lh; }
     };
@@ -636,8 +638,7 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
         float* lt = (float*)(gt + TB);
         ql.store(qt, tid);
         gl.store(gt, tid);
-        if (tid < CQ) lt[tid] = lr * A_LOG2E;
-        else if (tid < 2 * CQ) lt[tid] = lr;
+        if (wid < 2 && lane < CQ) lt[wid * CQ + lane] = wid == 0 ? lr * A_LOG2E : lr;
         __syncthreads();
         if (n + 1 < ntile) load();
         const int qa0 = q0;
@@ -645,54 +646,66 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
         if (q0 >= sq.nq) q0 = first * CQ;
         if (qa0 + CQ <= w0 - off) continue;                        // (wave-uniform) no query of the tile sees a key of the wave
         const bool masked = qa0 < all_see || qa0 + CQ > sq.nq;
+        // both 16-query halves at once: the fragments of V are read once for them
         x4 pp[2][2], ds[2][2];
+        f32x4 sc[2][2], dp[2][2];
 #pragma unroll
-        for (int q2 = 0; q2 < 2; ++q2) {
-            __builtin_amdgcn_sched_barrier(0);
-            f32x4 sc[2], dp[2];
+        for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) sc[kb] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int kb = 0; kb < 2; ++kb) sc[q2][kb] = dp[q2][kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
+        for (int ks = 0; ks < KS; ++ks) {
+            x8 vf[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) vf[kb] = Ti::row8(vt, 16 * kb, ks, lane);
+#pragma unroll
+            for (int q2 = 0; q2 < 2; ++q2) {
                 const x8 qa = Ti::row8(qt, 16 * q2, ks, lane);
                 const x8 ga = Ti::row8(gt, 16 * q2, ks, lane);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
-                    sc[kb] = mfma16(qa, kf[kb][ks], sc[kb]);
-                    dp[kb] = mfma16(ga, Ti::row8(vt, 16 * kb, ks, lane), dp[kb]);
+                    sc[q2][kb] = mfma16(qa, kf[kb][ks], sc[q2][kb]);
+                    dp[q2][kb] = mfma16(ga, vf[kb], dp[q2][kb]);
                 }
             }
+        }
+#pragma unroll
+        for (int q2 = 0; q2 < 2; ++q2) {
             const f32x4 ls = *(const f32x4*)(lt + 16 * q2 + 4 * g);
             const f32x4 de = *(const f32x4*)(lt + CQ + 16 * q2 + 4 * g);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[kb][i] = __builtin_fmaf(sc[kb][i], c2, -ls[i]);
-                    dp[kb][i] -= de[i];
+                    sc[q2][kb][i] = __builtin_fmaf(sc[q2][kb][i], c2, -ls[i]);
+                    dp[q2][kb][i] -= de[i];
                 }
-            if (masked) {
+        }
+        if (masked) {
+#pragma unroll
+            for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int qi = qa0 + 16 * q2 + 4 * g + i;
-                        const bool vis = qi >= see[kb] && qi < sq.nq;
-                        sc[kb][i] = vis ? sc[kb][i] : -INFINITY;
-                        dp[kb][i] = vis ? dp[kb][i] : 0.f;
+                        const bool vis = qi >= see + 16 * kb && qi < sq.nq;
+                        sc[q2][kb][i] = vis ? sc[q2][kb][i] : -INFINITY;
+                        dp[q2][kb][i] = vis ? dp[q2][kb][i] : 0.f;
                     }
-            }
+        }
+#pragma unroll
+        for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[kb][i] = __builtin_amdgcn_exp2f(sc[kb][i]);
-                    dp[kb][i] *= sc[kb][i];
+                    sc[q2][kb][i] = __builtin_amdgcn_exp2f(sc[q2][kb][i]);
+                    dp[q2][kb][i] *= sc[q2][kb][i];
                 }
-                pp[kb][q2] = pack4<T>(sc[kb]);
-                ds[kb][q2] = pack4<T>(dp[kb]);
+                pp[kb][q2] = pack4<T>(sc[q2][kb]);
+                ds[kb][q2] = pack4<T>(dp[q2][kb]);
             }
-        }
         __builtin_amdgcn_sched_barrier(0);
         x8 pf[2], df[2];
 #pragma unroll
