@@ -655,6 +655,8 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
             for (int kb = 0; kb < 2; ++kb) sc[q2][kb] = dp[q2][kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
+            // (head dim 96: the reads of all steps at once would not fit the registers)
+            if constexpr (HD == 96) __builtin_amdgcn_sched_barrier(0);
             x8 vf[2];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) vf[kb] = Ti::row8(vt, 16 * kb, ks, lane);
