@@ -474,12 +474,13 @@ typedef struct {
     int64_t q_sr, q_sh, k_sr, k_sh, v_sr, v_sh, o_sr, o_sh;
     int64_t lse_stride;
     int64_t k_rows;             /* rows of k, v, dk and dv */
+    int64_t dq_sr, dkv_sr;      /* row strides of dq, and of dk and dv (their heads are dense) */
     float scale;
 } star_causal_shape;
 int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles, int ntiles,
                     const star_causal_shape* s, void* o, float* lse, void* stream);
-/* Backward: P recomputed from lse.  do_ has o's strides; dq [rows,H,hd] and dk / dv [rows,Hkv,hd] are dense.  q_tiles as
- * tiles above; k_tiles [nk_tiles][2]: the same for tiles of STAR_CAUSAL_TILE keys.  delta [H][lse_stride] fp32 scratch.
+/* Backward: P recomputed from lse.  do_ has o's strides; dq [rows,H,hd] and dk / dv [rows,Hkv,hd] may be column
+ * ranges of one matrix (dq_sr, dkv_sr, multiples of 8).  q_tiles as tiles above; k_tiles [nk_tiles][2]: the same for tiles of STAR_CAUSAL_TILE keys.  delta [H][lse_stride] fp32 scratch.
  * No atomics: the gradient of a shared key head is summed over its query heads in a fixed order.
  * workspace: star_causal_bwd_workspace(s, nk_tiles) bytes (0 for most calls), 16-byte aligned, used by this call only. */
 size_t star_causal_bwd_workspace(const star_causal_shape* s, int nk_tiles);

@@ -6,10 +6,10 @@ reference's operator signatures), `step.py` (the NuggetStep used by smoke/bench)
 inference side of the path) and `dist.py` (batch sharding + flat RCCL gradient all-reduces).
 """
 from . import ops  # noqa: F401
-from .nugget import (NuggetCrossAttention, NuggetOpsMixin, NuggetScorer, gather_nuggets,  # noqa: F401
+from .nugget import (NuggetCrossAttention, NuggetOpsMixin, NuggetScorer, NuggetSelfAttention, gather_nuggets,  # noqa: F401
                      gather_nuggets_layernorm, score_biased_attn, share_encoder_kv, share_scorer_logits,
                      defer_projection_weight_grads)
 
-__all__ = ["ops", "NuggetScorer", "NuggetOpsMixin", "NuggetCrossAttention", "gather_nuggets",
+__all__ = ["ops", "NuggetScorer", "NuggetOpsMixin", "NuggetCrossAttention", "NuggetSelfAttention", "gather_nuggets",
            "gather_nuggets_layernorm", "score_biased_attn", "share_encoder_kv", "share_scorer_logits",
            "defer_projection_weight_grads"]

@@ -32,7 +32,8 @@ class CausalShape(C.Structure):
     _fields_ = [("H", C.c_int), ("Hkv", C.c_int), ("hd", C.c_int), ("dtype", C.c_int), ("nseq", C.c_int),
                 ("max_q", C.c_int), ("q_sr", C.c_int64), ("q_sh", C.c_int64), ("k_sr", C.c_int64), ("k_sh", C.c_int64),
                 ("v_sr", C.c_int64), ("v_sh", C.c_int64), ("o_sr", C.c_int64), ("o_sh", C.c_int64),
-                ("lse_stride", C.c_int64), ("k_rows", C.c_int64), ("scale", C.c_float)]
+                ("lse_stride", C.c_int64), ("k_rows", C.c_int64),
+                ("dq_sr", C.c_int64), ("dkv_sr", C.c_int64), ("scale", C.c_float)]
 
 
 class KV8Cache(C.Structure):

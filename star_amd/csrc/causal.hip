@@ -545,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
     for (int qb = 0; qb < 2; ++qb) {
         const int i = w0 + 16 * qb + r16;
         if (i >= sq.nq) continue;
-        T* row = dQ + ((int64_t)(sq.q0 + i) * s.H + h) * HD + 4 * g;
+        T* row = dQ + (int64_t)(sq.q0 + i) * s.dq_sr + h * HD + 4 * g;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             x4 o4;
@@ -730,9 +730,9 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     for (int kb = 0; kb < 2; ++kb) {
         const int j = w0 + 16 * kb + r16;
         if (j >= sq.nk) continue;
-        const int64_t at = ((int64_t)(sq.k0 + j) * s.Hkv + hk) * HD + 4 * g;
+        const int64_t at = (int64_t)(sq.k0 + j) * s.dkv_sr + hk * HD + 4 * g;
         if (parts > 1) {
-            float* sk = sums + (int64_t)part * 2 * s.k_rows * s.Hkv * HD + at;
+            float* sk = sums + ((int64_t)part * 2 * s.k_rows + sq.k0 + j) * s.Hkv * HD + hk * HD + 4 * g;
             float* sv = sk + s.k_rows * s.Hkv * HD;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -767,13 +767,13 @@ __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __rest
     const int64_t one = s.k_rows * s.Hkv * HD;
     for (int c = threadIdx.x; c < 2 * rows * (HD / 4); c += 256) {
         const int which = c / (rows * (HD / 4)), cc = c % (rows * (HD / 4));
-        const int64_t at = ((int64_t)(sq.k0 + j0 + cc / (HD / 4)) * s.Hkv + hk) * HD + 4 * (cc % (HD / 4));
+        const int64_t row = sq.k0 + j0 + cc / (HD / 4), d = hk * HD + 4 * (cc % (HD / 4)), at = row * s.Hkv * HD + d;
         f32x4 sum = (f32x4){0.f, 0.f, 0.f, 0.f};
         for (int p = 0; p < parts; ++p) sum += *(const f32x4*)(sums + (2 * p + which) * one + at);
         x4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (T)(which ? sum[e] : sum[e] * s.scale);
-        *(x4*)((which ? dV : dK) + at) = o;
+        *(x4*)((which ? dV : dK) + row * s.dkv_sr + d) = o;
     }
 }
 
@@ -918,6 +918,8 @@ extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, cons
                  "star_causal_bwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(do_) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                  "star_causal_bwd: tensors must be 16-byte aligned");
+    STAR_REQUIRE(s->dq_sr % 8 == 0 && s->dkv_sr % 8 == 0 && s->dq_sr >= (int64_t)s->H * s->hd && s->dkv_sr >= (int64_t)s->Hkv * s->hd,
+                 "star_causal_bwd: gradient row strides %lld, %lld", (long long)s->dq_sr, (long long)s->dkv_sr);
     const int64_t need = causal_bwd_bytes(s, nk_tiles);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !aligned16(workspace))) {
         set_error("star_causal_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);

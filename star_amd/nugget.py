@@ -13,6 +13,7 @@ The reference has no plugin interface; its boundary is these Python signatures:
   semantic_repr[arange(B)[:,None], nugget_indices]         gather_nuggets              (w2v_asr.py:566-567)
   MyGPT2Attention._attn (my_transformer.py:535)            score_biased_attn / NuggetCrossAttention._attn
   MyGPT2Attention.forward, cross branch (:490-533)         NuggetCrossAttention.forward
+  MyGPT2Attention.forward, self branch (:511-533)          NuggetSelfAttention.forward (causal, lengths for masks)
 
 A maintainer of the reference makes `W2VASRModel` / `W2VSimulModel` inherit `NuggetOpsMixin` (first in
 the MRO), builds `self.nugget_model = NuggetScorer(hidden_size)` and uses `NuggetCrossAttention` for
@@ -157,6 +158,51 @@ class NuggetOpsMixin:
 
 
 # ------------------------------------------------------------------------------------------ a8
+def _additive_bias(attention_mask, scorer_logits, B, K):
+    """The additive [B,1,1,K] encoder mask and the scorer logits [B,Kb<=K] as one per-key bias, fp32 [B,<=K] or None."""
+    bias = None
+    if attention_mask is not None:
+        if attention_mask.shape[-1] != K or attention_mask.numel() != B * K:
+            raise ValueError(f"attention_mask must broadcast as [B,1,1,K]; got {tuple(attention_mask.shape)}")
+        bias = attention_mask.reshape(B, K).to(torch.float32)
+    if scorer_logits is not None:
+        s = scorer_logits.to(torch.float32)
+        if s.shape[1] > K:
+            raise ValueError(f"scorer_logits has {s.shape[1]} columns but there are only {K} keys")
+        if bias is None:
+            bias = s            # prefix-bias variant (my_transformer.py:114-125): the kernel takes bias_len <= K
+        else:
+            if s.shape[1] < K:
+                s = torch.nn.functional.pad(s, (0, K - s.shape[1]))   # the pad mask covers all K keys
+            bias = bias + s
+    return bias
+
+
+def _attn_scale(head_dim, scale_attn_weights, scale_attn_by_inverse_layer_idx, layer_idx):
+    scale = 1.0
+    if scale_attn_weights:
+        scale = scale / (head_dim ** 0.5)
+    if scale_attn_by_inverse_layer_idx:
+        scale = scale / float(layer_idx + 1)
+    return scale
+
+
+def score_biased_cached_attn(query, cache, attention_mask=None, scorer_logits=None, limit_cross_attn=False,
+                             scale_attn_weights=True, scale_attn_by_inverse_layer_idx=False, layer_idx=0, query_offset=0):
+    """score_biased_attn for generation over an 8-bit cache of the memory's keys and values (ops.KVCache8): the same
+    masks and biases on the tokens that the cache holds (its device-side lens; attention_mask and scorer_logits may end
+    before or behind them).  query [B,h,L,hd]; returns [B,h,L,hd] in query's dtype.  No dropout, weights or gradient."""
+    scale = _attn_scale(query.shape[-1], scale_attn_weights, scale_attn_by_inverse_layer_idx, layer_idx)
+    K = cache.capacity if attention_mask is None else attention_mask.shape[-1]
+    if scorer_logits is not None and scorer_logits.dim() == 3:
+        raise ValueError("score_biased_cached_attn: give the [B,K] scorer logits themselves, not a share_scorer_logits() view")
+    bias = _additive_bias(attention_mask, scorer_logits, query.shape[0], K)
+    # (like the core, the cached attention computes on 16-bit operands: an fp32 query is rounded on entry)
+    out = ops.kv8_attn(query.to(cache.dtype), cache, causal=False, ilk_diag=2 + int(query_offset) if limit_cross_attn else -1,
+                       bias=bias, scale=scale)
+    return out.to(query.dtype)
+
+
 def score_biased_attn(query, key, value, attention_mask=None, head_mask=None, scorer_logits=None,
                       limit_cross_attn=False, scale_attn_weights=True, scale_attn_by_inverse_layer_idx=False,
                       layer_idx=0, key_lengths=None, output_attentions=False, dropout_p=0.0, dropout_rng=None,
@@ -189,12 +235,7 @@ def score_biased_attn(query, key, value, attention_mask=None, head_mask=None, sc
         if probs is not None:
             probs = probs * head_mask.to(probs.dtype)
         return out, probs
-    scale = 1.0
-    if scale_attn_weights:
-        scale = scale / (value.size(-1) ** 0.5)
-    if scale_attn_by_inverse_layer_idx:
-        scale = scale / float(layer_idx + 1)
-    bias = None
+    scale = _attn_scale(value.size(-1), scale_attn_weights, scale_attn_by_inverse_layer_idx, layer_idx)
     B, K = query.shape[0], key.shape[2]
     if scorer_logits is not None and scorer_logits.dim() == 3:
         # a per-layer view from share_scorer_logits(): the encoder mask is already folded in
@@ -203,20 +244,7 @@ def score_biased_attn(query, key, value, attention_mask=None, head_mask=None, sc
         return ops.xattn(query, key, value, bias=scorer_logits, key_len=key_lengths,
                          ilk_diag=2 + int(query_offset) if limit_cross_attn else -1, scale=scale, need_probs=output_attentions,
                          dropout_p=dropout_p, dropout_rng=dropout_rng, kv_grad=kv_grad)
-    if attention_mask is not None:
-        if attention_mask.shape[-1] != K or attention_mask.numel() != B * K:
-            raise ValueError(f"attention_mask must broadcast as [B,1,1,K]; got {tuple(attention_mask.shape)}")
-        bias = attention_mask.reshape(B, K).to(torch.float32)
-    if scorer_logits is not None:
-        s = scorer_logits.to(torch.float32)
-        if s.shape[1] > K:
-            raise ValueError(f"scorer_logits has {s.shape[1]} columns but there are only {K} keys")
-        if bias is None:
-            bias = s            # prefix-bias variant (my_transformer.py:114-125): the kernel takes bias_len <= K
-        else:
-            if s.shape[1] < K:
-                s = torch.nn.functional.pad(s, (0, K - s.shape[1]))   # the pad mask covers all K keys
-            bias = bias + s
+    bias = _additive_bias(attention_mask, scorer_logits, B, K)
     out, probs = ops.xattn(query, key, value, bias=bias, key_len=key_lengths,
                            ilk_diag=2 + int(query_offset) if limit_cross_attn else -1, scale=scale, need_probs=output_attentions,
                            dropout_p=dropout_p, dropout_rng=dropout_rng, kv_grad=kv_grad)
@@ -245,11 +273,12 @@ def share_scorer_logits(scorer_logits, n_layers: int, n_heads: int, attention_ma
 
 
 class EncoderKV:
-    """One decoder layer's share of share_encoder_kv(): key / value [B,h,K,hd] and the slot its dK / dV go to."""
-    __slots__ = ("key", "value", "grad_slot")
+    """One decoder layer's share of share_encoder_kv(): key / value [B,h,K,hd] and the slot its dK / dV go to.  Or, in
+    `cache`, an 8-bit cache that holds them (streaming.StreamingEncoderKV with eight_bit=True)."""
+    __slots__ = ("key", "value", "grad_slot", "cache")
 
-    def __init__(self, key, value, grad_slot):
-        self.key, self.value, self.grad_slot = key, value, grad_slot
+    def __init__(self, key, value, grad_slot, cache=None):
+        self.key, self.value, self.grad_slot, self.cache = key, value, grad_slot, cache
 
 
 def share_encoder_kv(attn_modules, encoder_hidden_states):
@@ -435,6 +464,15 @@ class NuggetCrossAttention(nn.Module):
             raise ValueError("NuggetCrossAttention is the cross-attention module: encoder_hidden_states is required")
         query = self._split_heads(self.q_attn(hidden_states))
         kv_grad = None
+        if encoder_kv is not None and encoder_kv.cache is not None:
+            if head_mask is not None or output_attentions or use_cache or layer_past is not None:
+                raise ValueError("an 8-bit encoder_kv takes no head_mask, output_attentions, use_cache or layer_past")
+            if self.training and self.attn_pdrop > 0.0:
+                raise ValueError("an 8-bit encoder_kv is for generation: attention dropout does not run on it")
+            out = score_biased_cached_attn(query, encoder_kv.cache, encoder_attention_mask, scorer_logits,
+                                           bool(limit_cross_attn), self.scale_attn_weights,
+                                           self.scale_attn_by_inverse_layer_idx, self.layer_idx, query_offset)
+            return self.resid_dropout(self.c_proj(out.permute(0, 2, 1, 3).flatten(2))), None
         if encoder_kv is not None:
             key, value = encoder_kv.key, encoder_kv.value
             kv_grad = encoder_kv.grad_slot if layer_past is None else None
@@ -459,3 +497,83 @@ class NuggetCrossAttention(nn.Module):
         if output_attentions:
             outputs += (attn_weights,)
         return outputs
+
+
+class NuggetSelfAttention(nn.Module):
+    """Self-attention branch of MyGPT2Attention.forward (my_transformer.py:511-533), causal: the attention of the
+    semantic encoder over the frames and of the decoder over its own tokens.  Parameters c_attn and c_proj (Conv1D
+    layout) as in GPT2Attention; kv_heads < num_heads (not in the reference) shares every key head between
+    num_heads // kv_heads query heads, c_attn is then [hidden, (num_heads + 2 kv_heads) * head_dim].
+
+    The core runs on 16-bit operands with fp32 softmax and sums, as NuggetCrossAttention's does: fp32 activations are
+    rounded to bfloat16 for it.  The softmax is never padded, so no additive attention_mask is taken: give the lengths.
+
+        attn(x)                                  x [B,T,d], every row T frames
+        attn(x, valid=frames)                    x [B,T,d] padded, frames an ops.ValidFrames; pad rows see nothing
+        attn(x, plan=plan)                       x [rows,d] packed, plan an ops.PackedSeqs
+        attn(x, plan=plan, cache=cache)          the same prompt, whose keys and values also go into an ops.KVCache8
+        attn(x, cache=cache, counts=n)           x [B,L,d]: the next (at most L) tokens of every sequence of the cache"""
+
+    def __init__(self, hidden_size: int, num_heads: int, layer_idx: int = 0, scale_attn_weights: bool = True,
+                 scale_attn_by_inverse_layer_idx: bool = False, resid_pdrop: float = 0.0, attn_pdrop: float = 0.0,
+                 kv_heads: Optional[int] = None):
+        super().__init__()
+        if hidden_size % num_heads:
+            raise ValueError("`embed_dim` must be divisible by num_heads")
+        self.embed_dim, self.num_heads, self.head_dim = hidden_size, num_heads, hidden_size // num_heads
+        self.kv_heads = num_heads if kv_heads is None else int(kv_heads)
+        if self.kv_heads < 1 or num_heads % self.kv_heads:
+            raise ValueError(f"{num_heads} query heads do not divide into {kv_heads} key heads")
+        if attn_pdrop:
+            raise NotImplementedError("NuggetSelfAttention: attention-probability dropout is not built (attn_pdrop must be 0)")
+        self.layer_idx = layer_idx
+        self.scale = _attn_scale(self.head_dim, scale_attn_weights, scale_attn_by_inverse_layer_idx, layer_idx)
+        self.c_attn = Conv1D((num_heads + 2 * self.kv_heads) * self.head_dim, hidden_size)
+        self.c_proj = Conv1D(hidden_size, hidden_size)
+        self.resid_dropout = nn.Dropout(resid_pdrop)
+        self._plan = None            # ((B, T, device), plan) of the last unpadded batch
+
+    def new_cache(self, batch: int, max_tokens: int, device=None, dtype=torch.bfloat16):
+        """An empty 8-bit cache for this layer."""
+        return ops.KVCache8(batch, self.kv_heads, max_tokens, self.head_dim, device or self.c_attn.weight.device, dtype)
+
+    def forward(self, hidden_states, plan=None, valid=None, cache=None, counts=None):
+        if cache is not None and plan is None:
+            return self._next_tokens(hidden_states, cache, counts)
+        if counts is not None:
+            raise ValueError("NuggetSelfAttention: counts go with the next tokens of a cache")
+        if plan is None:
+            if hidden_states.dim() != 3:
+                raise ValueError(f"NuggetSelfAttention: [B,T,{self.embed_dim}] or a plan expected, got {tuple(hidden_states.shape)}")
+            B, T, _ = hidden_states.shape
+            if valid is not None:
+                if not valid.matches(hidden_states):
+                    raise ValueError(f"NuggetSelfAttention: valid is for [{valid.B},{valid.T},d], got {tuple(hidden_states.shape)}")
+                plan = valid.seqs()
+            else:
+                key = (B, T, hidden_states.device)
+                if self._plan is None or self._plan[0] != key:
+                    self._plan = (key, ops.PackedSeqs([T] * B, hidden_states.device))
+                plan = self._plan[1]
+        elif valid is not None:
+            raise ValueError("NuggetSelfAttention: give plan or valid, not both")
+        qkv = self.c_attn(hidden_states).reshape(-1, self.c_attn.nf)
+        core = qkv.to(torch.bfloat16) if qkv.dtype == torch.float32 else qkv
+        out = ops.causal_attn_qkv(core, self.num_heads, self.kv_heads, plan, scale=self.scale)
+        if cache is not None:
+            _, k, v = ops._qkv_views(core.detach(), self.num_heads, self.kv_heads, self.head_dim)
+            ops.kv8_append(cache, k, v, plan=plan)
+        out = out.flatten(1).to(qkv.dtype).view(hidden_states.shape)
+        return self.resid_dropout(self.c_proj(out))
+
+    def _next_tokens(self, hidden_states, cache, counts):
+        if torch.is_grad_enabled():
+            raise ValueError("NuggetSelfAttention: nothing is differentiated through a cache; call it under torch.no_grad()")
+        if hidden_states.dim() != 3:
+            raise ValueError(f"NuggetSelfAttention: [B,L,{self.embed_dim}] expected with a cache, got {tuple(hidden_states.shape)}")
+        qkv = self.c_attn(hidden_states)
+        core = qkv.to(cache.dtype).unflatten(2, (-1, self.head_dim)).transpose(1, 2)       # [B, heads, L, hd]
+        q, k, v = core.split([self.num_heads, self.kv_heads, self.kv_heads], dim=1)
+        ops.kv8_append(cache, k, v, counts=counts)
+        out = ops.kv8_attn(q, cache, q_len=counts, scale=self.scale)
+        return self.resid_dropout(self.c_proj(out.transpose(1, 2).flatten(2).to(qkv.dtype)))

@@ -666,6 +666,7 @@ class ValidFrames:
     def __init__(self, lengths: Sequence[int], T: int, device, compact: bool = True):
         ln = np.minimum(np.asarray(list(lengths), dtype=np.int64), T)
         self.B, self.T = int(ln.size), int(T)
+        self.host_lengths, self._seqs = ln.tolist(), None
         self.compact = bool(compact)
         starts = np.arange(self.B, dtype=np.int64) * T
         live = set()
@@ -688,6 +689,13 @@ class ValidFrames:
         table[rows.astype(np.int64)] = np.arange(self.n_valid, dtype=np.int32)
         self.row_of_frame = torch.from_numpy(table).to(device)
         self.arange = torch.arange(max(self.n_valid, 1), dtype=torch.int32, device=device)[:self.n_valid]
+
+    def seqs(self) -> "PackedSeqs":
+        """The utterances as sequences of the flattened [B*T] frame axis, for causal_attn (built at the first call, which
+        copies to the device: make it before a HIP-graph capture)."""
+        if self._seqs is None:
+            self._seqs = PackedSeqs(self.host_lengths, self.lengths.device, padded_to=self.T)
+        return self._seqs
 
     def matches(self, x) -> bool:
         return x.dim() == 3 and x.shape[0] == self.B and x.shape[1] == self.T
@@ -1617,10 +1625,11 @@ class PackedSeqs:
     lengths: keys of every sequence.  q_lengths: its queries where there are fewer (they are the newest positions: query
     i sees the keys j <= i + lengths[s] - q_lengths[s]); more queries than keys are allowed, the first then see nothing.
     Sequences lie one behind the other; with padded_to=T sequence s starts at row s * T instead (a padded [B,T] batch,
-    flattened), for the queries too."""
+    flattened), for the queries too; k_starts gives the first key row of every sequence (for kv8_append: rows of two
+    sequences may be the same there, but causal_attn's gradients need them apart)."""
 
     def __init__(self, lengths: Sequence[int], device, q_lengths: Optional[Sequence[int]] = None,
-                 padded_to: Optional[int] = None):
+                 padded_to: Optional[int] = None, k_starts: Optional[Sequence[int]] = None):
         nk = np.asarray(list(lengths), dtype=np.int64).reshape(-1)
         nq = nk if q_lengths is None else np.asarray(list(q_lengths), dtype=np.int64).reshape(-1)
         if nq.size != nk.size:
@@ -1636,12 +1645,17 @@ class PackedSeqs:
             return np.concatenate([np.zeros(1, np.int64), np.cumsum(n)[:-1]]) if n.size else n
 
         q0, k0 = place(nq), place(nk)
+        if k_starts is not None:
+            k0 = np.asarray(list(k_starts), dtype=np.int64).reshape(-1)
+            if k0.size != nk.size or (k0.size and k0.min() < 0):
+                raise ValueError(f"PackedSeqs: {k0.size} key starts, none negative, for {nk.size} sequences expected")
         # rows that tensors have to have, and rows that belong to a sequence
         self.q_rows = int((q0 + nq).max()) if nk.size else 0
         self.k_rows = int((k0 + nk).max()) if nk.size else 0
         self.q_used, self.k_used = int(nq.sum()), int(nk.sum())
         if max(self.q_rows, self.k_rows) >= 2 ** 31:
             raise ValueError("PackedSeqs: more than 2^31 - 1 rows")
+        self.square = bool((nq == nk).all())
         self.n, self.max_q, self.max_k = int(nk.size), int(nq.max(initial=0)), int(nk.max(initial=0))
 
         def tiles(n, work):
@@ -1679,6 +1693,22 @@ def _causal_forward(q, k, v, plan, s):
     return o, lse
 
 
+def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
+    """Gradients into dq, dk and dv, whose rows are s.dq_sr and s.dkv_sr values apart."""
+    if torch.is_grad_enabled():
+        raise _lib.StarNuggetError("causal_attn has no second derivative (backward with create_graph=True)")
+    g = g.to(q.dtype).contiguous()
+    if g.data_ptr() % 16:
+        g = g.clone()
+    delta = torch.empty_like(lse)
+    need = lib().star_causal_bwd_workspace(s, plan.n_k_tiles) if s.H != s.Hkv else 0
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+    _launch(lib().star_causal_bwd, "star_causal_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+            g.data_ptr(), lse.data_ptr(), plan.seqs.data_ptr(), plan.q_tiles.data_ptr(), plan.n_q_tiles,
+            plan.k_tiles.data_ptr(), plan.n_k_tiles, s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+            ptr(ws), need)
+
+
 class _CausalAttn(torch.autograd.Function):
     """softmax(scale Q K^T, j <= i + nk - nq) V of packed sequences."""
 
@@ -1694,23 +1724,39 @@ class _CausalAttn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, _=None):
-        if torch.is_grad_enabled():
-            raise _lib.StarNuggetError("causal_attn has no second derivative (backward with create_graph=True)")
         q, k, v, o, lse = ctx.saved_tensors
-        plan, s, dev = ctx.plan, ctx.s, q.device
-        g = g.to(q.dtype).contiguous()
-        if g.data_ptr() % 16:
-            g = g.clone()
+        plan, s = ctx.plan, ctx.s
         dq = _rows_like(s.lse_stride, plan.q_used, s.H, s.hd, q)
         dk, dv = (_rows_like(s.k_rows, plan.k_used, s.Hkv, s.hd, t) for t in (k, v))
-        delta = torch.empty_like(lse)
-        need = lib().star_causal_bwd_workspace(s, plan.n_k_tiles) if s.H != s.Hkv else 0
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        _launch(lib().star_causal_bwd, "star_causal_bwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                g.data_ptr(), lse.data_ptr(), plan.seqs.data_ptr(), plan.q_tiles.data_ptr(), plan.n_q_tiles,
-                plan.k_tiles.data_ptr(), plan.n_k_tiles, s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
-                ptr(ws), need)
+        s.dq_sr, s.dkv_sr = s.H * s.hd, s.Hkv * s.hd
+        _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv)
         return dq, dk, dv, None, None, None
+
+
+class _CausalAttnQKV(torch.autograd.Function):
+    """The same on one projection [rows, (H + 2 Hkv) hd], whose gradient is written in place of three that autograd
+    would have to put side by side."""
+
+    @staticmethod
+    def forward(ctx, qkv, views, plan, s):
+        o, lse = _causal_forward(*views, plan, s)
+        ctx.save_for_backward(qkv, o, lse)
+        ctx.plan, ctx.s = plan, s
+        return o
+
+    @staticmethod
+    def backward(ctx, g):
+        qkv, o, lse = ctx.saved_tensors
+        plan, s = ctx.plan, ctx.s
+        d = _rows_like(s.lse_stride, plan.q_used, s.H + 2 * s.Hkv, s.hd, qkv)
+        s.dq_sr = s.dkv_sr = (s.H + 2 * s.Hkv) * s.hd
+        _causal_backward(g, *_qkv_views(qkv, s.H, s.Hkv, s.hd), o, lse, plan, s, *_qkv_views(d.flatten(1), s.H, s.Hkv, s.hd))
+        return d.flatten(1), None, None, None
+
+
+def _qkv_views(qkv, H, Hkv, hd):
+    t = qkv.unflatten(1, (H + 2 * Hkv, hd))
+    return t[:, :H], t[:, H:H + Hkv], t[:, H + Hkv:]
 
 
 def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_lse: bool = False):
@@ -1723,6 +1769,29 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     gradients.  Sums and softmax statistics are fp32; the softmax weights are rounded to the inputs' type for the
     product with v, and their gradient for the products with q and k.  An infinite or NaN v row reaches up to 63 earlier
     queries of its own sequence (they share a tile); k and v rows of other sequences or in no sequence reach nobody."""
+    s = _causal_shape(q, k, v, plan, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CausalAttn.apply(q, k, v, plan, s, need_lse)
+    o, lse = _causal_forward(q, k, v, plan, s)
+    return (o, lse) if need_lse else o
+
+
+def causal_attn_qkv(qkv, n_heads: int, kv_heads: int, plan: PackedSeqs, scale: Optional[float] = None):
+    """causal_attn on one projection qkv [rows, (n_heads + 2 kv_heads) hd], queries, keys and values side by side (GPT-2's
+    c_attn, my_transformer.py:512): returns o [rows, n_heads, hd].  The gradients of the three parts are written straight
+    into one matrix of qkv's shape."""
+    if qkv.dim() != 2 or n_heads < 1 or kv_heads < 1 or qkv.shape[1] % (n_heads + 2 * kv_heads):
+        raise ValueError(f"causal_attn_qkv: [rows, ({n_heads} + 2 * {kv_heads}) * hd] expected, got {tuple(qkv.shape)}")
+    if not plan.square:
+        raise ValueError("causal_attn_qkv: every sequence has as many queries as keys in one projection")
+    views = _qkv_views(qkv.detach(), n_heads, kv_heads, qkv.shape[1] // (n_heads + 2 * kv_heads))
+    s = _causal_shape(*views, plan, scale)
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return _CausalAttnQKV.apply(qkv, views, plan, s)
+    return _causal_forward(*views, plan, s)[0]
+
+
+def _causal_shape(q, k, v, plan, scale):
     dev = _same_device("causal_attn", q=q, k=k, v=v)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"causal_attn: [rows, heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -1748,10 +1817,7 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     s.o_sr, s.o_sh = H * hd, hd
     s.H, s.Hkv, s.hd, s.dtype, s.nseq, s.max_q = H, Hkv, hd, _DT16[q.dtype], plan.n, plan.max_q
     s.lse_stride, s.k_rows, s.scale = rows, k_rows, scale
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CausalAttn.apply(q, k, v, plan, s, need_lse)
-    o, lse = _causal_forward(q, k, v, plan, s)
-    return (o, lse) if need_lse else o
+    return s
 
 
 # ----------------------------------------------------------------------------- 8-bit key/value cache

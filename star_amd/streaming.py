@@ -150,9 +150,13 @@ class StreamingEncoderKV:
     encoder_hidden_states)`, my_transformer.py:500-501 under 724-733 / 1079-1099).  c_attn is row-wise, so a row that
     entered the memory is projected ONCE, for all layers at once ([rows, d] x [d, nl*2d]), into a preallocated
     [B, Kmax, nl*2d] buffer; extend(counts) projects the rows appended since the last call.  layers()
-    returns one EncoderKV per layer for NuggetCrossAttention(encoder_kv=...): strided head views, no copies."""
+    returns one EncoderKV per layer for NuggetCrossAttention(encoder_kv=...): strided head views, no copies.
 
-    def __init__(self, attn_modules: Sequence, segmenter: StreamingNuggetSegmenter):
+    eight_bit=True keeps the projections in one ops.KVCache8 per layer instead (about half the memory, and half the bytes
+    that every decoded token reads): e4m3 blocks of 64 nuggets, the newest ones as they came.  The attention then needs no
+    encoder_attention_mask (the caches know their lengths) and runs without gradients."""
+
+    def __init__(self, attn_modules: Sequence, segmenter: StreamingNuggetSegmenter, eight_bit: bool = False):
         from .nugget import EncoderKV
         self._EncoderKV = EncoderKV
         mods = list(attn_modules)
@@ -166,7 +170,13 @@ class StreamingEncoderKV:
             self.w_all = torch.cat([m.c_attn.weight for m in mods], dim=1).to(segmenter.device, dt).contiguous()
             self.b_all = torch.cat([m.c_attn.bias for m in mods], dim=0).to(segmenter.device, dt).contiguous()
         B, kmax, d = segmenter.B, segmenter.kmax, segmenter.d
-        self.kv = torch.zeros(B, kmax, self.nl * 2 * d, dtype=dt, device=segmenter.device)
+        self.caches = None
+        if eight_bit:
+            cdt = dt if dt in (torch.bfloat16, torch.float16) else torch.bfloat16
+            self.kv = None
+            self.caches = [ops.KVCache8(B, self.h, kmax, d // self.h, segmenter.device, cdt) for _ in mods]
+        else:
+            self.kv = torch.zeros(B, kmax, self.nl * 2 * d, dtype=dt, device=segmenter.device)
         self._prev = [0] * B                            # per utterance: rows [0, prev) are projected
 
     @torch.no_grad()
@@ -184,14 +194,32 @@ class StreamingEncoderKV:
             B, d = self.seg.B, self.seg.d
             rows = self.seg.state.mem[:, lo:hi].reshape(-1, d)
             out = torch.addmm(self.b_all, rows, self.w_all)
-            self.kv[:, lo:hi] = out.view(B, hi - lo, -1)
+            if self.caches is None:
+                self.kv[:, lo:hi] = out.view(B, hi - lo, -1)
+            else:
+                self._append(out, lo, hi, cur)
         self._prev = cur
 
+    def _append(self, out, lo, hi, cur):
+        """Rows [prev_b, cur_b) of every utterance, of the projected [lo, hi), into the layers' caches."""
+        if any(c < p for c, p in zip(cur, self._prev)):
+            raise ValueError("extend: a count went back; reset() the utterance first")
+        plan = ops.PackedSeqs([c - p for c, p in zip(cur, self._prev)], self.seg.device,
+                              k_starts=[b * (hi - lo) + p - lo for b, p in enumerate(self._prev)])
+        heads = out.to(self.caches[0].dtype).view(out.shape[0], 2 * self.nl, self.h, -1)
+        for l, cache in enumerate(self.caches):
+            ops.kv8_append(cache, heads[:, 2 * l], heads[:, 2 * l + 1], plan=plan)
+
     def reset(self, rows: Optional[Sequence[int]] = None):
-        for b in (range(self.seg.B) if rows is None else rows):
+        rows = list(range(self.seg.B) if rows is None else rows)
+        for b in rows:
             self._prev[b] = 0
+        for cache in self.caches or ():
+            cache.reset(torch.tensor(rows, dtype=torch.long, device=self.seg.device))
 
     def layers(self):
+        if self.caches is not None:
+            return [self._EncoderKV(None, None, None, cache) for cache in self.caches]
         B, kmax, d, h = self.seg.B, self.seg.kmax, self.seg.d, self.h
         out = []
         for l in range(self.nl):

@@ -144,6 +144,27 @@ def test_causal_attn_takes_views_of_one_projection_and_a_scale(ops):
 
 
 @gpu
+def test_causal_attn_qkv_equals_causal_attn_with_its_gradients_side_by_side(ops):
+    keys, H, Hkv, hd = [150, 40, 700], 4, 2, 64
+    plan = ops.PackedSeqs(keys, DEV)
+    qkv = rnd(7, sum(keys), (H + 2 * Hkv) * hd).requires_grad_()
+    do = rnd(8, sum(keys), H, hd)
+    o1 = ops.causal_attn_qkv(qkv, H, Hkv, plan, scale=0.2)
+    g1, = torch.autograd.grad(o1, qkv, do)
+    q, k, v = (t.view(-1, n, hd) for t, n in zip(qkv.split([H * hd, Hkv * hd, Hkv * hd], 1), (H, Hkv, Hkv)))
+    o2 = ops.causal_attn(q, k, v, plan, scale=0.2)
+    g2, = torch.autograd.grad(o2, qkv, do)
+    assert torch.equal(o1, o2) and torch.equal(g1, g2)
+    with torch.no_grad():
+        assert torch.equal(ops.causal_attn_qkv(qkv, H, Hkv, plan, scale=0.2), o1)
+    for bad in (qkv[:, :-1], qkv[None]):
+        with pytest.raises(ValueError, match="rows, "):
+            ops.causal_attn_qkv(bad, H, Hkv, plan)
+    with pytest.raises(ValueError, match="as many queries"):
+        ops.causal_attn_qkv(qkv, H, Hkv, ops.PackedSeqs([3, 5], DEV, q_lengths=[5, 3]))
+
+
+@gpu
 def test_causal_attn_strides_and_expanded_gradient(ops):
     """Rows and heads in another order, shared rows (stride 0) and a gradient without memory of its own."""
     keys, H, hd = [70, 129], 2, 64
@@ -633,8 +654,11 @@ def test_the_library_checks_sizes_before_any_launch():
     s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, scale=1)
     assert L.star_causal_fwd(16, 24, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"aligned" in L.star_last_error()
     assert L.star_causal_fwd(None, None, None, None, None, 0, s, None, None, None) == 0
-    s = _lib.CausalShape(H=4, Hkv=1, hd=64, dtype=0, nseq=1, k_rows=2000, scale=1)
+    s = _lib.CausalShape(H=4, Hkv=1, hd=64, dtype=0, nseq=1, k_rows=2000, scale=1, dq_sr=256, dkv_sr=64)
     assert L.star_causal_bwd_workspace(s, 16) > 0 and L.star_causal_bwd_workspace(s, 3) == 0
+    s.dq_sr = 128
+    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, s, 16, 16, 16, 16, None, 0, None) == -1 and b"gradient row" in L.star_last_error()
+    s.dq_sr = 256
     assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, s, 16, 16, 16, 16, None, 0, None) == -3 and b"workspace" in L.star_last_error()
     c = _lib.KV8Cache(B=1, Hkv=2, T=100, hd=64, dtype=0)
     assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 0, 0, None, None, 1, None, 1, None) == -1 and b"capacity 100" in L.star_last_error()
