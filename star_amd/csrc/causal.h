@@ -9,6 +9,8 @@ constexpr float A_LN2 = 0.6931471805599453f;
 constexpr float M_NONE = -1.0e30f;       // running maximum before the first visible key (finite: no inf - inf)
 constexpr float M_SLACK = 8.0f;          // log2 units: the running maximum follows only when a tile exceeds it by 2^8
 
+constexpr float M_MOST = 4096.0f;        // largest sum of a lane's weights of a tile against an earlier tile's maximum
+
 template <typename T> struct Vec;
 template <> struct Vec<__bf16> { typedef bf16x8 x8; typedef bf16x4 x4; };
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;

@@ -119,39 +119,54 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
                     for (int i = 0; i < 4; ++i)
                         sc[qb][kt4][i] = key0 + 16 * kt4 + 4 * g + i < lim[qb] ? sc[qb][kt4][i] : -INFINITY;
         }
+        // The weights are formed against the maximum of an earlier tile and only their sum is looked at: while it stays
+        // under M_MOST no weight can have overflowed 16 bits, and the tile needs no maximum of its own.  The first visible
+        // tile (M_NONE makes the sum infinite) and a rise of the logits by 12 in log2 take the other way once.
         x8 pf[2][2];
+        float sum[2];
+        auto weights = [&](int qb) {
+            sum[qb] = 0.f;
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-            float mx = sc[qb][0][0];                               // of the raw products: the scale is positive
+            for (int hf = 0; hf < 2; ++hf) {
+                f32x4 p[2];
 #pragma unroll
-            for (int kt4 = 0; kt4 < 4; ++kt4)
+                for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[qb][kt4][i]);
-            mx *= c2;
-            if (!__all(mx <= m[qb] + M_SLACK)) {
+                    for (int i = 0; i < 4; ++i) {
+                        p[k2][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][2 * hf + k2][i], c2, -m[qb]));
+                        sum[qb] += p[k2][i];
+                    }
+                pf[qb][hf] = pack_b<T>(p[0], p[1]);
+            }
+        };
+        weights(0);
+        weights(1);
+        if (!__all(sum[0] < M_MOST && sum[1] < M_MOST)) {
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                float mx = sc[qb][0][0];                           // of the raw products: the scale is positive
+#pragma unroll
+                for (int kt4 = 0; kt4 < 4; ++kt4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[qb][kt4][i]);
+                mx *= c2;
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(m[qb], mx), a = __builtin_amdgcn_exp2f(m[qb] - mn);
+                int over = !(sum[qb] < M_MOST);                    // of this row: no other row of the wave changes its bits
+                over |= __shfl_xor(over, 16, 64);
+                over |= __shfl_xor(over, 32, 64);
+                const float mn = over ? fmaxf(m[qb], mx) : m[qb], a = __builtin_amdgcn_exp2f(m[qb] - mn);
                 m[qb] = mn;
                 l[qb] *= a;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) oacc[qb][nt][i] *= a;
+                weights(qb);
             }
-            float sum = 0.f;
-#pragma unroll
-            for (int kt4 = 0; kt4 < 4; ++kt4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qb][kt4][i], c2, -m[qb]));
-                    sum += p;
-                    sc[qb][kt4][i] = p;
-                }
-            l[qb] += sum;
-            pf[qb][0] = pack_b<T>(sc[qb][0], sc[qb][1]);
-            pf[qb][1] = pack_b<T>(sc[qb][2], sc[qb][3]);
         }
+        l[0] += sum[0];
+        l[1] += sum[1];
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll

@@ -7,7 +7,9 @@ Tolerances follow from where 16-bit roundings enter, u = finfo(dtype).eps / 2 re
   dQ   dS rounded; delta = rowsum(dO o) is formed from the stored o, off by |dO| (err of o); dQ rounded:
        scale (u |dS| + P |dO|.(err of o)) |K| + u |dQ|;   dK the same with dS^T, |Q|
 plus 2^-12 of the magnitudes for fp32 arithmetic: a logit of hd <= 128 fp32 products is off by at most 128 * 2^-24 *
-sum|q k| scale, below 2^-12 for the values here (sum|q k| scale < 32)."""
+sum|q k| scale, below 2^-12 for the values here (sum|q k| scale < 32).  A weight P under 2^-126, the smallest normal
+fp32, may be taken for 0: 2^-126 of absolute error per weight, times what it is multiplied with (|v| for o, |dO| for dV,
+|dP| + |delta| for dS)."""
 import math
 
 import numpy as np
@@ -17,6 +19,7 @@ import torch
 DEV = "cuda:0"
 BF, FP = torch.bfloat16, torch.float16
 F32 = 2.0 ** -12
+FLUSH = 2.0 ** -126
 gpu = pytest.mark.gpu
 
 
@@ -56,7 +59,7 @@ def formula(q, k, v, scale, do=None, off=0):
     p = torch.nan_to_num(torch.softmax(s, 1)) * seen if len(k) else s
     lse = torch.logsumexp(s, 1) if len(k) else torch.full((len(q),), -math.inf, dtype=torch.float64, device=DEV)
     o = p @ v
-    ob = (u + F32) * (p @ v.abs()) + u * o.abs() + t * (1 + seen.double() @ v.abs())
+    ob = (u + F32) * (p @ v.abs()) + u * o.abs() + t + (t + FLUSH) * (seen.double() @ v.abs())
     if do is None:
         return dict(o=(o, ob), lse=lse)
     do = do.double()
@@ -64,9 +67,10 @@ def formula(q, k, v, scale, do=None, off=0):
     de = (do * o).sum(1, keepdim=True)
     ds = p * (dp - de)
     db = u * ds.abs() + p * (do.abs() * ob).sum(1, keepdim=True) + F32 * p * (do.abs() @ v.abs().T + (do * o).abs().sum(1, keepdim=True)) + t * seen
+    db = db + FLUSH * seen * (dp.abs() + de.abs())
     dq, dk, dv = ds @ k * scale, ds.T @ q * scale, p.T @ do
     return dict(o=(o, ob), lse=lse, dq=(dq, scale * db @ k.abs() + u * dq.abs() + t), dk=(dk, scale * db.T @ q.abs() + u * dk.abs() + t),
-                dv=(dv, (u + F32) * (p.T @ do.abs()) + u * dv.abs() + t * (1 + seen.double().T @ do.abs())))
+                dv=(dv, (u + F32) * (p.T @ do.abs()) + u * dv.abs() + t + (t + FLUSH) * (seen.double().T @ do.abs())))
 
 
 # ------------------------------------------------------------------------------------------------------ causal_attn
@@ -237,6 +241,29 @@ def test_causal_attn_large_and_small_logits(ops, big):
     check(o, want["o"][0], want["o"][1] + 5e-4 * v.detach().double().abs().max())
     for g in torch.autograd.grad(o, (q, k, v), do):
         assert torch.isfinite(g).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("rise", [5.0, 11.0, 13.0, 40.0, -40.0])
+def test_causal_attn_logits_that_climb_from_tile_to_tile(ops, dtype, rise):
+    """Logits that rise (fall) by `rise` in log2 with every 64 keys: the weights of a tile are formed against the maximum of
+    an earlier one until their sum would pass 2^12, and rescaled then."""
+    n, hd = 400, 64
+    q = torch.zeros(n, 1, hd, device=DEV, dtype=dtype)
+    k = torch.zeros(n, 1, hd, device=DEV, dtype=dtype)
+    q[..., 0] = 1
+    tile = torch.arange(n, device=DEV) // 64
+    k[:, 0, 0] = (tile * rise * math.log(2) + torch.rand(n, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)).to(dtype)
+    v, do = rnd(2, n, 1, hd, dtype=dtype), rnd(3, n, 1, hd, dtype=dtype)
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    o, lse = ops.causal_attn(q, k, v, ops.PackedSeqs([n], DEV), scale=1.0, need_lse=True)
+    want, want_lse = by_formula(q.detach(), k.detach(), v.detach(), [n], [n], 1.0, do)
+    check(o, *want["o"])
+    assert (lse.double() - want_lse).abs().max().item() < F32
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, (q, k, v), do)):
+        # (logits up to 167: an fp32 logit or log-sum-exp is off by 2^-17 of 1, beyond F32's share by little)
+        check(g, want[name][0], want[name][1] * 1.01, name)
 
 
 @gpu
