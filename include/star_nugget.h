@@ -459,7 +459,7 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
  *        strides in elements, multiples of 8; base addresses multiples of 16 bytes.  hd in {64, 96, 128}
  *   seqs [nseq][4] int32: first query row, queries nq, first key row, keys nk.  Query i of a sequence sees its keys
  *        j <= i + nk - nq (the queries are the newest nq positions); a query that sees no key gets o = 0, lse = -inf
- *   tiles [ntiles][2] int32: sequence and first query of every tile of STAR_CAUSAL_TILE queries, each exactly once, in
+ *   tiles [n_q_tiles][2] int32: sequence and first query of every tile of STAR_CAUSAL_TILE queries, each exactly once, in
  *        the order in which they are to start (longest first balances the load).  Rows in no sequence are not touched
  *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward
  * Softmax statistics and sums are fp32; the weights P are rounded to dtype for the product with V (as the inputs are).
@@ -469,25 +469,27 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
 #define STAR_DT_F16 2
 #define STAR_CAUSAL_TILE 128
 typedef struct {
-    int H, Hkv, hd, dtype, nseq;
-    int max_q;                  /* queries of the longest sequence */
+    int H, Hkv, hd, dtype;
+    int max_q, max_k;           /* queries and keys of the longest sequence */
+    int n_q_tiles, n_k_tiles;
     int64_t q_sr, q_sh, k_sr, k_sh, v_sr, v_sh, o_sr, o_sh;
     int64_t lse_stride;
     int64_t k_rows;             /* rows of k, v, dk and dv */
     int64_t dq_sr, dkv_sr;      /* row strides of dq, and of dk and dv (their heads are dense) */
     float scale;
 } star_causal_shape;
-int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles, int ntiles,
-                    const star_causal_shape* s, void* o, float* lse, void* stream);
+/* workspace (here and below): star_causal_*_workspace(s) bytes, 0 for most calls, 16-byte aligned, used by this call only */
+size_t star_causal_fwd_workspace(const star_causal_shape* s);
+int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+                    const star_causal_shape* s, void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 /* Backward: P recomputed from lse.  do_ has o's strides; dq [rows,H,hd] and dk / dv [rows,Hkv,hd] may be column
- * ranges of one matrix (dq_sr, dkv_sr, multiples of 8).  q_tiles as tiles above; k_tiles [nk_tiles][2]: the same for tiles of STAR_CAUSAL_TILE keys.  delta [H][lse_stride] fp32 scratch.
- * No atomics: the gradient of a shared key head is summed over its query heads in a fixed order.
- * workspace: star_causal_bwd_workspace(s, nk_tiles) bytes (0 for most calls), 16-byte aligned, used by this call only. */
-size_t star_causal_bwd_workspace(const star_causal_shape* s, int nk_tiles);
+ * ranges of one matrix (dq_sr, dkv_sr, multiples of 8).  q_tiles as tiles above; k_tiles [n_k_tiles][2]: the same for
+ * tiles of STAR_CAUSAL_TILE keys.  delta [H][lse_stride] fp32 scratch.
+ * No atomics: the gradient of a shared key head is summed over its query heads in a fixed order. */
+size_t star_causal_bwd_workspace(const star_causal_shape* s);
 int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                    const int32_t* seqs, const int32_t* q_tiles, int nq_tiles, const int32_t* k_tiles, int nk_tiles,
-                    const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta, void* workspace,
-                    size_t workspace_bytes, void* stream);
+                    const int32_t* seqs, const int32_t* q_tiles, const int32_t* k_tiles, const star_causal_shape* s,
+                    void* dq, void* dk, void* dv, float* delta, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- 8-bit key/value cache and attention over it
  * A cache of B sequences x Hkv key heads x T tokens (T a multiple of STAR_KV8_BLOCK = 64), for generation and for the
@@ -500,7 +502,7 @@ int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, 
  *   k_codes [B][Hkv][T][hd], k_scales [B][Hkv][T/64]         k_tail [B][Hkv][64][hd]  (row = token % 64)
  *   v_codes [B][Hkv][T/64][hd][64], v_scales [B][Hkv][T/64]  v_tail [B][Hkv][hd][64]  (V is transposed inside a block)
  *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written);
- *   tickets [B * STAR_KV8_TICKET_STRIDE]: zero before the first call, zero after every call.  All base addresses multiples of 16 bytes.
+ *   tickets [B * (1 + 2 * Hkv) * STAR_KV8_TICKET_STRIDE]: zero before the first call, zero after every call.  All base addresses multiples of 16 bytes.
  * Calls on one cache are ordered by the stream: two appends, or an append and an attention, must not overlap. */
 #define STAR_KV8_BLOCK 64
 #define STAR_KV8_TICKET_STRIDE 32

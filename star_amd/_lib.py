@@ -29,11 +29,11 @@ class XAttnShape(C.Structure):
 
 
 class CausalShape(C.Structure):
-    _fields_ = [("H", C.c_int), ("Hkv", C.c_int), ("hd", C.c_int), ("dtype", C.c_int), ("nseq", C.c_int),
-                ("max_q", C.c_int), ("q_sr", C.c_int64), ("q_sh", C.c_int64), ("k_sr", C.c_int64), ("k_sh", C.c_int64),
-                ("v_sr", C.c_int64), ("v_sh", C.c_int64), ("o_sr", C.c_int64), ("o_sh", C.c_int64),
-                ("lse_stride", C.c_int64), ("k_rows", C.c_int64),
-                ("dq_sr", C.c_int64), ("dkv_sr", C.c_int64), ("scale", C.c_float)]
+    _fields_ = [("H", C.c_int), ("Hkv", C.c_int), ("hd", C.c_int), ("dtype", C.c_int), ("max_q", C.c_int), ("max_k", C.c_int),
+                ("n_q_tiles", C.c_int), ("n_k_tiles", C.c_int), ("q_sr", C.c_int64), ("q_sh", C.c_int64),
+                ("k_sr", C.c_int64), ("k_sh", C.c_int64), ("v_sr", C.c_int64), ("v_sh", C.c_int64), ("o_sr", C.c_int64),
+                ("o_sh", C.c_int64), ("lse_stride", C.c_int64), ("k_rows", C.c_int64), ("dq_sr", C.c_int64),
+                ("dkv_sr", C.c_int64), ("scale", C.c_float)]
 
 
 class KV8Cache(C.Structure):
@@ -104,9 +104,10 @@ SIGNATURES = {
     "star_colsum_workspace": (_SZ, [_I64, _I]),
     "star_colsum": (_I, [_P, _I, _I64, _I, _I64, _P, _P, _SZ, _P]),
     "star_colsum_batched": (_I, [C.POINTER(C.c_void_p), _I, _I, _I64, _I, _I64, _P, _P, _SZ, _P]),
-    "star_causal_fwd": (_I, [_P, _P, _P, _P, _P, _I, C.POINTER(CausalShape), _P, _P, _P]),
-    "star_causal_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, C.POINTER(CausalShape), _P, _P, _P, _P, _P, _SZ, _P]),
-    "star_causal_bwd_workspace": (_SZ, [C.POINTER(CausalShape), _I]),
+    "star_causal_fwd_workspace": (_SZ, [C.POINTER(CausalShape)]),
+    "star_causal_fwd": (_I, [_P, _P, _P, _P, _P, C.POINTER(CausalShape), _P, _P, _P, _SZ, _P]),
+    "star_causal_bwd_workspace": (_SZ, [C.POINTER(CausalShape)]),
+    "star_causal_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, C.POINTER(CausalShape), _P, _P, _P, _P, _P, _SZ, _P]),
     "star_kv8_append": (_I, [C.POINTER(KV8Cache), _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I, _P, _I, _P]),
     "star_kv8_attn_workspace": (_SZ, [C.POINTER(KV8Cache), _I, _I]),
     "star_kv8_attn": (_I, [C.POINTER(KV8Cache), _P, _P, _P, C.POINTER(KV8Query), _P, _P, _SZ, _P]),

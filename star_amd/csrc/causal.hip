@@ -23,12 +23,27 @@ __device__ __forceinline__ SeqOf seq_of(const int32_t* seqs, int s) {
     return SeqOf{seqs[4 * s], seqs[4 * s + 1], seqs[4 * s + 2], seqs[4 * s + 3]};
 }
 
+// Few query tiles over long keys are cut along the keys: part p of `parts` walks its share of a tile's key tiles and
+// leaves its softmax state, sums[tile][head][part][row][HD], then maximum and sum [tile][head][part][row][2].
+struct KeyTiles { int first, end; };
+__device__ __forceinline__ KeyTiles key_tiles(int keys, int part, int parts) {
+    const int n = (keys + CK - 1) / CK, per = (n + parts - 1) / parts, first = min(n, part * per);
+    return KeyTiles{first, min(n, first + per)};
+}
+struct Partial { float *o, *ml; };
+template <int HD>
+__device__ __forceinline__ Partial partial(float* sums, const star_causal_shape& s, int parts, int rows, int t, int part, int h, int row) {
+    const int64_t at = (((int64_t)t * s.H + h) * parts + part) * rows + row, all = (int64_t)s.n_q_tiles * s.H * parts * rows;
+    return Partial{sums + at * HD, sums + all * HD + at * 2};
+}
+
 // ------------------------------------------------------------------------------------------------------ forward
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                            const T* __restrict__ V, const int32_t* __restrict__ seqs,
                                                            const int32_t* __restrict__ tiles, star_causal_shape s,
-                                                           T* __restrict__ O, float* __restrict__ lse) {
+                                                           int parts, float* __restrict__ sums, T* __restrict__ O,
+                                                           float* __restrict__ lse) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
     using Ti = Tile<T, HD>;
@@ -40,7 +55,7 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
     const int r16 = lane & 15, g = lane >> 4;
     // consecutive workgroups go to consecutive XCDs: key heads first, so that the tiles and query heads that share a
     // key head meet in one L2 when Hkv is a multiple of 8
-    const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int hi = blockIdx.x % s.H, part = blockIdx.x / s.H % parts, t = blockIdx.x / s.H / parts;
     const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
     const SeqOf sq = seq_of(seqs, tiles[2 * t]);
     const int i0 = tiles[2 * t + 1];                               // first query of the workgroup
@@ -76,15 +91,16 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
     }
 
     TileLoad<T, HD, CK, 256> kl, vl;
-    const int ntile = (end + CK - 1) / CK;
+    const KeyTiles kt_ = key_tiles(end, part, parts);
+    const int ntile = kt_.end;
     kl.place(s.k_sr, tid);
     vl.place(s.v_sr, tid);
-    if (ntile > 0) {
-        kl.load(Kh, s.k_sr, 0, sq.nk, tid);
-        vl.load(Vh, s.v_sr, 0, sq.nk, tid);
+    if (kt_.first < ntile) {
+        kl.load(Kh, s.k_sr, kt_.first * CK, sq.nk, tid);
+        vl.load(Vh, s.v_sr, kt_.first * CK, sq.nk, tid);
     }
 #pragma unroll 1
-    for (int tile = 0; tile < ntile; ++tile) {
+    for (int tile = kt_.first; tile < ntile; ++tile) {
         uint8_t* kt = smem + (tile & 1) * 2 * TB;
         uint8_t* vt = kt + TB;
         kl.store(kt, tid);                                         // (the tile two before is done: barrier of the last step)
@@ -184,6 +200,13 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
         sum += __shfl_xor(sum, 32, 64);
         const int i = w0 + 16 * qb + r16;
         if (i >= sq.nq) continue;
+        if (parts > 1) {
+            const Partial p = partial<HD>(sums, s, parts, CT, t, part, h, i - i0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) *(f32x4*)(p.o + 16 * nt + 4 * g) = oacc[qb][nt];
+            if (g == 0) { p.ml[0] = m[qb]; p.ml[1] = sum; }
+            continue;
+        }
         const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   // no visible key: 0; NaN stays NaN
         T* orow = O + (int64_t)(sq.q0 + i) * s.o_sr + (int64_t)h * s.o_sh + 4 * g;
 #pragma unroll
@@ -207,7 +230,8 @@ template <typename T, int HD, int QB>
 __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                            const T* __restrict__ V, const int32_t* __restrict__ seqs,
                                                            const int32_t* __restrict__ tiles, star_causal_shape s,
-                                                           T* __restrict__ O, float* __restrict__ lse) {
+                                                           int parts, float* __restrict__ sums, T* __restrict__ O,
+                                                           float* __restrict__ lse) {
     typedef typename Vec<T>::x8 x8;
     using Ti = Tile<T, HD>;
     constexpr int KS = HD / 32, NT = HD / 16, OP = HD + 4;
@@ -216,10 +240,12 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
 
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
-    const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int hi = blockIdx.x % s.H, part = blockIdx.x / s.H % parts, t = blockIdx.x / s.H / parts;
     const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
     const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int off = sq.nk - sq.nq, end = max(0, sq.nk);            // (the last query sees every key)
+    const int off = sq.nk - sq.nq;                                 // (the last query sees every key)
+    const KeyTiles kt_ = key_tiles(sq.nk, part, parts);
+    const int end = min(sq.nk, kt_.end * CK);
     const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
     const T* Vh = V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh;
     int lim[QB];
@@ -245,7 +271,7 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
     }
     uint8_t* vt = smem + wid * CK * Ti::ROWB;
 #pragma unroll 1
-    for (int key0 = wid * CK; key0 < end; key0 += 4 * CK) {
+    for (int key0 = (kt_.first + wid) * CK; key0 < end; key0 += 4 * CK) {
         TileLoad<T, HD, CK, 64> vl;
         vl.place(s.v_sr, lane);
         vl.load(Vh, s.v_sr, key0, sq.nk, lane);
@@ -349,12 +375,47 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
 #pragma unroll
             for (int e = 0; e < PER; ++e) o[e] += f * osh[(w * 16 * QB + row) * OP + d0 + e];
         }
+        if (parts > 1) {
+            const Partial p = partial<HD>(sums, s, parts, 16 * QB, t, part, h, row);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) p.o[d0 + e] = o[e];
+            if ((tid & 15) == 0) { p.ml[0] = mm; p.ml[1] = ll; }
+            continue;
+        }
         const float inv = ll > 0.f ? 1.0f / ll : ll;               // no visible key: 0; NaN stays NaN
         T* orow = O + (int64_t)(sq.q0 + row) * s.o_sr + (int64_t)h * s.o_sh + d0;
 #pragma unroll
         for (int e = 0; e < PER; ++e) orow[e] = (T)(o[e] * inv);
         if ((tid & 15) == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + row] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
     }
+}
+
+// The states that the parts of a row's keys left, joined: one wave a row.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void causal_join_kernel(const int32_t* __restrict__ seqs, const int32_t* __restrict__ tiles,
+                                                         star_causal_shape s, int parts, int rows, const float* __restrict__ sums,
+                                                         T* __restrict__ O, float* __restrict__ lse) {
+    const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const int h = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const int i = tiles[2 * t + 1] + row;
+    if (row >= rows || i >= sq.nq) return;
+    float mm = M_NONE;
+    for (int p = 0; p < parts; ++p) mm = fmaxf(mm, partial<HD>((float*)sums, s, parts, rows, t, p, h, row).ml[0]);
+    float ll = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 2
+    for (int p = 0; p < parts; ++p) {
+        const Partial x = partial<HD>((float*)sums, s, parts, rows, t, p, h, row);
+        const float f = __builtin_amdgcn_exp2f(x.ml[0] - mm);
+        ll += f * x.ml[1];
+        o0 += f * x.o[lane];
+        if (lane + 64 < HD) o1 += f * x.o[lane + 64];
+    }
+    const float inv = ll > 0.f ? 1.0f / ll : ll;                   // no visible key: 0; NaN stays NaN
+    T* orow = O + (int64_t)(sq.q0 + i) * s.o_sr + (int64_t)h * s.o_sh;
+    orow[lane] = (T)(o0 * inv);
+    if (lane + 64 < HD) orow[lane + 64] = (T)(o1 * inv);
+    if (lane == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
 }
 
 // ------------------------------------------------------------------------------------------------------ gradient of Q
@@ -770,7 +831,7 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     }
 }
 
-// parts fp32 sums of a key tile -> dK, dV
+// parts fp32 sums of 16 keys -> dK, dV
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ seqs,
                                                             const int32_t* __restrict__ tiles, star_causal_shape s, int parts,
@@ -778,12 +839,14 @@ __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __rest
     typedef typename Vec<T>::x4 x4;
     const int hk = blockIdx.x % s.Hkv, t = blockIdx.x / s.Hkv;
     const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int j0 = tiles[2 * t + 1], rows = min(CT, sq.nk - j0);
+    const int j0 = tiles[2 * t + 1] + 16 * blockIdx.y, rows = min(16, sq.nk - j0);
     const int64_t one = s.k_rows * s.Hkv * HD;
-    for (int c = threadIdx.x; c < 2 * rows * (HD / 4); c += 256) {
-        const int which = c / (rows * (HD / 4)), cc = c % (rows * (HD / 4));
+    for (int c = threadIdx.x; c < 2 * 16 * (HD / 4); c += 256) {
+        const int which = c / (16 * (HD / 4)), cc = c % (16 * (HD / 4));
+        if (cc / (HD / 4) >= rows) continue;
         const int64_t row = sq.k0 + j0 + cc / (HD / 4), d = hk * HD + 4 * (cc % (HD / 4)), at = row * s.Hkv * HD + d;
         f32x4 sum = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int p = 0; p < parts; ++p) sum += *(const f32x4*)(sums + (2 * p + which) * one + at);
         x4 o;
 #pragma unroll
@@ -792,14 +855,16 @@ __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __rest
     }
 }
 
-// Parts of the query heads of a group: 1 when the key tiles alone make two workgroups for each of the 512 places (two a
-// CU), or when a sequence is short (under four tiles of keys on average) and its walk with it; otherwise the fewest that
-// make them.
-static int dkv_parts(const star_causal_shape* s, int nk_tiles) {
-    const int grp = s->H / s->Hkv;
+// Parts of the query heads of a group: 1 when the longest walk is short (under 16 tiles of 32 queries over all heads), or
+// the key tiles alone fill the 512 places (two workgroups a CU) once -- twice where walks go from 1 tile to 32 and more,
+// which leave no balance to a single round; otherwise the fewest that do.  Forward and backward of 2 sequences of up to 622
+// tokens, 16 heads on 2 of 96: 75 us, 217 in one part; 25 of up to 131, 32 heads on 4 of 64: 61 and 81; 8191 tokens, 16
+// heads on 4 of 128: 1223 for 1024 workgroups, 1422 for 512.
+static int dkv_parts(const star_causal_shape* s) {
+    const int grp = s->H / s->Hkv, walk = cdiv(s->max_q, CQ);
     int parts = 1;
-    if (nk_tiles >= 4 * s->nseq)
-        while (parts < grp && (int64_t)nk_tiles * s->Hkv * parts < 1024) {
+    if ((int64_t)grp * walk >= 16)
+        while (parts < grp && (int64_t)s->n_k_tiles * s->Hkv * parts < (walk >= 32 ? 1024 : 512)) {
             do ++parts; while (grp % parts);
         }
     return parts;
@@ -811,7 +876,10 @@ static int check_causal(const star_causal_shape* s, const char* who) {
     STAR_REQUIRE(s->hd == 64 || s->hd == 96 || s->hd == 128, "%s: head dim %d not in {64, 96, 128}", who, s->hd);
     STAR_REQUIRE(s->dtype == STAR_DT_BF16 || s->dtype == STAR_DT_F16, "%s: dtype %d is neither bf16 nor fp16", who, s->dtype);
     STAR_REQUIRE(s->Hkv >= 1 && s->H >= s->Hkv && s->H % s->Hkv == 0, "%s: %d query heads do not divide into %d key heads", who, s->H, s->Hkv);
-    STAR_REQUIRE(s->nseq >= 0 && s->max_q >= 0 && s->lse_stride >= 0 && s->k_rows >= 0, "%s: negative size", who);
+    STAR_REQUIRE(s->max_q >= 0 && s->max_k >= 0 && s->n_q_tiles >= 0 && s->n_k_tiles >= 0 && s->lse_stride >= 0 && s->k_rows >= 0,
+                 "%s: negative size", who);
+    STAR_REQUIRE((int64_t)s->n_q_tiles * s->H < (1ll << 31) && (int64_t)s->n_k_tiles * s->H < (1ll << 31), "%s: %d and %d tiles x %d heads",
+                 who, s->n_q_tiles, s->n_k_tiles, s->H);
     const int64_t st[8] = {s->q_sr, s->q_sh, s->k_sr, s->k_sh, s->v_sr, s->v_sh, s->o_sr, s->o_sh};
     for (int i = 0; i < 8; ++i) STAR_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
     for (int i = 0; i < 8; i += 2)
@@ -821,45 +889,58 @@ static int check_causal(const star_causal_shape* s, const char* who) {
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <typename T, int HD, int QB>
-static int launch_causal_few(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
-                             int ntiles, const star_causal_shape* s, void* o, float* lse, hipStream_t st) {
-    constexpr int tile = 4 * CK * Tile<T, HD>::ROWB, join = 4 * 16 * QB * (HD + 4) * 4, smem = tile > join ? tile : join;
-    static DevOnce once;
-    if (!reserve_lds_once(once, (const void*)causal_few_kernel<T, HD, QB>, smem)) {
-        set_error("star_causal_fwd: cannot reserve %d bytes of LDS", smem);
-        return STAR_ERR_LAUNCH;
-    }
-    hipLaunchKernelGGL((causal_few_kernel<T, HD, QB>), dim3((unsigned)ntiles * s->H), dim3(256), smem, st, (const T*)q, (const T*)k,
-                       (const T*)v, seqs, tiles, *s, (T*)o, lse);
-    return STAR_OK;
+// Rows of a workgroup of the forward, and the parts that its keys are cut into: 1 when the query tiles alone fill half of
+// the 512 places (two workgroups a CU) or the keys are few, otherwise so many that they fill them, each of at least 8
+// tiles of keys (two for every wave of the few-query kernel; a part costs its state's trip to memory and a join).
+// 29 queries over 17 sequences of up to 4321 keys, one head of 128: 22 us, 58 in one part; 73 queries over two of up to 4686
+// keys, 24 heads of 96: 33 and 106.
+static int fwd_rows(const star_causal_shape* s) { return s->max_q <= 16 ? 16 : s->max_q <= 32 ? 32 : CT; }
+static int fwd_parts(const star_causal_shape* s) {
+    const int64_t wgs = (int64_t)s->n_q_tiles * s->H;
+    const int most = cdiv(s->max_k, CK) / 8;
+    if (wgs < 1 || wgs >= 256 || most < 2) return 1;
+    return (int)min((int64_t)most, 512 / wgs);
+}
+static int64_t causal_fwd_bytes(const star_causal_shape* s) {
+    const int parts = fwd_parts(s);
+    return parts == 1 ? 0 : (int64_t)s->n_q_tiles * s->H * parts * fwd_rows(s) * (s->hd + 2) * 4;
 }
 
 template <typename T, int HD>
 static int launch_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
-                             int ntiles, const star_causal_shape* s, void* o, float* lse, hipStream_t st) {
-    if (s->max_q <= 16) return launch_causal_few<T, HD, 1>(q, k, v, seqs, tiles, ntiles, s, o, lse, st);
-    if (s->max_q <= 32) return launch_causal_few<T, HD, 2>(q, k, v, seqs, tiles, ntiles, s, o, lse, st);
-    constexpr int smem = 4 * CK * Tile<T, HD>::ROWB;
-    static DevOnce once;
-    if (!reserve_lds_once(once, (const void*)causal_fwd_kernel<T, HD>, smem)) {
+                             const star_causal_shape* s, void* o, float* lse, float* sums, hipStream_t st) {
+    constexpr int tile = 4 * CK * Tile<T, HD>::ROWB, join2 = 4 * 32 * (HD + 4) * 4;
+    constexpr int smem_few = tile > join2 ? tile : join2;
+    const int rows = fwd_rows(s), parts = fwd_parts(s);
+    const void* fn = rows == 16 ? (const void*)causal_few_kernel<T, HD, 1> : rows == 32 ? (const void*)causal_few_kernel<T, HD, 2>
+                                                                                       : (const void*)causal_fwd_kernel<T, HD>;
+    const int smem = rows == CT ? tile : smem_few;
+    static DevOnce once[3];
+    if (!reserve_lds_once(once[rows == 16 ? 0 : rows == 32 ? 1 : 2], fn, smem)) {
         set_error("star_causal_fwd: cannot reserve %d bytes of LDS", smem);
         return STAR_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL((causal_fwd_kernel<T, HD>), dim3((unsigned)ntiles * s->H), dim3(256), smem, st, (const T*)q, (const T*)k,
-                       (const T*)v, seqs, tiles, *s, (T*)o, lse);
+    const dim3 grid((unsigned)((int64_t)s->n_q_tiles * s->H * parts));
+#define CAUSAL_FWD_ARGS grid, dim3(256), smem, st, (const T*)q, (const T*)k, (const T*)v, seqs, tiles, *s, parts, sums, (T*)o, lse
+    if (rows == 16) hipLaunchKernelGGL((causal_few_kernel<T, HD, 1>), CAUSAL_FWD_ARGS);
+    else if (rows == 32) hipLaunchKernelGGL((causal_few_kernel<T, HD, 2>), CAUSAL_FWD_ARGS);
+    else hipLaunchKernelGGL((causal_fwd_kernel<T, HD>), CAUSAL_FWD_ARGS);
+#undef CAUSAL_FWD_ARGS
+    if (parts > 1)
+        hipLaunchKernelGGL((causal_join_kernel<T, HD>), dim3((unsigned)((int64_t)s->n_q_tiles * s->H), rows / 4), dim3(256), 0, st,
+                           seqs, tiles, *s, parts, rows, (const float*)sums, (T*)o, lse);
     return STAR_OK;
 }
 
-static int64_t causal_bwd_bytes(const star_causal_shape* s, int nk_tiles) {
-    const int parts = dkv_parts(s, nk_tiles);
+static int64_t causal_bwd_bytes(const star_causal_shape* s) {
+    const int parts = dkv_parts(s);
     return parts == 1 ? 0 : (int64_t)parts * 2 * s->k_rows * s->Hkv * s->hd * 4;
 }
 
 template <typename T, int HD>
 static int launch_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                             const int32_t* seqs, const int32_t* q_tiles, int nq_tiles, const int32_t* k_tiles,
-                             int nk_tiles, const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta,
+                             const int32_t* seqs, const int32_t* q_tiles, const int32_t* k_tiles,
+                             const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta,
                              float* sums, hipStream_t st) {
     constexpr int smem_q = 4 * CK * Tile<T, HD>::ROWB;
     constexpr int smem_k = CT * Tile<T, HD>::ROWB + 2 * (2 * CQ * Tile<T, HD>::ROWB + 2 * CQ * 4);
@@ -869,16 +950,16 @@ static int launch_causal_bwd(const void* q, const void* k, const void* v, const 
         set_error("star_causal_bwd: cannot reserve %d bytes of LDS", smem_k);
         return STAR_ERR_LAUNCH;
     }
-    if (nq_tiles > 0)
-        hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3((unsigned)nq_tiles * s->H), dim3(256), smem_q, st, (const T*)q,
+    if (s->n_q_tiles > 0)
+        hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3((unsigned)s->n_q_tiles * s->H), dim3(256), smem_q, st, (const T*)q,
                            (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, seqs, q_tiles, *s, (T*)dq, delta);
-    if (nk_tiles > 0) {
-        const int parts = dkv_parts(s, nk_tiles);
-        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)nk_tiles * s->Hkv * parts), dim3(256), smem_k, st,
+    if (s->n_k_tiles > 0) {
+        const int parts = dkv_parts(s);
+        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)s->n_k_tiles * s->Hkv * parts), dim3(256), smem_k, st,
                            (const T*)q, (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, seqs, k_tiles, *s,
                            parts, sums, (T*)dk, (T*)dv);
         if (parts > 1)
-            hipLaunchKernelGGL((causal_dkv_sum_kernel<T, HD>), dim3((unsigned)nk_tiles * s->Hkv), dim3(256), 0, st,
+            hipLaunchKernelGGL((causal_dkv_sum_kernel<T, HD>), dim3((unsigned)s->n_k_tiles * s->Hkv, CT / 16), dim3(256), 0, st,
                                (const float*)sums, seqs, k_tiles, *s, parts, (T*)dk, (T*)dv);
     }
     return STAR_OK;
@@ -899,49 +980,57 @@ static int launch_causal_bwd(const void* q, const void* k, const void* v, const 
 
 }  // namespace star
 
+extern "C" size_t star_causal_fwd_workspace(const star_causal_shape* s) {
+    using namespace star;
+    return check_causal(s, "star_causal_fwd_workspace") ? 0 : (size_t)causal_fwd_bytes(s);
+}
+
 extern "C" int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
-                               int ntiles, const star_causal_shape* s, void* o, float* lse, void* stream) {
+                               const star_causal_shape* s, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                               void* stream) {
     using namespace star;
     int rc = check_causal(s, "star_causal_fwd");
     if (rc) return rc;
-    STAR_REQUIRE(ntiles >= 0 && (int64_t)ntiles * s->H < (1ll << 31), "star_causal_fwd: %d tiles x %d heads", ntiles, s->H);
-    if (ntiles == 0) return STAR_OK;
+    if (s->n_q_tiles == 0) return STAR_OK;
     STAR_REQUIRE(q && k && v && seqs && tiles && o && lse, "star_causal_fwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "star_causal_fwd: tensors must be 16-byte aligned");
-    CAUSAL_BY_TYPE((launch_causal_fwd<T, HD>(q, k, v, seqs, tiles, ntiles, s, o, lse, (hipStream_t)stream)));
+    const int64_t need = causal_fwd_bytes(s);
+    if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !aligned16(workspace))) {
+        set_error("star_causal_fwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);
+        return STAR_ERR_WORKSPACE;
+    }
+    CAUSAL_BY_TYPE((launch_causal_fwd<T, HD>(q, k, v, seqs, tiles, s, o, lse, (float*)workspace, (hipStream_t)stream)));
     if (rc) return rc;
     STAR_LAUNCH_CHECK("star_causal_fwd");
     return STAR_OK;
 }
 
-extern "C" size_t star_causal_bwd_workspace(const star_causal_shape* s, int nk_tiles) {
+extern "C" size_t star_causal_bwd_workspace(const star_causal_shape* s) {
     using namespace star;
-    return check_causal(s, "star_causal_bwd_workspace") || nk_tiles < 0 ? 0 : (size_t)causal_bwd_bytes(s, nk_tiles);
+    return check_causal(s, "star_causal_bwd_workspace") ? 0 : (size_t)causal_bwd_bytes(s);
 }
 
 extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_,
-                               const float* lse, const int32_t* seqs, const int32_t* q_tiles, int nq_tiles,
-                               const int32_t* k_tiles, int nk_tiles, const star_causal_shape* s, void* dq, void* dk,
-                               void* dv, float* delta, void* workspace, size_t workspace_bytes, void* stream) {
+                               const float* lse, const int32_t* seqs, const int32_t* q_tiles, const int32_t* k_tiles,
+                               const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta, void* workspace,
+                               size_t workspace_bytes, void* stream) {
     using namespace star;
     int rc = check_causal(s, "star_causal_bwd");
     if (rc) return rc;
-    STAR_REQUIRE(nq_tiles >= 0 && nk_tiles >= 0 && (int64_t)nq_tiles * s->H < (1ll << 31) && (int64_t)nk_tiles * s->H < (1ll << 31),
-                 "star_causal_bwd: %d and %d tiles x %d heads", nq_tiles, nk_tiles, s->H);
-    if (nq_tiles == 0 && nk_tiles == 0) return STAR_OK;
-    STAR_REQUIRE(q && k && v && o && do_ && lse && seqs && (q_tiles || !nq_tiles) && (k_tiles || !nk_tiles) && dq && dk && dv && delta,
+    if (s->n_q_tiles == 0 && s->n_k_tiles == 0) return STAR_OK;
+    STAR_REQUIRE(q && k && v && o && do_ && lse && seqs && (q_tiles || !s->n_q_tiles) && (k_tiles || !s->n_k_tiles) && dq && dk && dv && delta,
                  "star_causal_bwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(do_) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                  "star_causal_bwd: tensors must be 16-byte aligned");
     STAR_REQUIRE(s->dq_sr % 8 == 0 && s->dkv_sr % 8 == 0 && s->dq_sr >= (int64_t)s->H * s->hd && s->dkv_sr >= (int64_t)s->Hkv * s->hd,
                  "star_causal_bwd: gradient row strides %lld, %lld", (long long)s->dq_sr, (long long)s->dkv_sr);
-    const int64_t need = causal_bwd_bytes(s, nk_tiles);
+    const int64_t need = causal_bwd_bytes(s);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !aligned16(workspace))) {
         set_error("star_causal_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);
         return STAR_ERR_WORKSPACE;
     }
-    CAUSAL_BY_TYPE((launch_causal_bwd<T, HD>(q, k, v, o, do_, lse, seqs, q_tiles, nq_tiles, k_tiles, nk_tiles, s, dq, dk, dv,
-                                             delta, (float*)workspace, (hipStream_t)stream)));
+    CAUSAL_BY_TYPE((launch_causal_bwd<T, HD>(q, k, v, o, do_, lse, seqs, q_tiles, k_tiles, s, dq, dk, dv, delta, (float*)workspace,
+                                             (hipStream_t)stream)));
     if (rc) return rc;
     STAR_LAUNCH_CHECK("star_causal_bwd");
     return STAR_OK;

@@ -38,6 +38,8 @@ __device__ __forceinline__ u32x2 codes8(const X8& x, float inv) {
     return r;
 }
 
+__device__ __forceinline__ int count(int32_t* p) { return __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 struct AppendArgs {
     star_kv8_cache c;
     const void *k, *v;
@@ -184,16 +186,20 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
         }
     }
     // lens is read by every workgroup of the sequence and changed by the last of them to get here: a workgroup's count
-    // goes out after its own read has come back (the value has steered everything above), so no fence is needed.  The
-    // counters of two sequences lie in different cache lines.
+    // goes out after its own read has come back (the value has steered everything above), so no fence is needed.  Counted
+    // in two steps, first among the workgroups of one head's K or V, each counter in a cache line of its own: one counter
+    // for all of 3432 workgroups took longer than their work.
     __syncthreads();
     if (tid == 0) {
-        const int total = (int)(gridDim.x * gridDim.y);
-        int32_t* ticket = c.tickets + (int64_t)b * STAR_KV8_TICKET_STRIDE;
-        if (__hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == total - 1) {
-            c.lens[b] = end;
-            if (want > n) c.dropped[b] += want - n;
-            *ticket = 0;
+        int32_t* ticket = c.tickets + (int64_t)b * (1 + 2 * c.Hkv) * STAR_KV8_TICKET_STRIDE;
+        int32_t* mine = ticket + (1 + blockIdx.y) * STAR_KV8_TICKET_STRIDE;
+        if (gridDim.x == 1 || count(mine) == (int)gridDim.x - 1) {
+            if (gridDim.x > 1) *mine = 0;
+            if (count(ticket) == (int)gridDim.y - 1) {
+                c.lens[b] = end;
+                if (want > n) c.dropped[b] += want - n;
+                *ticket = 0;
+            }
         }
     }
 }

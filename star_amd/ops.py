@@ -1688,8 +1688,11 @@ def _causal_forward(q, k, v, plan, s):
     lse = torch.empty((s.H, s.lse_stride), dtype=torch.float32, device=q.device)
     if plan.q_used != s.lse_stride:
         lse.fill_(-math.inf)
+    # (only launches of few workgroups over many keys are cut along the keys)
+    need = lib().star_causal_fwd_workspace(s) if plan.max_k > 960 and plan.n_q_tiles * s.H < 256 else 0
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     _launch(lib().star_causal_fwd, "star_causal_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.seqs.data_ptr(),
-            plan.q_tiles.data_ptr(), plan.n_q_tiles, s, o.data_ptr(), lse.data_ptr())
+            plan.q_tiles.data_ptr(), s, o.data_ptr(), lse.data_ptr(), ptr(ws), need)
     return o, lse
 
 
@@ -1701,11 +1704,11 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
     if g.data_ptr() % 16:
         g = g.clone()
     delta = torch.empty_like(lse)
-    need = lib().star_causal_bwd_workspace(s, plan.n_k_tiles) if s.H != s.Hkv else 0
+    need = lib().star_causal_bwd_workspace(s) if s.H != s.Hkv else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     _launch(lib().star_causal_bwd, "star_causal_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            g.data_ptr(), lse.data_ptr(), plan.seqs.data_ptr(), plan.q_tiles.data_ptr(), plan.n_q_tiles,
-            plan.k_tiles.data_ptr(), plan.n_k_tiles, s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+            g.data_ptr(), lse.data_ptr(), plan.seqs.data_ptr(), plan.q_tiles.data_ptr(),
+            plan.k_tiles.data_ptr(), s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
             ptr(ws), need)
 
 
@@ -1815,7 +1818,8 @@ def _causal_shape(q, k, v, plan, scale):
     s.k_sr, s.k_sh = _row_strides("causal_attn", "k", k)
     s.v_sr, s.v_sh = _row_strides("causal_attn", "v", v)
     s.o_sr, s.o_sh = H * hd, hd
-    s.H, s.Hkv, s.hd, s.dtype, s.nseq, s.max_q = H, Hkv, hd, _DT16[q.dtype], plan.n, plan.max_q
+    s.H, s.Hkv, s.hd, s.dtype, s.max_q, s.max_k = H, Hkv, hd, _DT16[q.dtype], plan.max_q, plan.max_k
+    s.n_q_tiles, s.n_k_tiles = plan.n_q_tiles, plan.n_k_tiles
     s.lse_stride, s.k_rows, s.scale = rows, k_rows, scale
     return s
 
@@ -1877,7 +1881,7 @@ class KVCache8:
             setattr(self, n, t)
         self.batch, self.kv_heads, self.capacity, self.head_dim, self.dtype, self.device = B, H, T, hd, dt, dev
         self._dropped = torch.zeros(B, dtype=torch.int32, device=dev)
-        self._tickets = torch.zeros(B * KV8_TICKET_STRIDE, dtype=torch.int32, device=dev)
+        self._tickets = torch.zeros(B * (1 + 2 * H) * KV8_TICKET_STRIDE, dtype=torch.int32, device=dev)
         self._workspace = {}                       # bytes of kv8_attn's workspace by (heads, queries)
         c = self._c = KV8Cache()
         c.B, c.Hkv, c.T, c.hd, c.dtype = B, H, T, hd, _DT16[dt]

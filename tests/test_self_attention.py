@@ -88,6 +88,11 @@ SHAPES = [  # keys, queries (None: the same), H, Hkv, hd, dtype
     ([3, 700, 64, 0, 257], [16, 1, 9, 2, 16], 4, 2, 128, BF),  # few queries each: the waves share them
     ([520, 5, 1], [30, 17, 1], 2, 1, 64, FP),
     ([100, 300], [32, 20], 3, 3, 96, BF),
+    # few query tiles over many keys, cut along them and joined
+    ([5000, 64, 0, 1030], [16, 7, 0, 1], 2, 1, 128, BF),
+    ([3001], [30], 2, 2, 64, FP),
+    ([2000, 100], [130, 100], 2, 1, 96, BF),
+    ([10, 1500], [200, 60], 1, 1, 128, FP),
 ]
 
 
@@ -665,28 +670,39 @@ def test_cpu_tensors_are_refused(ops):
 def test_the_library_checks_sizes_before_any_launch():
     from star_amd import _lib
     L = _lib.lib()
-    s = _lib.CausalShape(H=4, Hkv=2, hd=80, dtype=0)
-    assert L.star_causal_fwd(1, 1, 1, 1, 1, 1, s, 1, 1, None) == -1 and b"head dim 80" in L.star_last_error()
-    s = _lib.CausalShape(H=4, Hkv=3, hd=64, dtype=0)
-    assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"divide" in L.star_last_error()
-    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=1)
-    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 1, 16, 1, s, 16, 16, 16, 16, None, 0, None) == -1 and b"dtype" in L.star_last_error()
-    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, q_sr=4)
-    assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"multiples of 8" in L.star_last_error()
-    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, q_sr=1 << 23, scale=1)
-    assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"row stride" in L.star_last_error()
-    for scale in (0.0, -1.0, math.inf, math.nan):
-        s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, scale=scale)
-        assert L.star_causal_fwd(16, 16, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"scale" in L.star_last_error()
-    s = _lib.CausalShape(H=4, Hkv=2, hd=64, dtype=0, scale=1)
-    assert L.star_causal_fwd(16, 24, 16, 16, 16, 1, s, 16, 16, None) == -1 and b"aligned" in L.star_last_error()
-    assert L.star_causal_fwd(None, None, None, None, None, 0, s, None, None, None) == 0
-    s = _lib.CausalShape(H=4, Hkv=1, hd=64, dtype=0, nseq=1, k_rows=2000, scale=1, dq_sr=256, dkv_sr=64)
-    assert L.star_causal_bwd_workspace(s, 16) > 0 and L.star_causal_bwd_workspace(s, 3) == 0
+    S = _lib.CausalShape
+    fwd = lambda s, k=16, ws=None, n=0: L.star_causal_fwd(16, k, 16, 16, 16, s, 16, 16, ws, n, None)  # noqa: E731
+    bwd = lambda s, ws=None, n=0: L.star_causal_bwd(*[16] * 9, s, 16, 16, 16, 16, ws, n, None)  # noqa: E731
+    for kw, text in [(dict(hd=80), b"head dim 80"), (dict(Hkv=3), b"divide"), (dict(dtype=1), b"dtype"), (dict(q_sr=4), b"multiples of 8"),
+                     (dict(q_sr=1 << 23), b"row stride"), (dict(q_sr=-8), b"row stride"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"),
+                     (dict(scale=math.inf), b"scale"), (dict(scale=math.nan), b"scale"), (dict(max_k=-1), b"negative"),
+                     (dict(n_k_tiles=1 << 30), b"tiles x 4 heads")]:
+        s = S(**{**dict(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1), **kw})
+        for call in (fwd, bwd):
+            assert call(s) == -1 and text in L.star_last_error(), kw
+        assert L.star_causal_fwd_workspace(s) == 0 and L.star_causal_bwd_workspace(s) == 0
+    s = S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1)
+    assert fwd(s, k=24) == -1 and b"aligned" in L.star_last_error()
+    assert fwd(s, k=None) == -1 and b"null pointer" in L.star_last_error()
+    assert L.star_causal_fwd(None, None, None, None, None, S(H=4, Hkv=2, hd=64, dtype=0, scale=1), None, None, None, 0, None) == 0
+    # cut along the keys: few query tiles, many keys
+    need = lambda nq, n, nk: L.star_causal_fwd_workspace(S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=n, max_q=nq, max_k=nk))  # noqa: E731
+    assert need(16, 1, 960) == 0 and need(16, 1, 1024) == 4 * 2 * 16 * 66 * 4 and need(16, 64, 100000) == 0
+    assert need(17, 2, 10 ** 6) == 2 * 4 * 64 * 32 * 66 * 4 and need(33, 63, 10 ** 6) == 63 * 4 * 2 * 128 * 66 * 4
+    s = S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1, max_q=16, max_k=4096)
+    assert fwd(s) == -3 and b"workspace" in L.star_last_error() and fwd(s, ws=16, n=100) == -3 and fwd(s, ws=24, n=1 << 30) == -3
+    # cut by query heads: few key tiles, long walks
+    s = S(H=4, Hkv=1, hd=64, dtype=0, k_rows=2000, scale=1, dq_sr=256, dkv_sr=64, n_k_tiles=16, max_q=2000)
+    assert L.star_causal_bwd_workspace(s) == 4 * 2 * 2000 * 64 * 4
+    assert bwd(s) == -3 and b"workspace" in L.star_last_error()
     s.dq_sr = 128
-    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, s, 16, 16, 16, 16, None, 0, None) == -1 and b"gradient row" in L.star_last_error()
-    s.dq_sr = 256
-    assert L.star_causal_bwd(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, s, 16, 16, 16, 16, None, 0, None) == -3 and b"workspace" in L.star_last_error()
+    assert bwd(s) == -1 and b"gradient row" in L.star_last_error()
+    s.n_k_tiles = 512
+    assert L.star_causal_bwd_workspace(s) == 2 * 2 * 2000 * 64 * 4
+    s.n_k_tiles = 1024
+    assert L.star_causal_bwd_workspace(s) == 0
+    s.n_k_tiles, s.max_q = 16, 96
+    assert L.star_causal_bwd_workspace(s) == 0
     c = _lib.KV8Cache(B=1, Hkv=2, T=100, hd=64, dtype=0)
     assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 0, 0, None, None, 1, None, 1, None) == -1 and b"capacity 100" in L.star_last_error()
     c = _lib.KV8Cache(B=1, Hkv=2, T=128, hd=64, dtype=0)
