@@ -457,10 +457,10 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
  * behind the other instead of in a padded batch, with grouped heads (query head h reads key head h / (H / Hkv)).
  *   q [rows,H,hd], k / v [rows,Hkv,hd], o like q: 16-bit values of one type (dtype), hd contiguous, row and head
  *        strides in elements, multiples of 8; base addresses multiples of 16 bytes.  hd in {64, 96, 128}
- *   seqs [nseq][4] int32: first query row, queries nq, first key row, keys nk.  Query i of a sequence sees its keys
- *        j <= i + nk - nq (the queries are the newest nq positions); a query that sees no key gets o = 0, lse = -inf
- *   tiles [n_q_tiles][2] int32: sequence and first query of every tile of STAR_CAUSAL_TILE queries, each exactly once, in
- *        the order in which they are to start (longest first balances the load).  Rows in no sequence are not touched
+ *   tiles [n_q_tiles][8] int32, every tile of STAR_CAUSAL_TILE queries of every sequence exactly once, in the order in which
+ *        they are to start: the sequence's first query row, queries nq, first key row and keys nk, the tile's first query,
+ *        and three unused words.  Query i of a sequence sees its keys j <= i + nk - nq (the queries are the newest nq
+ *        positions); a query that sees no key gets o = 0, lse = -inf.  Rows in no sequence are not touched
  *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward
  * Softmax statistics and sums are fp32; the weights P are rounded to dtype for the product with V (as the inputs are).
  * Nothing is masked by arithmetic on values: a key after the query never enters its maximum, sum or output, with one
@@ -480,15 +480,15 @@ typedef struct {
 } star_causal_shape;
 /* workspace (here and below): star_causal_*_workspace(s) bytes, 0 for most calls, 16-byte aligned, used by this call only */
 size_t star_causal_fwd_workspace(const star_causal_shape* s);
-int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* tiles,
                     const star_causal_shape* s, void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 /* Backward: P recomputed from lse.  do_ has o's strides; dq [rows,H,hd] and dk / dv [rows,Hkv,hd] may be column
- * ranges of one matrix (dq_sr, dkv_sr, multiples of 8).  q_tiles as tiles above; k_tiles [n_k_tiles][2]: the same for
+ * ranges of one matrix (dq_sr, dkv_sr, multiples of 8).  q_tiles as tiles above; k_tiles [n_k_tiles][8]: the same for
  * tiles of STAR_CAUSAL_TILE keys.  delta [H][lse_stride] fp32 scratch.
  * No atomics: the gradient of a shared key head is summed over its query heads in a fixed order. */
 size_t star_causal_bwd_workspace(const star_causal_shape* s);
 int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                    const int32_t* seqs, const int32_t* q_tiles, const int32_t* k_tiles, const star_causal_shape* s,
+                    const int32_t* q_tiles, const int32_t* k_tiles, const star_causal_shape* s,
                     void* dq, void* dk, void* dv, float* delta, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- 8-bit key/value cache and attention over it

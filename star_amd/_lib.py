@@ -105,9 +105,9 @@ SIGNATURES = {
     "star_colsum": (_I, [_P, _I, _I64, _I, _I64, _P, _P, _SZ, _P]),
     "star_colsum_batched": (_I, [C.POINTER(C.c_void_p), _I, _I, _I64, _I, _I64, _P, _P, _SZ, _P]),
     "star_causal_fwd_workspace": (_SZ, [C.POINTER(CausalShape)]),
-    "star_causal_fwd": (_I, [_P, _P, _P, _P, _P, C.POINTER(CausalShape), _P, _P, _P, _SZ, _P]),
+    "star_causal_fwd": (_I, [_P, _P, _P, _P, C.POINTER(CausalShape), _P, _P, _P, _SZ, _P]),
     "star_causal_bwd_workspace": (_SZ, [C.POINTER(CausalShape)]),
-    "star_causal_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, C.POINTER(CausalShape), _P, _P, _P, _P, _P, _SZ, _P]),
+    "star_causal_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, C.POINTER(CausalShape), _P, _P, _P, _P, _P, _SZ, _P]),
     "star_kv8_append": (_I, [C.POINTER(KV8Cache), _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I, _P, _I, _P]),
     "star_kv8_attn_workspace": (_SZ, [C.POINTER(KV8Cache), _I, _I]),
     "star_kv8_attn": (_I, [C.POINTER(KV8Cache), _P, _P, _P, C.POINTER(KV8Query), _P, _P, _SZ, _P]),

@@ -18,9 +18,10 @@ namespace star {
 constexpr int CT = STAR_CAUSAL_TILE;     // rows of one workgroup: 4 waves x 32
 constexpr int CK = 64;                   // rows of the tiles it walks
 
-struct SeqOf { int q0, nq, k0, nk; };
-__device__ __forceinline__ SeqOf seq_of(const int32_t* seqs, int s) {
-    return SeqOf{seqs[4 * s], seqs[4 * s + 1], seqs[4 * s + 2], seqs[4 * s + 3]};
+struct Work { int q0, nq, k0, nk, first; };      // a tile's sequence (first query row, queries, first key row, keys), its first row
+__device__ __forceinline__ Work work_of(const int32_t* tiles, int t) {
+    const int32_t* w = tiles + 8 * (int64_t)t;
+    return Work{w[0], w[1], w[2], w[3], w[4]};
 }
 
 // Few query tiles over long keys are cut along the keys: part p of `parts` walks its share of a tile's key tiles and
@@ -40,8 +41,7 @@ __device__ __forceinline__ Partial partial(float* sums, const star_causal_shape&
 // ------------------------------------------------------------------------------------------------------ forward
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K,
-                                                           const T* __restrict__ V, const int32_t* __restrict__ seqs,
-                                                           const int32_t* __restrict__ tiles, star_causal_shape s,
+                                                           const T* __restrict__ V, const int32_t* __restrict__ tiles, star_causal_shape s,
                                                            int parts, float* __restrict__ sums, T* __restrict__ O,
                                                            float* __restrict__ lse) {
     typedef typename Vec<T>::x8 x8;
@@ -57,8 +57,8 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
     // key head meet in one L2 when Hkv is a multiple of 8
     const int hi = blockIdx.x % s.H, part = blockIdx.x / s.H % parts, t = blockIdx.x / s.H / parts;
     const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
-    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int i0 = tiles[2 * t + 1];                               // first query of the workgroup
+    const Work sq = work_of(tiles, t);
+    const int i0 = sq.first;                               // first query of the workgroup
     const int off = sq.nk - sq.nq;
     const T* Qh = Q + (int64_t)sq.q0 * s.q_sr + (int64_t)h * s.q_sh;
     const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
@@ -228,8 +228,7 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
 // four without a query.
 template <typename T, int HD, int QB>
 __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict__ Q, const T* __restrict__ K,
-                                                           const T* __restrict__ V, const int32_t* __restrict__ seqs,
-                                                           const int32_t* __restrict__ tiles, star_causal_shape s,
+                                                           const T* __restrict__ V, const int32_t* __restrict__ tiles, star_causal_shape s,
                                                            int parts, float* __restrict__ sums, T* __restrict__ O,
                                                            float* __restrict__ lse) {
     typedef typename Vec<T>::x8 x8;
@@ -242,7 +241,7 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
     const int r16 = lane & 15, g = lane >> 4;
     const int hi = blockIdx.x % s.H, part = blockIdx.x / s.H % parts, t = blockIdx.x / s.H / parts;
     const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
-    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
+    const Work sq = work_of(tiles, t);
     const int off = sq.nk - sq.nq;                                 // (the last query sees every key)
     const KeyTiles kt_ = key_tiles(sq.nk, part, parts);
     const int end = min(sq.nk, kt_.end * CK);
@@ -392,13 +391,13 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
 
 // The states that the parts of a row's keys left, joined: one wave a row.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void causal_join_kernel(const int32_t* __restrict__ seqs, const int32_t* __restrict__ tiles,
+__global__ __launch_bounds__(256) void causal_join_kernel(const int32_t* __restrict__ tiles,
                                                          star_causal_shape s, int parts, int rows, const float* __restrict__ sums,
                                                          T* __restrict__ O, float* __restrict__ lse) {
     const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + (threadIdx.x >> 6);
     const int h = blockIdx.x % s.H, t = blockIdx.x / s.H;
-    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int i = tiles[2 * t + 1] + row;
+    const Work sq = work_of(tiles, t);
+    const int i = sq.first + row;
     if (row >= rows || i >= sq.nq) return;
     float mm = M_NONE;
     for (int p = 0; p < parts; ++p) mm = fmaxf(mm, partial<HD>((float*)sums, s, parts, rows, t, p, h, row).ml[0]);
@@ -428,7 +427,6 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                           const T* __restrict__ V, const T* __restrict__ O,
                                                           const T* __restrict__ dO, const float* __restrict__ lse,
-                                                          const int32_t* __restrict__ seqs,
                                                           const int32_t* __restrict__ tiles, star_causal_shape s,
                                                           T* __restrict__ dQ, float* __restrict__ delta) {
     typedef typename Vec<T>::x8 x8;
@@ -442,8 +440,8 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
     const int r16 = lane & 15, g = lane >> 4;
     const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
     const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
-    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int i0 = tiles[2 * t + 1];
+    const Work sq = work_of(tiles, t);
+    const int i0 = sq.first;
     const int off = sq.nk - sq.nq;
     const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
     const T* Vh = V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh;
@@ -644,7 +642,6 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                            const T* __restrict__ V, const T* __restrict__ dO,
                                                            const float* __restrict__ lse, const float* __restrict__ delta,
-                                                           const int32_t* __restrict__ seqs,
                                                            const int32_t* __restrict__ tiles, star_causal_shape s,
                                                            int parts, float* __restrict__ sums, T* __restrict__ dK,
                                                            T* __restrict__ dV) {
@@ -659,8 +656,8 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     const int r16 = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % s.Hkv, part = blockIdx.x / s.Hkv % parts, t = blockIdx.x / s.Hkv / parts;
     const int heads = s.H / s.Hkv / parts, h0 = hk * (s.H / s.Hkv) + part * heads;
-    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int j0 = tiles[2 * t + 1], w0 = j0 + 32 * wid;           // first key of the workgroup, of the wave
+    const Work sq = work_of(tiles, t);
+    const int j0 = sq.first, w0 = j0 + 32 * wid;           // first key of the workgroup, of the wave
     const int off = sq.nk - sq.nq;
     uint8_t* vt = smem + 32 * wid * Ti::ROWB;                      // the wave's rows of V
 
@@ -833,13 +830,12 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
 
 // parts fp32 sums of 16 keys -> dK, dV
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ seqs,
-                                                            const int32_t* __restrict__ tiles, star_causal_shape s, int parts,
+__global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ tiles, star_causal_shape s, int parts,
                                                             T* __restrict__ dK, T* __restrict__ dV) {
     typedef typename Vec<T>::x4 x4;
     const int hk = blockIdx.x % s.Hkv, t = blockIdx.x / s.Hkv;
-    const SeqOf sq = seq_of(seqs, tiles[2 * t]);
-    const int j0 = tiles[2 * t + 1] + 16 * blockIdx.y, rows = min(16, sq.nk - j0);
+    const Work sq = work_of(tiles, t);
+    const int j0 = sq.first + 16 * blockIdx.y, rows = min(16, sq.nk - j0);
     const int64_t one = s.k_rows * s.Hkv * HD;
     for (int c = threadIdx.x; c < 2 * 16 * (HD / 4); c += 256) {
         const int which = c / (16 * (HD / 4)), cc = c % (16 * (HD / 4));
@@ -907,7 +903,7 @@ static int64_t causal_fwd_bytes(const star_causal_shape* s) {
 }
 
 template <typename T, int HD>
-static int launch_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+static int launch_causal_fwd(const void* q, const void* k, const void* v, const int32_t* tiles,
                              const star_causal_shape* s, void* o, float* lse, float* sums, hipStream_t st) {
     constexpr int tile = 4 * CK * Tile<T, HD>::ROWB, join2 = 4 * 32 * (HD + 4) * 4;
     constexpr int smem_few = tile > join2 ? tile : join2;
@@ -921,14 +917,14 @@ static int launch_causal_fwd(const void* q, const void* k, const void* v, const 
         return STAR_ERR_LAUNCH;
     }
     const dim3 grid((unsigned)((int64_t)s->n_q_tiles * s->H * parts));
-#define CAUSAL_FWD_ARGS grid, dim3(256), smem, st, (const T*)q, (const T*)k, (const T*)v, seqs, tiles, *s, parts, sums, (T*)o, lse
+#define CAUSAL_FWD_ARGS grid, dim3(256), smem, st, (const T*)q, (const T*)k, (const T*)v, tiles, *s, parts, sums, (T*)o, lse
     if (rows == 16) hipLaunchKernelGGL((causal_few_kernel<T, HD, 1>), CAUSAL_FWD_ARGS);
     else if (rows == 32) hipLaunchKernelGGL((causal_few_kernel<T, HD, 2>), CAUSAL_FWD_ARGS);
     else hipLaunchKernelGGL((causal_fwd_kernel<T, HD>), CAUSAL_FWD_ARGS);
 #undef CAUSAL_FWD_ARGS
     if (parts > 1)
         hipLaunchKernelGGL((causal_join_kernel<T, HD>), dim3((unsigned)((int64_t)s->n_q_tiles * s->H), rows / 4), dim3(256), 0, st,
-                           seqs, tiles, *s, parts, rows, (const float*)sums, (T*)o, lse);
+                           tiles, *s, parts, rows, (const float*)sums, (T*)o, lse);
     return STAR_OK;
 }
 
@@ -939,7 +935,7 @@ static int64_t causal_bwd_bytes(const star_causal_shape* s) {
 
 template <typename T, int HD>
 static int launch_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                             const int32_t* seqs, const int32_t* q_tiles, const int32_t* k_tiles,
+                             const int32_t* q_tiles, const int32_t* k_tiles,
                              const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta,
                              float* sums, hipStream_t st) {
     constexpr int smem_q = 4 * CK * Tile<T, HD>::ROWB;
@@ -952,15 +948,15 @@ static int launch_causal_bwd(const void* q, const void* k, const void* v, const 
     }
     if (s->n_q_tiles > 0)
         hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3((unsigned)s->n_q_tiles * s->H), dim3(256), smem_q, st, (const T*)q,
-                           (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, seqs, q_tiles, *s, (T*)dq, delta);
+                           (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, q_tiles, *s, (T*)dq, delta);
     if (s->n_k_tiles > 0) {
         const int parts = dkv_parts(s);
         hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)s->n_k_tiles * s->Hkv * parts), dim3(256), smem_k, st,
-                           (const T*)q, (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, seqs, k_tiles, *s,
+                           (const T*)q, (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, k_tiles, *s,
                            parts, sums, (T*)dk, (T*)dv);
         if (parts > 1)
             hipLaunchKernelGGL((causal_dkv_sum_kernel<T, HD>), dim3((unsigned)s->n_k_tiles * s->Hkv, CT / 16), dim3(256), 0, st,
-                               (const float*)sums, seqs, k_tiles, *s, parts, (T*)dk, (T*)dv);
+                               (const float*)sums, k_tiles, *s, parts, (T*)dk, (T*)dv);
     }
     return STAR_OK;
 }
@@ -985,21 +981,21 @@ extern "C" size_t star_causal_fwd_workspace(const star_causal_shape* s) {
     return check_causal(s, "star_causal_fwd_workspace") ? 0 : (size_t)causal_fwd_bytes(s);
 }
 
-extern "C" int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* tiles,
+extern "C" int star_causal_fwd(const void* q, const void* k, const void* v, const int32_t* tiles,
                                const star_causal_shape* s, void* o, float* lse, void* workspace, size_t workspace_bytes,
                                void* stream) {
     using namespace star;
     int rc = check_causal(s, "star_causal_fwd");
     if (rc) return rc;
     if (s->n_q_tiles == 0) return STAR_OK;
-    STAR_REQUIRE(q && k && v && seqs && tiles && o && lse, "star_causal_fwd: null pointer");
+    STAR_REQUIRE(q && k && v && tiles && o && lse, "star_causal_fwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "star_causal_fwd: tensors must be 16-byte aligned");
     const int64_t need = causal_fwd_bytes(s);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !aligned16(workspace))) {
         set_error("star_causal_fwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);
         return STAR_ERR_WORKSPACE;
     }
-    CAUSAL_BY_TYPE((launch_causal_fwd<T, HD>(q, k, v, seqs, tiles, s, o, lse, (float*)workspace, (hipStream_t)stream)));
+    CAUSAL_BY_TYPE((launch_causal_fwd<T, HD>(q, k, v, tiles, s, o, lse, (float*)workspace, (hipStream_t)stream)));
     if (rc) return rc;
     STAR_LAUNCH_CHECK("star_causal_fwd");
     return STAR_OK;
@@ -1011,14 +1007,14 @@ extern "C" size_t star_causal_bwd_workspace(const star_causal_shape* s) {
 }
 
 extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_,
-                               const float* lse, const int32_t* seqs, const int32_t* q_tiles, const int32_t* k_tiles,
+                               const float* lse, const int32_t* q_tiles, const int32_t* k_tiles,
                                const star_causal_shape* s, void* dq, void* dk, void* dv, float* delta, void* workspace,
                                size_t workspace_bytes, void* stream) {
     using namespace star;
     int rc = check_causal(s, "star_causal_bwd");
     if (rc) return rc;
     if (s->n_q_tiles == 0 && s->n_k_tiles == 0) return STAR_OK;
-    STAR_REQUIRE(q && k && v && o && do_ && lse && seqs && (q_tiles || !s->n_q_tiles) && (k_tiles || !s->n_k_tiles) && dq && dk && dv && delta,
+    STAR_REQUIRE(q && k && v && o && do_ && lse && (q_tiles || !s->n_q_tiles) && (k_tiles || !s->n_k_tiles) && dq && dk && dv && delta,
                  "star_causal_bwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(do_) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                  "star_causal_bwd: tensors must be 16-byte aligned");
@@ -1029,7 +1025,7 @@ extern "C" int star_causal_bwd(const void* q, const void* k, const void* v, cons
         set_error("star_causal_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);
         return STAR_ERR_WORKSPACE;
     }
-    CAUSAL_BY_TYPE((launch_causal_bwd<T, HD>(q, k, v, o, do_, lse, seqs, q_tiles, k_tiles, s, dq, dk, dv, delta, (float*)workspace,
+    CAUSAL_BY_TYPE((launch_causal_bwd<T, HD>(q, k, v, o, do_, lse, q_tiles, k_tiles, s, dq, dk, dv, delta, (float*)workspace,
                                              (hipStream_t)stream)));
     if (rc) return rc;
     STAR_LAUNCH_CHECK("star_causal_bwd");

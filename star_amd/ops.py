@@ -1662,17 +1662,25 @@ class PackedSeqs:
             per = -(-n // CAUSAL_TILE)
             seq = np.repeat(np.arange(n.size, dtype=np.int64), per)
             first = (np.arange(seq.size, dtype=np.int64) - np.repeat(np.cumsum(per) - per, per)) * CAUSAL_TILE
-            order = np.argsort(-work(seq, first), kind="stable")
-            return np.stack([seq[order], first[order]], 1)
+            # One sequence behind the other, so that the tiles that walk the same rows meet in the caches (all longest tiles
+            # first: 128 sequences of 512, 8 heads of 128, 176 us; so 158), its longest tile first, the longest sequence first; the
+            # shortest eighth of the work last of all, to fill the places that fall free at different times.
+            w = work(seq, first) + CAUSAL_TILE
+            by_work = np.argsort(-w, kind="stable")
+            late = np.zeros(seq.size, dtype=bool)
+            late[by_work] = np.cumsum(w[by_work][::-1])[::-1] * 8 <= w.sum()
+            order = np.lexsort((-w, seq, -np.where(late, 0, n[seq]), -np.where(late, w, 0), late))
+            seq, zero = seq[order], np.zeros(seq.size, dtype=np.int64)
+            return np.stack([q0[seq], nq[seq], k0[seq], nk[seq], first[order], zero, zero, zero], 1)
 
         qt = tiles(nq, lambda s, i: np.clip(np.minimum(i + CAUSAL_TILE, nq[s]) + nk[s] - nq[s], 0, nk[s]))
         kt = tiles(nk, lambda s, j: nq[s] - np.clip(j - (nk[s] - nq[s]), 0, nq[s]))
         seqs = np.stack([q0, nq, k0, nk], 1)
-        flat = np.concatenate([seqs.ravel(), qt.ravel(), kt.ravel()]).astype(np.int32)
+        flat = np.concatenate([qt.ravel(), kt.ravel(), seqs.ravel()]).astype(np.int32)
         buf = torch.from_numpy(flat).to(device)
         self.device = buf.device
-        a, b = seqs.size, seqs.size + qt.size
-        self.seqs, self.q_tiles, self.k_tiles = buf[:a].view(-1, 4), buf[a:b].view(-1, 2), buf[b:].view(-1, 2)
+        a, b = qt.size, qt.size + kt.size
+        self.q_tiles, self.k_tiles, self.seqs = buf[:a].view(-1, 8), buf[a:b].view(-1, 8), buf[b:].view(-1, 4)
         self.starts, self.counts = self.seqs[:, 2], self.seqs[:, 3]
         self.n_q_tiles, self.n_k_tiles = len(qt), len(kt)
 
@@ -1691,8 +1699,8 @@ def _causal_forward(q, k, v, plan, s):
     # (only launches of few workgroups over many keys are cut along the keys)
     need = lib().star_causal_fwd_workspace(s) if plan.max_k > 960 and plan.n_q_tiles * s.H < 256 else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-    _launch(lib().star_causal_fwd, "star_causal_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.seqs.data_ptr(),
-            plan.q_tiles.data_ptr(), s, o.data_ptr(), lse.data_ptr(), ptr(ws), need)
+    _launch(lib().star_causal_fwd, "star_causal_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.q_tiles.data_ptr(),
+            s, o.data_ptr(), lse.data_ptr(), ptr(ws), need)
     return o, lse
 
 
@@ -1707,8 +1715,7 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
     need = lib().star_causal_bwd_workspace(s) if s.H != s.Hkv else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     _launch(lib().star_causal_bwd, "star_causal_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            g.data_ptr(), lse.data_ptr(), plan.seqs.data_ptr(), plan.q_tiles.data_ptr(),
-            plan.k_tiles.data_ptr(), s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+            g.data_ptr(), lse.data_ptr(), plan.q_tiles.data_ptr(), plan.k_tiles.data_ptr(), s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
             ptr(ws), need)
 
 

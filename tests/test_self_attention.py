@@ -641,13 +641,18 @@ def test_packed_seqs_layout_and_refusals(ops):
     p = ops.PackedSeqs([130, 0, 5], "cpu", q_lengths=[3, 0, 200])
     assert p.seqs.tolist() == [[0, 3, 0, 130], [3, 0, 130, 0], [3, 200, 130, 5]]
     assert (p.q_rows, p.k_rows, p.q_used, p.k_used, p.max_q, p.max_k, p.n) == (203, 135, 203, 135, 200, 130, 3)
-    assert sorted(map(tuple, p.q_tiles.tolist())) == [(0, 0), (2, 0), (2, 128)]
-    assert p.q_tiles.tolist()[0] == [0, 0]                     # the longest walk starts first
-    assert sorted(map(tuple, p.k_tiles.tolist())) == [(0, 0), (0, 128), (2, 0)]
+    tiles = lambda t: sorted((p.seqs.tolist().index(w[:4]), w[4]) for w in t.tolist())  # noqa: E731
+    assert tiles(p.q_tiles) == [(0, 0), (2, 0), (2, 128)]
+    assert tiles(p.k_tiles) == [(0, 0), (0, 128), (2, 0)]
     p = ops.PackedSeqs([2, 7], "cpu", padded_to=7)
     assert p.seqs.tolist() == [[0, 2, 0, 2], [7, 7, 7, 7]] and (p.q_rows, p.q_used) == (14, 9)
+    p = ops.PackedSeqs([40, 2000, 2000, 500], "cpu")
+    assert tiles(p.q_tiles) == sorted((s, f) for s, n in enumerate([40, 2000, 2000, 500]) for f in range(0, n, 128))
+    order = [(p.seqs.tolist().index(w[:4]), w[4]) for w in p.q_tiles.tolist()]
+    assert order[0] == (1, 1920) and order[-1] == (0, 0)       # the longest walk starts first, the shortest last,
+    assert [f for s, f in order if s == 2 and f >= 1024] == list(range(1920, 1023, -128))   # each sequence from its end
     p = ops.PackedSeqs([], "cpu")
-    assert p.n == 0 and p.q_rows == 0 and p.q_tiles.shape == (0, 2)
+    assert p.n == 0 and p.q_rows == 0 and p.q_tiles.shape == (0, 8)
     assert p.starts.numel() == 0
     with pytest.raises(ValueError, match="negative"):
         ops.PackedSeqs([3, -1], "cpu")
@@ -671,8 +676,8 @@ def test_the_library_checks_sizes_before_any_launch():
     from star_amd import _lib
     L = _lib.lib()
     S = _lib.CausalShape
-    fwd = lambda s, k=16, ws=None, n=0: L.star_causal_fwd(16, k, 16, 16, 16, s, 16, 16, ws, n, None)  # noqa: E731
-    bwd = lambda s, ws=None, n=0: L.star_causal_bwd(*[16] * 9, s, 16, 16, 16, 16, ws, n, None)  # noqa: E731
+    fwd = lambda s, k=16, ws=None, n=0: L.star_causal_fwd(16, k, 16, 16, s, 16, 16, ws, n, None)  # noqa: E731
+    bwd = lambda s, ws=None, n=0: L.star_causal_bwd(*[16] * 8, s, 16, 16, 16, 16, ws, n, None)  # noqa: E731
     for kw, text in [(dict(hd=80), b"head dim 80"), (dict(Hkv=3), b"divide"), (dict(dtype=1), b"dtype"), (dict(q_sr=4), b"multiples of 8"),
                      (dict(q_sr=1 << 23), b"row stride"), (dict(q_sr=-8), b"row stride"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"),
                      (dict(scale=math.inf), b"scale"), (dict(scale=math.nan), b"scale"), (dict(max_k=-1), b"negative"),
@@ -684,7 +689,7 @@ def test_the_library_checks_sizes_before_any_launch():
     s = S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1)
     assert fwd(s, k=24) == -1 and b"aligned" in L.star_last_error()
     assert fwd(s, k=None) == -1 and b"null pointer" in L.star_last_error()
-    assert L.star_causal_fwd(None, None, None, None, None, S(H=4, Hkv=2, hd=64, dtype=0, scale=1), None, None, None, 0, None) == 0
+    assert L.star_causal_fwd(None, None, None, None, S(H=4, Hkv=2, hd=64, dtype=0, scale=1), None, None, None, 0, None) == 0
     # cut along the keys: few query tiles, many keys
     need = lambda nq, n, nk: L.star_causal_fwd_workspace(S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=n, max_q=nq, max_k=nk))  # noqa: E731
     assert need(16, 1, 960) == 0 and need(16, 1, 1024) == 4 * 2 * 16 * 66 * 4 and need(16, 64, 100000) == 0
