@@ -461,7 +461,7 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
  *        they are to start: the sequence's first query row, queries nq, first key row and keys nk, the tile's first query,
  *        and three unused words.  Query i of a sequence sees its keys j <= i + nk - nq (the queries are the newest nq
  *        positions); a query that sees no key gets o = 0, lse = -inf.  Rows in no sequence are not touched
- *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward
+ *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward (NULL: not wanted)
  * Softmax statistics and sums are fp32; the weights P are rounded to dtype for the product with V (as the inputs are).
  * Nothing is masked by arithmetic on values: a key after the query never enters its maximum, sum or output, with one
  * exception: V rows of the SAME sequence behind the query but inside its 64-key tile meet a weight of exactly 0, so an

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
             for (int e = 0; e < 4; ++e) o4[e] = (T)(oacc[qb][nt][e] * inv);
             *(x4*)(orow + 16 * nt) = o4;
         }
-        if (g == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = sum == 0.f ? -INFINITY : m[qb] * A_LN2 + logf(sum);
+        if (g == 0 && lse) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = sum == 0.f ? -INFINITY : m[qb] * A_LN2 + logf(sum);
     }
 }
 
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
         T* orow = O + (int64_t)(sq.q0 + row) * s.o_sr + (int64_t)h * s.o_sh + d0;
 #pragma unroll
         for (int e = 0; e < PER; ++e) orow[e] = (T)(o[e] * inv);
-        if ((tid & 15) == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + row] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
+        if ((tid & 15) == 0 && lse) lse[(int64_t)h * s.lse_stride + sq.q0 + row] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
     }
 }
 
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void causal_join_kernel(const int32_t* __restr
     T* orow = O + (int64_t)(sq.q0 + i) * s.o_sr + (int64_t)h * s.o_sh;
     orow[lane] = (T)(o0 * inv);
     if (lane + 64 < HD) orow[lane + 64] = (T)(o1 * inv);
-    if (lane == 0) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
+    if (lane == 0 && lse) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
 }
 
 // ------------------------------------------------------------------------------------------------------ gradient of Q
@@ -988,7 +988,7 @@ extern "C" int star_causal_fwd(const void* q, const void* k, const void* v, cons
     int rc = check_causal(s, "star_causal_fwd");
     if (rc) return rc;
     if (s->n_q_tiles == 0) return STAR_OK;
-    STAR_REQUIRE(q && k && v && tiles && o && lse, "star_causal_fwd: null pointer");
+    STAR_REQUIRE(q && k && v && tiles && o, "star_causal_fwd: null pointer");
     STAR_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "star_causal_fwd: tensors must be 16-byte aligned");
     const int64_t need = causal_fwd_bytes(s);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !aligned16(workspace))) {

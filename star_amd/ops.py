@@ -1565,16 +1565,18 @@ def xattn(q, k, v, bias=None, key_len=None, ilk_diag: int = -1, scale: Optional[
 DT_F16 = 2
 _DT16 = {torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 CAUSAL_TILE = 128                 # STAR_CAUSAL_TILE
+_HEAD_DIMS = (64, 96, 128)
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
-    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+# (the C functions behind torch.cuda.current_stream() / current_device(), which take some 3 us of a call's 10)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(fn, what, dev, *args):
     """fn(*args, the current stream of dev), with dev as the current device for the launch."""
     index = dev.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -1600,21 +1602,21 @@ def _same_device(what, **ts):
 def _row_strides(what, name, t):
     """The strides of a [.., hd] operand but for hd's, after checking what the kernels' 16-byte loads need of it.  That
     of a dimension of size 1, which is never used and may be anything, is given as 0."""
+    shape, strides = t.shape, t.stride()
     if t.dtype not in _DT16:
         raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16 or float16 is required")
-    *shape, hd = t.shape
-    *strides, one = t.stride()
-    if hd not in (64, 96, 128):
-        raise ValueError(f"{what}: head dim {hd} not in (64, 96, 128)")
-    if one != 1 and t.numel():
+    if shape[-1] not in _HEAD_DIMS:
+        raise ValueError(f"{what}: head dim {shape[-1]} not in {_HEAD_DIMS}")
+    if strides[-1] != 1 and t.numel():
         raise ValueError(f"{what}: {name} must have a contiguous head dimension")
-    strides = [st if n > 1 else 0 for st, n in zip(strides, shape)]
-    bits = t.data_ptr()
-    for st in strides:
-        bits |= st * 2
-    if bits & 15:
+    bits = t.data_ptr() >> 1
+    if 1 in shape:
+        strides = tuple(st if n > 1 else 0 for st, n in zip(strides, shape))
+    for st in strides[:-1]:
+        bits |= st
+    if bits & 7:
         raise ValueError(f"{what}: {name} must be 16-byte aligned in every row")
-    return strides
+    return strides[:-1]
 
 
 class PackedSeqs:
@@ -1683,6 +1685,8 @@ class PackedSeqs:
         self.q_tiles, self.k_tiles, self.seqs = buf[:a].view(-1, 8), buf[a:b].view(-1, 8), buf[b:].view(-1, 4)
         self.starts, self.counts = self.seqs[:, 2], self.seqs[:, 3]
         self.n_q_tiles, self.n_k_tiles = len(qt), len(kt)
+        self.q_tiles_ptr, self.k_tiles_ptr = self.q_tiles.data_ptr(), self.k_tiles.data_ptr()
+        self.starts_ptr, self.counts_ptr = self.starts.data_ptr(), self.counts.data_ptr()
 
 
 def _rows_like(rows, used, heads, hd, t):
@@ -1691,16 +1695,19 @@ def _rows_like(rows, used, heads, hd, t):
     return make((rows, heads, hd), dtype=t.dtype, device=t.device)
 
 
-def _causal_forward(q, k, v, plan, s):
-    o = _rows_like(s.lse_stride, plan.q_used, s.H, s.hd, q)
-    lse = torch.empty((s.H, s.lse_stride), dtype=torch.float32, device=q.device)
-    if plan.q_used != s.lse_stride:
-        lse.fill_(-math.inf)
+def _causal_forward(q, k, v, plan, s, want_lse):
+    rows, dev = s.lse_stride, q.device
+    o = _rows_like(rows, plan.q_used, s.H, s.hd, q)
+    lse = None
+    if want_lse:
+        lse = torch.empty((s.H, rows), dtype=torch.float32, device=dev)
+        if plan.q_used != rows:
+            lse.fill_(-math.inf)
     # (only launches of few workgroups over many keys are cut along the keys)
     need = lib().star_causal_fwd_workspace(s) if plan.max_k > 960 and plan.n_q_tiles * s.H < 256 else 0
-    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-    _launch(lib().star_causal_fwd, "star_causal_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.q_tiles.data_ptr(),
-            s, o.data_ptr(), lse.data_ptr(), ptr(ws), need)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _launch(lib().star_causal_fwd, "star_causal_fwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.q_tiles_ptr, s,
+            o.data_ptr(), ptr(lse), ptr(ws), need)
     return o, lse
 
 
@@ -1715,7 +1722,7 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
     need = lib().star_causal_bwd_workspace(s) if s.H != s.Hkv else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     _launch(lib().star_causal_bwd, "star_causal_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            g.data_ptr(), lse.data_ptr(), plan.q_tiles.data_ptr(), plan.k_tiles.data_ptr(), s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+            g.data_ptr(), lse.data_ptr(), plan.q_tiles_ptr, plan.k_tiles_ptr, s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
             ptr(ws), need)
 
 
@@ -1724,7 +1731,7 @@ class _CausalAttn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, plan, s, need_lse):
-        o, lse = _causal_forward(q, k, v, plan, s)
+        o, lse = _causal_forward(q, k, v, plan, s, True)
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.plan, ctx.s = plan, s
         if not need_lse:
@@ -1749,7 +1756,7 @@ class _CausalAttnQKV(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, views, plan, s):
-        o, lse = _causal_forward(*views, plan, s)
+        o, lse = _causal_forward(*views, plan, s, True)
         ctx.save_for_backward(qkv, o, lse)
         ctx.plan, ctx.s = plan, s
         return o
@@ -1782,7 +1789,7 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     s = _causal_shape(q, k, v, plan, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CausalAttn.apply(q, k, v, plan, s, need_lse)
-    o, lse = _causal_forward(q, k, v, plan, s)
+    o, lse = _causal_forward(q, k, v, plan, s, need_lse)
     return (o, lse) if need_lse else o
 
 
@@ -1798,37 +1805,33 @@ def causal_attn_qkv(qkv, n_heads: int, kv_heads: int, plan: PackedSeqs, scale: O
     s = _causal_shape(*views, plan, scale)
     if torch.is_grad_enabled() and qkv.requires_grad:
         return _CausalAttnQKV.apply(qkv, views, plan, s)
-    return _causal_forward(*views, plan, s)[0]
+    return _causal_forward(*views, plan, s, False)[0]
 
 
 def _causal_shape(q, k, v, plan, scale):
-    dev = _same_device("causal_attn", q=q, k=k, v=v)
+    dev = q.device
+    if not (k.device == dev == v.device == plan.device and q.is_cuda):
+        dev = _same_device("causal_attn", q=q, k=k, v=v)
+        raise ValueError(f"causal_attn: the plan is on {plan.device}, the tensors on {dev}")
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"causal_attn: [rows, heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     rows, H, hd = q.shape
-    k_rows, Hkv, _ = k.shape
-    if k.shape != v.shape or hd != k.shape[2]:
+    k_rows, Hkv, k_hd = k.shape
+    if k.shape != v.shape or hd != k_hd:
         raise ValueError(f"causal_attn: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
-    if not q.dtype == k.dtype == v.dtype:
+    dtype = q.dtype
+    if not dtype == k.dtype == v.dtype:
         raise TypeError(f"causal_attn: q, k and v must share one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     if Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError(f"causal_attn: {H} query heads do not divide into {Hkv} key heads")
     scale = hd ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"causal_attn: scale = {scale}; a positive number is required")
-    if plan.device != dev:
-        raise ValueError(f"causal_attn: the plan is on {plan.device}, the tensors on {dev}")
     if rows < plan.q_rows or k_rows < plan.k_rows:
         raise ValueError(f"causal_attn: the plan needs {plan.q_rows} query and {plan.k_rows} key rows, got {rows} and {k_rows}")
-    s = CausalShape()
-    s.q_sr, s.q_sh = _row_strides("causal_attn", "q", q)
-    s.k_sr, s.k_sh = _row_strides("causal_attn", "k", k)
-    s.v_sr, s.v_sh = _row_strides("causal_attn", "v", v)
-    s.o_sr, s.o_sh = H * hd, hd
-    s.H, s.Hkv, s.hd, s.dtype, s.max_q, s.max_k = H, Hkv, hd, _DT16[q.dtype], plan.max_q, plan.max_k
-    s.n_q_tiles, s.n_k_tiles = plan.n_q_tiles, plan.n_k_tiles
-    s.lse_stride, s.k_rows, s.scale = rows, k_rows, scale
-    return s
+    return CausalShape(H, Hkv, hd, _DT16.get(dtype, -1), plan.max_q, plan.max_k, plan.n_q_tiles, plan.n_k_tiles,
+                       *_row_strides("causal_attn", "q", q), *_row_strides("causal_attn", "k", k),
+                       *_row_strides("causal_attn", "v", v), H * hd, hd, rows, k_rows, 0, 0, scale)
 
 
 # ----------------------------------------------------------------------------- 8-bit key/value cache
@@ -1923,11 +1926,14 @@ class KVCache8:
         return torch.where(live, k, 0.0), torch.where(live, v, 0.0)
 
 
-def _i32(what, t, n):
-    if t is None:
-        return None
+def _i32(what, t, n, dev):
+    if t.device != dev:
+        _need_cuda(t)
+        raise ValueError(f"{what} is on {t.device}, the cache on {dev}")
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what} must be [{n}], got {tuple(t.shape)}")
+    if t.dtype == torch.int32 and t.is_contiguous():
+        return t
     if t.is_floating_point():
         raise TypeError(f"{what} must hold integers, got {t.dtype}")
     return t.to(torch.int32).contiguous()
@@ -1941,37 +1947,42 @@ def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = 
     keys that the plan gives each sequence.  at [batch] (device integers): write at these positions instead of behind
     the last token -- 0 fills anew, a position in the incomplete block takes tokens back; other positions, whose block is
     complete, must not be given.  Nothing is differentiated through a cache.  One launch, no host sync."""
-    dev = _same_device("kv8_append", k=k, v=v, counts=counts, at=at, cache=cache.lens)
-    B, H, hd = cache.batch, cache.kv_heads, cache.head_dim
+    dev, B, H, hd = cache.device, cache.batch, cache.kv_heads, cache.head_dim
+    if not (k.device == v.device == dev):
+        _same_device("kv8_append", k=k, v=v, cache=cache.lens)
     if k.shape != v.shape:
         raise ValueError(f"kv8_append: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise TypeError(f"kv8_append: the cache takes {cache.dtype}, got {k.dtype} and {v.dtype}")
+    st = (0,) * 6
     if plan is None:
-        if k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (B, H, hd):
+        if k.dim() != 4 or k.shape[0] != B or k.shape[1] != H or k.shape[3] != hd:
             raise ValueError(f"kv8_append: [{B}, {H}, n, {hd}] expected, got {tuple(k.shape)}")
-        counts, starts, step, most = _i32("kv8_append: counts", counts, B), None, 1, k.shape[2]
-        if k.numel():
+        most = k.shape[2]
+        if most:
             st = _row_strides("kv8_append", "k", k) + _row_strides("kv8_append", "v", v)
+        if counts is not None:
+            counts = _i32("kv8_append: counts", counts, B, dev)
+        starts_ptr, counts_ptr, step = None, ptr(counts), 1
     else:
         if counts is not None:
             raise ValueError("kv8_append: counts go with a batch, a plan has its own")
-        if k.dim() != 3 or (k.shape[1], k.shape[2]) != (H, hd):
+        if k.dim() != 3 or k.shape[1] != H or k.shape[2] != hd:
             raise ValueError(f"kv8_append: [rows, {H}, {hd}] expected, got {tuple(k.shape)}")
         if plan.n != B or plan.device != dev:
             raise ValueError(f"kv8_append: a plan of {plan.n} sequences on {plan.device} for a cache of {B} on {dev}")
         if k.shape[0] < plan.k_rows:
             raise ValueError(f"kv8_append: the plan needs {plan.k_rows} rows, got {k.shape[0]}")
-        counts, starts, step, most = plan.counts, plan.starts, 4, plan.max_k
-        if k.numel():
+        most = plan.max_k
+        if most:
             (kr, kh), (vr, vh) = _row_strides("kv8_append", "k", k), _row_strides("kv8_append", "v", v)
             st = 0, kh, kr, 0, vh, vr
-    if most == 0 and at is None:
+        starts_ptr, counts_ptr, step = plan.starts_ptr, plan.counts_ptr, 4
+    if at is not None:
+        at = _i32("kv8_append: at", at, B, dev)
+    elif most == 0:
         return
-    if not k.numel():
-        st = (0,) * 6
-    at = _i32("kv8_append: at", at, B)
-    _launch(lib().star_kv8_append, "star_kv8_append", dev, cache._c, k.data_ptr(), v.data_ptr(), *st, ptr(starts), ptr(counts),
+    _launch(lib().star_kv8_append, "star_kv8_append", dev, cache._c, k.data_ptr(), v.data_ptr(), *st, starts_ptr, counts_ptr,
             step, ptr(at), most)
 
 
@@ -1986,8 +1997,9 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
     The values that the cache stands for are used as they are; softmax and sums are fp32, the softmax weights are rounded
     to 16 bits for the product with v.  An infinite or NaN v of a token reaches every query of the sequence that sees a
     token of its block."""
-    dev = _same_device("kv8_attn", q=q, q_len=q_len, bias=bias, cache=cache.lens)
-    B, hd = cache.batch, cache.head_dim
+    dev, B, hd = cache.device, cache.batch, cache.head_dim
+    if q.device != dev or (bias is not None and bias.device != dev):
+        _same_device("kv8_attn", q=q, bias=bias, cache=cache.lens)
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
         raise ValueError(f"kv8_attn: [{B}, a multiple of {cache.kv_heads}, L, {hd}] expected, got {tuple(q.shape)}")
     if q.dtype != cache.dtype:
@@ -1995,19 +2007,21 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
     if torch.is_grad_enabled() and (q.requires_grad or (bias is not None and bias.requires_grad)):
         raise _lib.StarNuggetError("kv8_attn has no backward: call it under torch.no_grad()")
     H, L = q.shape[1], q.shape[2]
+    n_bias = 0
     if bias is not None:
         if bias.dim() != 2 or bias.shape[0] != B or bias.shape[1] > cache.capacity:
             raise ValueError(f"kv8_attn: bias [{B}, at most {cache.capacity}] expected, got {tuple(bias.shape)}")
-        bias = bias.detach().to(torch.float32).contiguous()
-    o = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev).permute(0, 2, 1, 3)
+        n_bias = bias.shape[1]
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().to(torch.float32).contiguous()
+    if q_len is not None:
+        q_len = _i32("kv8_attn: q_len", q_len, B, dev)
+    o_st = L * H * hd, hd, H * hd
+    o = torch.empty_strided((B, H, L, hd), (*o_st, 1), dtype=q.dtype, device=dev)
     if L == 0:
         return o
-    s = KV8Query()
-    s.q_sb, s.q_sh, s.q_sr = _row_strides("kv8_attn", "q", q)
-    s.H, s.L, s.o_sb, s.o_sh, s.o_sr = H, L, L * H * hd, hd, H * hd
-    s.bias_len = 0 if bias is None else bias.shape[1]
-    s.causal, s.ilk_diag, s.scale = int(bool(causal)), int(ilk_diag), hd ** -0.5 if scale is None else float(scale)
-    q_len = _i32("kv8_attn: q_len", q_len, B)
+    s = KV8Query(H, L, *_row_strides("kv8_attn", "q", q), *o_st, n_bias, 1 if causal else 0, int(ilk_diag),
+                 hd ** -0.5 if scale is None else float(scale))
     need = cache._workspace.get((H, L))
     if need is None:
         need = cache._workspace[H, L] = lib().star_kv8_attn_workspace(cache._c, H, L)
