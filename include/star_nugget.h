@@ -464,8 +464,8 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
  *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward (NULL: not wanted)
  * Softmax statistics and sums are fp32; the weights P are rounded to dtype for the product with V (as the inputs are).
  * Nothing is masked by arithmetic on values: a key after the query never enters its maximum, sum or output, with one
- * exception: V rows of the SAME sequence behind the query but inside its 64-key tile meet a weight of exactly 0, so an
- * infinite or NaN V reaches up to 63 earlier queries of its own sequence. */
+ * exception: V rows of the SAME sequence behind the query but inside a 64-key tile that another query of its 32 sees meet a
+ * weight of exactly 0, so an infinite or NaN V reaches up to 94 earlier queries of its own sequence. */
 #define STAR_DT_F16 2
 #define STAR_CAUSAL_TILE 128
 typedef struct {
@@ -503,7 +503,7 @@ int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, 
  *   v_codes [B][Hkv][T/64][hd][64], v_scales [B][Hkv][T/64]  v_tail [B][Hkv][hd][64]  (V is transposed inside a block)
  *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written);
  *   tickets [B * (1 + 2 * Hkv) * STAR_KV8_TICKET_STRIDE]: zero before the first call, zero after every call.  All base addresses multiples of 16 bytes.
- * Calls on one cache are ordered by the stream: two appends, or an append and an attention, must not overlap. */
+ * An append must not overlap any other call on the cache (the stream orders them); attentions alone may. */
 #define STAR_KV8_BLOCK 64
 #define STAR_KV8_TICKET_STRIDE 32
 typedef struct {
@@ -522,8 +522,9 @@ typedef struct {
 /* Append rows of k, v (dtype; element strides per sequence, head, row, multiples of 8; hd contiguous; 16-byte aligned).
  *   starts, counts (either may be NULL): sequence b gives the rows starts[b * idx_stride] .. + counts[b * idx_stride] of
  *       k + b * k_sb; NULL starts: from row 0; NULL counts: max_rows rows.  counts are clamped to [0, max_rows]
- *   at [B] or NULL: the position of the first of them, in place of lens[b].  Only positions at or behind the first token
- *       of the open block can be written again.  lens[b] becomes at + count, clipped to T */
+ *   at [B] or NULL: the position of the first of them, in place of lens[b]; lens[b] becomes at + count, clipped to T.  The
+ *       tokens in front of `at` in its block are taken from k_tail / v_tail, where those of the open block lie (and still
+ *       lie after the call that completed it, if that call wrote no token behind it) */
 int star_kv8_append(const star_kv8_cache* c, const void* k, const void* v, int64_t k_sb, int64_t k_sh, int64_t k_sr,
                     int64_t v_sb, int64_t v_sh, int64_t v_sr, const int32_t* starts, const int32_t* counts,
                     int idx_stride, const int32_t* at, int max_rows, void* stream);

@@ -874,7 +874,8 @@ static int check_causal(const star_causal_shape* s, const char* who) {
     STAR_REQUIRE(s->Hkv >= 1 && s->H >= s->Hkv && s->H % s->Hkv == 0, "%s: %d query heads do not divide into %d key heads", who, s->H, s->Hkv);
     STAR_REQUIRE(s->max_q >= 0 && s->max_k >= 0 && s->n_q_tiles >= 0 && s->n_k_tiles >= 0 && s->lse_stride >= 0 && s->k_rows >= 0,
                  "%s: negative size", who);
-    STAR_REQUIRE((int64_t)s->n_q_tiles * s->H < (1ll << 31) && (int64_t)s->n_k_tiles * s->H < (1ll << 31), "%s: %d and %d tiles x %d heads",
+    // (a launch has less than 2^32 threads in x)
+    STAR_REQUIRE((int64_t)s->n_q_tiles * s->H < (1ll << 24) && (int64_t)s->n_k_tiles * s->H < (1ll << 24), "%s: %d and %d tiles x %d heads",
                  who, s->n_q_tiles, s->n_k_tiles, s->H);
     const int64_t st[8] = {s->q_sr, s->q_sh, s->k_sr, s->k_sh, s->v_sr, s->v_sh, s->o_sr, s->o_sh};
     for (int i = 0; i < 8; ++i) STAR_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);

@@ -723,7 +723,7 @@ extern "C" int star_kv8_append(const star_kv8_cache* c, const void* k, const voi
 
 extern "C" size_t star_kv8_attn_workspace(const star_kv8_cache* c, int H, int L) {
     using namespace star;
-    if (check_cache(c, "star_kv8_attn_workspace") || H < c->Hkv || H % c->Hkv || L < 1) return 0;
+    if (check_cache(c, "star_kv8_attn_workspace") || H < c->Hkv || H % c->Hkv || L < 1 || (int64_t)H * L >= (1ll << 24)) return 0;
     const int slots = attn_slots(c, H, L);
     return slots == c->B ? 0 : (size_t)slots * H * L * (c->hd + 2) * sizeof(float);
 }
@@ -739,10 +739,11 @@ extern "C" int star_kv8_attn(const star_kv8_cache* c, const void* q, const float
     STAR_REQUIRE((((uintptr_t)q | (uintptr_t)o) & 15) == 0, "star_kv8_attn: q and o must be 16-byte aligned");
     const int64_t sd[6] = {s->q_sb, s->q_sh, s->q_sr, s->o_sb, s->o_sh, s->o_sr};
     for (int i = 0; i < 6; ++i) STAR_REQUIRE(sd[i] % 8 == 0, "star_kv8_attn: strides must be multiples of 8 elements");
+    // (a launch has less than 2^32 threads in x)
+    STAR_REQUIRE((int64_t)c->B * s->H * s->L < (1ll << 24), "star_kv8_attn: %d sequences x %d heads x %d queries", c->B, s->H, s->L);
     const int rows = s->H / c->Hkv * s->L, rt = row_tiles(rows);
     AttnArgs a{*c, *s, q, o, s->bias_len > 0 ? bias : nullptr, q_len, attn_slots(c, s->H, s->L), cdiv(rows, 16 * rt), (float*)workspace};
-    STAR_REQUIRE((int64_t)s->H * s->L < (1ll << 24) && (int64_t)a.slots * c->Hkv * a.nrg < (1ll << 31) && (int64_t)c->B * s->H * s->L < (1ll << 31),
-                 "star_kv8_attn: %d sequences x %d heads x %d queries", c->B, s->H, s->L);
+    STAR_REQUIRE((int64_t)a.slots * c->Hkv * a.nrg < (1ll << 24), "star_kv8_attn: %d parts x %d heads x %d groups of rows", a.slots, c->Hkv, a.nrg);
     STAR_REQUIRE(!(s->bias_len > 0 && !bias), "star_kv8_attn: bias_len > 0 but bias is null");
     if (workspace_bytes < star_kv8_attn_workspace(c, s->H, s->L) || (a.slots > c->B && !workspace)) {
         set_error("star_kv8_attn: workspace of %zu bytes, %zu needed", workspace_bytes, star_kv8_attn_workspace(c, s->H, s->L));

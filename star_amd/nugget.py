@@ -13,7 +13,7 @@ The reference has no plugin interface; its boundary is these Python signatures:
   semantic_repr[arange(B)[:,None], nugget_indices]         gather_nuggets              (w2v_asr.py:566-567)
   MyGPT2Attention._attn (my_transformer.py:535)            score_biased_attn / NuggetCrossAttention._attn
   MyGPT2Attention.forward, cross branch (:490-533)         NuggetCrossAttention.forward
-  MyGPT2Attention.forward, self branch (:511-533)          NuggetSelfAttention.forward (causal, lengths for masks)
+  MyGPT2Attention.forward, self branch (:490-533)          NuggetSelfAttention.forward (causal, lengths for masks)
 
 A maintainer of the reference makes `W2VASRModel` / `W2VSimulModel` inherit `NuggetOpsMixin` (first in
 the MRO), builds `self.nugget_model = NuggetScorer(hidden_size)` and uses `NuggetCrossAttention` for
@@ -500,13 +500,14 @@ class NuggetCrossAttention(nn.Module):
 
 
 class NuggetSelfAttention(nn.Module):
-    """Self-attention branch of MyGPT2Attention.forward (my_transformer.py:511-533), causal: the attention of the
+    """Self-attention branch of MyGPT2Attention.forward (my_transformer.py:490-533), causal: the attention of the
     semantic encoder over the frames and of the decoder over its own tokens.  Parameters c_attn and c_proj (Conv1D
     layout) as in GPT2Attention; kv_heads < num_heads (not in the reference) shares every key head between
     num_heads // kv_heads query heads, c_attn is then [hidden, (num_heads + 2 kv_heads) * head_dim].
 
     The core runs on 16-bit operands with fp32 softmax and sums, as NuggetCrossAttention's does: fp32 activations are
     rounded to bfloat16 for it.  The softmax is never padded, so no additive attention_mask is taken: give the lengths.
+    The plan of an unpadded or padded batch is made at its first call: make that before a HIP-graph capture.
 
         attn(x)                                  x [B,T,d], every row T frames
         attn(x, valid=frames)                    x [B,T,d] padded, frames an ops.ValidFrames; pad rows see nothing

@@ -1627,8 +1627,8 @@ class PackedSeqs:
     lengths: keys of every sequence.  q_lengths: its queries where there are fewer (they are the newest positions: query
     i sees the keys j <= i + lengths[s] - q_lengths[s]); more queries than keys are allowed, the first then see nothing.
     Sequences lie one behind the other; with padded_to=T sequence s starts at row s * T instead (a padded [B,T] batch,
-    flattened), for the queries too; k_starts gives the first key row of every sequence (for kv8_append: rows of two
-    sequences may be the same there, but causal_attn's gradients need them apart)."""
+    flattened), for the queries too; k_starts gives the first key row of every sequence instead (two sequences may then
+    have rows in common, such as the same prompt; causal_attn refuses the gradients of such rows)."""
 
     def __init__(self, lengths: Sequence[int], device, q_lengths: Optional[Sequence[int]] = None,
                  padded_to: Optional[int] = None, k_starts: Optional[Sequence[int]] = None):
@@ -1651,13 +1651,16 @@ class PackedSeqs:
             k0 = np.asarray(list(k_starts), dtype=np.int64).reshape(-1)
             if k0.size != nk.size or (k0.size and k0.min() < 0):
                 raise ValueError(f"PackedSeqs: {k0.size} key starts, none negative, for {nk.size} sequences expected")
+        some = np.flatnonzero(nk)
+        some = some[np.argsort(k0[some], kind="stable")]
+        self.apart = bool((k0[some][1:] >= (k0 + nk)[some][:-1]).all())      # no key row in two sequences
         # rows that tensors have to have, and rows that belong to a sequence
         self.q_rows = int((q0 + nq).max()) if nk.size else 0
         self.k_rows = int((k0 + nk).max()) if nk.size else 0
         self.q_used, self.k_used = int(nq.sum()), int(nk.sum())
         if max(self.q_rows, self.k_rows) >= 2 ** 31:
             raise ValueError("PackedSeqs: more than 2^31 - 1 rows")
-        self.square = bool((nq == nk).all())
+        self.square = bool((nq == nk).all()) and k_starts is None            # one projection holds q, k and v
         self.n, self.max_q, self.max_k = int(nk.size), int(nq.max(initial=0)), int(nk.max(initial=0))
 
         def tiles(n, work):
@@ -1784,10 +1787,14 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     Returns o [rows,H,hd]; with need_lse also the natural log-sum-exp of every row's logits, fp32 [H,rows] (not
     differentiable).  A query that sees no key gives 0 and -inf, and rows in no sequence give 0 and -inf and have zero
     gradients.  Sums and softmax statistics are fp32; the softmax weights are rounded to the inputs' type for the
-    product with v, and their gradient for the products with q and k.  An infinite or NaN v row reaches up to 63 earlier
-    queries of its own sequence (they share a tile); k and v rows of other sequences or in no sequence reach nobody."""
+    product with v, and their gradient for the products with q and k (in float16 a gradient of a logit beyond 65504 becomes
+    infinite).  An infinite or NaN v row reaches up to 94 earlier queries of its own sequence, which share a tile with it;
+    so do k rows in the gradient of q, and rows of q and of o's gradient reach later keys' gradients.  Rows of other
+    sequences or in no sequence reach nobody."""
     s = _causal_shape(q, k, v, plan, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if not plan.apart:
+            raise ValueError("causal_attn: no gradients for a plan whose sequences have key rows in common")
         return _CausalAttn.apply(q, k, v, plan, s, need_lse)
     o, lse = _causal_forward(q, k, v, plan, s, need_lse)
     return (o, lse) if need_lse else o
@@ -1795,7 +1802,7 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
 
 def causal_attn_qkv(qkv, n_heads: int, kv_heads: int, plan: PackedSeqs, scale: Optional[float] = None):
     """causal_attn on one projection qkv [rows, (n_heads + 2 kv_heads) hd], queries, keys and values side by side (GPT-2's
-    c_attn, my_transformer.py:512): returns o [rows, n_heads, hd].  The gradients of the three parts are written straight
+    c_attn): returns o [rows, n_heads, hd].  The gradients of the three parts are written straight
     into one matrix of qkv's shape."""
     if qkv.dim() != 2 or n_heads < 1 or kv_heads < 1 or qkv.shape[1] % (n_heads + 2 * kv_heads):
         raise ValueError(f"causal_attn_qkv: [rows, ({n_heads} + 2 * {kv_heads}) * hd] expected, got {tuple(qkv.shape)}")
@@ -1844,7 +1851,8 @@ class KVCache8:
     does not depend on how the tokens were split into calls).  kv8_append fills it, kv8_attn reads it.
 
     lens [batch] int32 lives on the device and counts the tokens held; tokens that find no room are dropped and counted
-    (`overflow()`).  Calls on one cache must be ordered on one stream.  Captured calls replay on the cache as it then is."""
+    (`overflow()`).  An append must be ordered with every other call on the cache (by one stream, or events); reads alone may
+    overlap.  Captured calls replay on the cache as it then is."""
 
     _PARTS = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "lens")
 
@@ -1945,8 +1953,10 @@ def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = 
     k, v [batch, kv_heads, n, hd] (any strides with hd contiguous): n new tokens of every sequence, or the first
     counts[b] of them (device integers).  Or, with a plan of `batch` sequences, packed rows [rows, kv_heads, hd]: the
     keys that the plan gives each sequence.  at [batch] (device integers): write at these positions instead of behind
-    the last token -- 0 fills anew, a position in the incomplete block takes tokens back; other positions, whose block is
-    complete, must not be given.  Nothing is differentiated through a cache.  One launch, no host sync."""
+    the last token, which is then the last one written -- 0 (or a multiple of 64) fills anew from there, a position in the
+    incomplete block takes tokens back, and the position of the last append repeats it if that wrote no token behind the
+    block it began in.  At any other position the tokens in front of it in its block are lost: do not give one.
+    Nothing is differentiated through a cache.  One launch, no host sync."""
     dev, B, H, hd = cache.device, cache.batch, cache.kv_heads, cache.head_dim
     if not (k.device == v.device == dev):
         _same_device("kv8_append", k=k, v=v, cache=cache.lens)
@@ -1995,8 +2005,8 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
     is added to the logits of token j < n.  scale defaults to hd ** -0.5.  A query that sees nothing gives 0.
     Returns [batch, H, L, hd] (memory order [batch, L, H, hd], as xattn).  Inference only: call it under no_grad.
     The values that the cache stands for are used as they are; softmax and sums are fp32, the softmax weights are rounded
-    to 16 bits for the product with v.  An infinite or NaN v of a token reaches every query of the sequence that sees a
-    token of its block."""
+    to 16 bits for the product with v.  An infinite or NaN v of a token reaches every query of its sequence in the call as
+    soon as one of them sees a token of its block."""
     dev, B, hd = cache.device, cache.batch, cache.head_dim
     if q.device != dev or (bias is not None and bias.device != dev):
         _same_device("kv8_attn", q=q, bias=bias, cache=cache.lens)

@@ -171,6 +171,14 @@ def test_causal_attn_qkv_equals_causal_attn_with_its_gradients_side_by_side(ops)
             ops.causal_attn_qkv(bad, H, Hkv, plan)
     with pytest.raises(ValueError, match="as many queries"):
         ops.causal_attn_qkv(qkv, H, Hkv, ops.PackedSeqs([3, 5], DEV, q_lengths=[5, 3]))
+    # two sequences on the same key rows: forward only
+    both = ops.PackedSeqs([100, 60], DEV, q_lengths=[10, 20], k_starts=[0, 40])
+    with torch.no_grad():
+        o = ops.causal_attn(q[:30], k, v, both)
+        apart = ops.causal_attn(q[:30], torch.cat([k[:100], k[40:100]]), torch.cat([v[:100], v[40:100]]), ops.PackedSeqs([100, 60], DEV, q_lengths=[10, 20]))
+    assert torch.equal(o, apart)
+    with pytest.raises(ValueError, match="in common"):
+        ops.causal_attn(q[:30], k, v, both)
 
 
 @gpu
@@ -452,6 +460,15 @@ def test_kv8_append_at_takes_tokens_back(ops):
     check_cache(cache, ks, vs, [104, 130])
     ops.kv8_append(cache, k, v, at=torch.zeros(2, dtype=torch.int64, device=DEV))
     check_cache(cache, list(k.transpose(1, 2).contiguous()), list(v.transpose(1, 2).contiguous()), [100, 100])
+    ops.kv8_append(cache, k[:, :, :0], v[:, :, :0], at=torch.tensor([64, 99], device=DEV))      # nothing but taken back
+    check_cache(cache, [k[0, :, :64].transpose(0, 1), k[1, :, :99].transpose(0, 1)], [v[0, :, :64].transpose(0, 1), v[1, :, :99].transpose(0, 1)], [64, 99])
+    at = torch.tensor([64 + 63, 127], device=DEV)
+    ops.kv8_append(cache, k[:, :, :63], v[:, :, :63], counts=torch.tensor([63, 28], device=DEV))
+    for i in (0, 1, 2):                                        # the append that completes a block, repeated
+        ops.kv8_append(cache, k[:, :, i:i + 1], v[:, :, i:i + 1], at=at)
+    ks = [torch.cat([k[0, :, :64], k[0, :, :63], k[0, :, 2:3]], 1), torch.cat([k[1, :, :99], k[1, :, :28], k[1, :, 2:3]], 1)]
+    vs = [torch.cat([v[0, :, :64], v[0, :, :63], v[0, :, 2:3]], 1), torch.cat([v[1, :, :99], v[1, :, :28], v[1, :, 2:3]], 1)]
+    check_cache(cache, [t.transpose(0, 1) for t in ks], [t.transpose(0, 1) for t in vs], [128, 128])
 
 
 @gpu
@@ -681,7 +698,7 @@ def test_the_library_checks_sizes_before_any_launch():
     for kw, text in [(dict(hd=80), b"head dim 80"), (dict(Hkv=3), b"divide"), (dict(dtype=1), b"dtype"), (dict(q_sr=4), b"multiples of 8"),
                      (dict(q_sr=1 << 23), b"row stride"), (dict(q_sr=-8), b"row stride"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"),
                      (dict(scale=math.inf), b"scale"), (dict(scale=math.nan), b"scale"), (dict(max_k=-1), b"negative"),
-                     (dict(n_k_tiles=1 << 30), b"tiles x 4 heads")]:
+                     (dict(n_k_tiles=1 << 22), b"tiles x 4 heads"), (dict(n_q_tiles=1 << 22), b"tiles x 4 heads")]:
         s = S(**{**dict(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1), **kw})
         for call in (fwd, bwd):
             assert call(s) == -1 and text in L.star_last_error(), kw
@@ -714,6 +731,13 @@ def test_the_library_checks_sizes_before_any_launch():
     assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 0, 0, None, None, 1, None, 1, None) == -1 and b"null pointer" in L.star_last_error()
     for n in ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "lens", "dropped", "tickets"):
         setattr(c, n, 16)
+    q = _lib.KV8Query(H=4, L=1 << 22)
+    assert L.star_kv8_attn(c, 16, None, None, q, 16, None, 0, None) == -1 and b"4194304 queries" in L.star_last_error()
+    assert L.star_kv8_attn_workspace(c, 4, 1 << 22) == 0
+    for sr in (1 << 23, -8):
+        assert L.star_kv8_append(c, 16, 16, 0, 0, sr, 0, 0, 0, None, None, 1, None, 1, None) == -1 and b"row strides" in L.star_last_error()
+    assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 4, 0, None, None, 1, None, 1, None) == -1 and b"multiples of 8" in L.star_last_error()
+    assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 0, 0, None, None, 1, None, -1, None) == -1 and b"max_rows" in L.star_last_error()
     q = _lib.KV8Query(H=3, L=1)
     assert L.star_kv8_attn(c, 16, None, None, q, 16, None, 0, None) == -1 and b"divide" in L.star_last_error()
     c.T = 1 << 20
