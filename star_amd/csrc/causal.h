@@ -109,4 +109,63 @@ struct TileLoad {
     }
 };
 
+// A row's softmax state in parts: part p's maximum and sum at ml[2 p stride], its HD weighted sums at o[p stride HD].  One
+// wave adds them up, HD / 4 lanes a part, two or four parts side by side, eight of each on their way at once.  What the
+// first trip to memory can hold is asked for in ask(), before anything is waited for; sum() then leaves the whole's
+// maximum and sum of weights in every lane and four of the sums in each lane below HD / 4.
+template <int HD>
+struct PartSum {
+    static constexpr int D4 = HD / 4, G = 64 / D4, U = 8;
+    const float *o, *ml;
+    int64_t stride;
+    int np, at, d4;
+    f32x4 x[U];
+    float m0, l0;
+    __device__ __forceinline__ void load(int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = *(const f32x4*)(o + min(i + u * G + at, np - 1) * stride * HD + 4 * d4);
+    }
+    __device__ __forceinline__ void ask(const float* o_, const float* ml_, int64_t stride_, int np_, int lane) {
+        o = o_, ml = ml_, stride = stride_, np = np_;
+        at = min(lane / D4, G - 1), d4 = lane % D4;                // (96: the last 16 lanes repeat and are not added)
+        const float* p = ml + 2 * min(lane, np - 1) * stride;
+        m0 = p[0], l0 = p[1];
+        load(0);
+    }
+    __device__ __forceinline__ void sum(int lane, float& mm, float& ll, f32x4& r) {
+        mm = m0;
+        for (int p = 64 + lane; p < np; p += 64) mm = fmaxf(mm, ml[2 * p * stride]);
+#pragma unroll
+        for (int k = 32; k > 0; k >>= 1) mm = fmaxf(mm, __shfl_xor(mm, k, 64));
+        ll = 0.f;
+        r = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int c0 = 0; c0 < np; c0 += 64) {
+            const int cnt = min(np - c0, 64);
+            if (c0 > 0) {
+                const float* p = ml + 2 * (c0 + min(lane, cnt - 1)) * stride;
+                m0 = p[0], l0 = p[1];
+            }
+            const float f = lane < cnt ? __builtin_amdgcn_exp2f(m0 - mm) : 0.f;
+            if (lane < cnt) ll += f * l0;
+            for (int i = 0; i < cnt; i += G * U) {
+                if (c0 + i > 0) load(c0 + i);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int p = i + u * G + at;
+                    const float w = __shfl(f, min(p, 63), 64);
+                    if (p < cnt) r += w * x[u];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float t = r[e];
+            if constexpr (HD == 64) t += __shfl_xor(t, 16, 64);
+            t += __shfl(t, HD == 96 ? min(lane + 24, 63) : lane ^ 32, 64);
+            r[e] = t;
+        }
+        ll = wave_sum(ll);
+    }
+};
+
 }  // namespace star

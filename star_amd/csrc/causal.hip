@@ -389,31 +389,44 @@ __global__ __launch_bounds__(256, 1) void causal_few_kernel(const T* __restrict_
     }
 }
 
-// The states that the parts of a row's keys left, joined: one wave a row.
-template <typename T, int HD>
+// The states that the parts of a row's keys left, joined: W waves a row, each adding up its share of the parts.
+template <typename T, int HD, int W>
 __global__ __launch_bounds__(256) void causal_join_kernel(const int32_t* __restrict__ tiles,
                                                          star_causal_shape s, int parts, int rows, const float* __restrict__ sums,
                                                          T* __restrict__ O, float* __restrict__ lse) {
-    const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + (threadIdx.x >> 6);
+    __shared__ __attribute__((aligned(16))) float osh[W > 1 ? W * HD : 4];
+    __shared__ float msh[4], lsh[4];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.y * (4 / W) + wid / W;
     const int h = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int per = (parts + W - 1) / W, p0 = min(wid % W * per, parts - 1);
+    const Partial x = partial<HD>((float*)sums, s, parts, rows, t, p0, h, row);
+    PartSum<HD> ps;
+    ps.ask(x.o, x.ml, rows, min(per, parts - p0), lane);           // (rows that the tile lacks have room as well)
     const Work sq = work_of(tiles, t);
     const int i = sq.first + row;
-    if (row >= rows || i >= sq.nq) return;
-    float mm = M_NONE;
-    for (int p = 0; p < parts; ++p) mm = fmaxf(mm, partial<HD>((float*)sums, s, parts, rows, t, p, h, row).ml[0]);
-    float ll = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 2
-    for (int p = 0; p < parts; ++p) {
-        const Partial x = partial<HD>((float*)sums, s, parts, rows, t, p, h, row);
-        const float f = __builtin_amdgcn_exp2f(x.ml[0] - mm);
-        ll += f * x.ml[1];
-        o0 += f * x.o[lane];
-        if (lane + 64 < HD) o1 += f * x.o[lane + 64];
+    if (i >= sq.nq) return;                                        // (a row's waves alike)
+    float mm, ll;
+    f32x4 o;
+    ps.sum(lane, mm, ll, o);
+    if constexpr (W > 1) {
+        if (lane < HD / 4) *(f32x4*)(osh + wid * HD + 4 * lane) = o;
+        if (lane == 0) msh[wid] = mm, lsh[wid] = ll;
+        __syncthreads();
+        if (wid > 0 || lane >= HD / 4) return;
+        mm = fmaxf(fmaxf(msh[0], msh[1]), fmaxf(msh[2], msh[3]));
+        ll = 0.f;
+        o = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w * per >= parts) break;
+            const float f = __builtin_amdgcn_exp2f(msh[w] - mm);
+            o += f * *(const f32x4*)(osh + w * HD + 4 * lane);
+            ll += f * lsh[w];
+        }
     }
+    if (lane >= HD / 4) return;
     const float inv = ll > 0.f ? 1.0f / ll : ll;                   // no visible key: 0; NaN stays NaN
-    T* orow = O + (int64_t)(sq.q0 + i) * s.o_sr + (int64_t)h * s.o_sh;
-    orow[lane] = (T)(o0 * inv);
-    if (lane + 64 < HD) orow[lane + 64] = (T)(o1 * inv);
+    *(typename Vec<T>::x4*)(O + (int64_t)(sq.q0 + i) * s.o_sr + (int64_t)h * s.o_sh + 4 * lane) = pack4<T>(o * inv);
     if (lane == 0 && lse) lse[(int64_t)h * s.lse_stride + sq.q0 + i] = ll == 0.f ? -INFINITY : mm * A_LN2 + logf(ll);
 }
 
@@ -886,17 +899,23 @@ static int check_causal(const star_causal_shape* s, const char* who) {
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Rows of a workgroup of the forward, and the parts that its keys are cut into: 1 when the query tiles alone fill half of
-// the 512 places (two workgroups a CU) or the keys are few, otherwise so many that they fill them, each of at least 8
-// tiles of keys (two for every wave of the few-query kernel; a part costs its state's trip to memory and a join).
-// 29 queries over 17 sequences of up to 4321 keys, one head of 128: 22 us, 58 in one part; 73 queries over two of up to 4686
-// keys, 24 heads of 96: 33 and 106.
+// Rows of a workgroup of the forward, and the parts that its keys are cut into.  A tile of keys takes a workgroup about
+// 1 us whoever else runs (each CU fetches it for itself), a second launch that joins the parts 3, so few workgroups over
+// keys that are not quite short are cut until there is one for every CU, or two where the parts would still be long.
+// The few-query kernel takes four tiles at once; its break-even is by bytes.  Us in one part and in parts, hd 128, 8 heads,
+// 16 queries: 8.0 and 7.8 over 375 keys, 14.0 and 7.9 over 1000, 80 and 12 over 8000; 64 queries: 11.1 and 9.0 over
+// 320, 26 and 9.2 over 1000, 167 and 17 over 8000.
 static int fwd_rows(const star_causal_shape* s) { return s->max_q <= 16 ? 16 : s->max_q <= 32 ? 32 : CT; }
 static int fwd_parts(const star_causal_shape* s) {
     const int64_t wgs = (int64_t)s->n_q_tiles * s->H;
-    const int most = cdiv(s->max_k, CK) / 8;
-    if (wgs < 1 || wgs >= 256 || most < 2) return 1;
-    return (int)min((int64_t)most, 512 / wgs);
+    const int n = cdiv(s->max_k, CK);
+    const bool few_keys = fwd_rows(s) == CT ? n < 6 : n * s->hd < 7 * 128;
+    if (wgs < 1 || wgs >= 256 || few_keys) return 1;
+    int per = cdiv(n, 256 / wgs);
+    // (two a CU: 200 queries of 16 sequences with 2 heads over 8000 keys 46 -> 35 us; 16 queries, 144 workgroups over 8000
+    // keys 77 -> 59, over 2000 18 -> 20)
+    if (per >= (2 * wgs > 256 ? 40 : 12)) per = cdiv(n, 512 / wgs);
+    return cdiv(n, per);
 }
 static int64_t causal_fwd_bytes(const star_causal_shape* s) {
     const int parts = fwd_parts(s);
@@ -923,9 +942,11 @@ static int launch_causal_fwd(const void* q, const void* k, const void* v, const 
     else if (rows == 32) hipLaunchKernelGGL((causal_few_kernel<T, HD, 2>), CAUSAL_FWD_ARGS);
     else hipLaunchKernelGGL((causal_fwd_kernel<T, HD>), CAUSAL_FWD_ARGS);
 #undef CAUSAL_FWD_ARGS
-    if (parts > 1)
-        hipLaunchKernelGGL((causal_join_kernel<T, HD>), dim3((unsigned)((int64_t)s->n_q_tiles * s->H), rows / 4), dim3(256), 0, st,
-                           tiles, *s, parts, rows, (const float*)sums, (T*)o, lse);
+#define CAUSAL_JOIN_ARGS dim3(256), 0, st, tiles, *s, parts, rows, (const float*)sums, (T*)o, lse
+    const unsigned tiles_h = (unsigned)((int64_t)s->n_q_tiles * s->H);
+    if (parts > 16) hipLaunchKernelGGL((causal_join_kernel<T, HD, 4>), dim3(tiles_h, rows), CAUSAL_JOIN_ARGS);
+    else if (parts > 1) hipLaunchKernelGGL((causal_join_kernel<T, HD, 1>), dim3(tiles_h, rows / 4), CAUSAL_JOIN_ARGS);
+#undef CAUSAL_JOIN_ARGS
     return STAR_OK;
 }
 

@@ -213,11 +213,11 @@ struct AttnArgs {
     const float* bias;
     const int32_t* q_len;
     int slots;                 // (sequence, part) pairs that the grid has room for, >= B
+    int min_part;              // blocks of a part at least
     int nrg;                   // groups of 16 * RT rows
     float* part;               // [slots][Hkv][rows][HD] partial sums, [slots][Hkv][rows][2] maximum and sum behind them
 };
 
-constexpr int MIN_PART = 8;    // blocks (512 tokens) of a part at least: two per wave
 
 __device__ __forceinline__ int held_by(const AttnArgs& a, int b) { return min(max(a.c.lens[b], 0), a.c.T); }
 __device__ __forceinline__ int queries_of(const AttnArgs& a, int b) { return a.q_len ? min(max(a.q_len[b], 0), a.s.L) : a.s.L; }
@@ -241,7 +241,7 @@ __device__ __forceinline__ Parts cut(const AttnArgs& a, int lane) {
     }
     total = wave_sum(total);
     const int64_t room = a.slots - a.c.B;
-    return Parts{(int)max((int64_t)MIN_PART, (total + room - 1) / room)};
+    return Parts{(int)max((int64_t)a.min_part, (total + room - 1) / room)};
 }
 __device__ __forceinline__ int parts_of(int nb, int per) { return nb <= per ? 1 : (nb - 1) / per + 1; }
 
@@ -564,23 +564,15 @@ __global__ __launch_bounds__(256) void kv8_join_few_kernel(AttnArgs a) {
     base = wave_sum(base);
     const float* ml = a.part + (int64_t)a.slots * c.Hkv * rows * HD;
     const int64_t stride = (int64_t)c.Hkv * rows, at0 = (int64_t)base * stride + (int64_t)hk * rows + rho;
-    float mm = M_NONE;
-    for (int p = lane; p < np; p += 64) mm = fmaxf(mm, ml[2 * (at0 + p * stride)]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
-    float ll = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 2
-    for (int p = 0; p < np; ++p) {
-        const int64_t at = at0 + p * stride;
-        const float f = __builtin_amdgcn_exp2f(ml[2 * at] - mm);
-        ll += f * ml[2 * at + 1];
-        o0 += f * a.part[at * HD + lane];
-        if (lane + 64 < HD) o1 += f * a.part[at * HD + 64 + lane];
-    }
+    PartSum<HD> ps;
+    ps.ask(a.part + at0 * HD, ml + 2 * at0, stride, np, lane);
+    float mm, ll;
+    f32x4 o;
+    ps.sum(lane, mm, ll, o);
+    if (lane >= HD / 4) return;
     const float inv = (ll > 0.f ? 1.0f / ll : ll) / VHalf<T>::by;
     T* orow = (T*)a.o + (int64_t)b * a.s.o_sb + (int64_t)(hk * grp + rho % grp) * a.s.o_sh + (int64_t)(rho / grp) * a.s.o_sr;
-    orow[lane] = (T)(o0 * inv);
-    if (lane + 64 < HD) orow[64 + lane] = (T)(o1 * inv);
+    *(typename Vec<T>::x4*)(orow + 4 * lane) = pack4<T>(o * inv);
 }
 
 // Many parts: one workgroup a row, the parts' factors first, one per thread, then every thread adds the
@@ -659,14 +651,22 @@ static int check_cache(const star_kv8_cache* c, const char* who) {
 
 // rows of one workgroup: 16 while they suffice, else as many as keep the codes' conversion cheap against the products
 static int row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-// (sequence, part) pairs that the grid has room for.  512 workgroups (two a CU) run at once: few sequences are cut into
-// parts that fill these places once; where the sequences alone make half of them or more, there is room for three times
-// as many parts besides, so that a sequence much longer than the others does not run alone at the end.
-static int attn_slots(const star_kv8_cache* c, int H, int L) {
-    const int rows = H / c->Hkv * L, nrg = cdiv(rows, 16 * row_tiles(rows));
-    const int64_t places = 512 / ((int64_t)c->Hkv * nrg), most = (int64_t)c->B * cdiv(c->T / KB, MIN_PART);
-    const int64_t s = places >= 2 * c->B ? places : c->B + 3 * (places > 1 ? places : 1);
-    return (int)(s < most ? s : most);
+// (sequence, part) pairs that the grid has room for.  512 workgroups (two a CU) run at once, 256 where the rows take a
+// whole CU's registers: few sequences are cut into parts that fill these places once (8 queries, 64 rows a key head of 64,
+// over 32000 tokens: 32 us with 512 workgroups, 20 with 256); where the sequences alone make half of them or more, there is
+// room for three times as many parts besides, so that a sequence much longer than the others does not run alone at the end.
+// A part has 4 blocks (256 tokens) at least, one per wave, or 24 where the card is full without it.  The join is a launch of
+// its own, 3.4 us, which a short cache does not repay (one query, 8 heads of 128: 10.1 us whole and 12.5 in parts for 1024
+// tokens, 15.0 and 12.9 for 1536, 204 and 21 for 32000; 64 rows a key head of 64: 17.2 and 17.4 for 1024).
+struct Cut { int slots, min_part; };
+static Cut attn_cut(const star_kv8_cache* c, int H, int L) {
+    const int rows = H / c->Hkv * L, rt = row_tiles(rows), nrg = cdiv(rows, 16 * rt), blocks = c->T / KB;
+    const int64_t places = (rt * c->hd <= 192 ? 512 : 256) / ((int64_t)c->Hkv * nrg);
+    const bool full = places < 2 * c->B;
+    const int min_part = full ? 24 : 4;
+    if (full ? blocks <= 32 : blocks * c->hd <= (rt == 4 ? 8 : 18) * 128) return Cut{c->B, min_part};
+    const int64_t most = (int64_t)c->B * cdiv(blocks, min_part), s = full ? c->B + 3 * (places > 1 ? places : 1) : places;
+    return Cut{(int)(s < most ? s : most), min_part};
 }
 
 #define KV8_BY_TYPE(DT, HDIM, CALL)                                                        \
@@ -689,9 +689,9 @@ static void launch_attn(const AttnArgs& a, int rt, hipStream_t st) {
     else if (rt == 2) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 2>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 4>), grid, dim3(256), 0, st, a);
     if (a.slots == a.c.B) return;
-    // (measured at 32 heads: 2 parts on average 4.9 us by waves, 8.3 by workgroups; 32 parts 19 and 7.4)
+    // (one wave has 16 parts, 32 at hd 64, on their way at once: up to 32 the two take the same time, beyond it 64 parts 1 us more)
     const int64_t rows = (int64_t)a.c.B * a.s.H * a.s.L;
-    if (a.slots <= 8 * a.c.B) hipLaunchKernelGGL((kv8_join_few_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    if (a.slots <= 32 * a.c.B) hipLaunchKernelGGL((kv8_join_few_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_join_kernel<T, HD>), dim3((unsigned)rows), dim3(256), 0, st, a);
 }
 
@@ -724,7 +724,7 @@ extern "C" int star_kv8_append(const star_kv8_cache* c, const void* k, const voi
 extern "C" size_t star_kv8_attn_workspace(const star_kv8_cache* c, int H, int L) {
     using namespace star;
     if (check_cache(c, "star_kv8_attn_workspace") || H < c->Hkv || H % c->Hkv || L < 1 || (int64_t)H * L >= (1ll << 24)) return 0;
-    const int slots = attn_slots(c, H, L);
+    const int slots = attn_cut(c, H, L).slots;
     return slots == c->B ? 0 : (size_t)slots * H * L * (c->hd + 2) * sizeof(float);
 }
 
@@ -742,7 +742,8 @@ extern "C" int star_kv8_attn(const star_kv8_cache* c, const void* q, const float
     // (a launch has less than 2^32 threads in x)
     STAR_REQUIRE((int64_t)c->B * s->H * s->L < (1ll << 24), "star_kv8_attn: %d sequences x %d heads x %d queries", c->B, s->H, s->L);
     const int rows = s->H / c->Hkv * s->L, rt = row_tiles(rows);
-    AttnArgs a{*c, *s, q, o, s->bias_len > 0 ? bias : nullptr, q_len, attn_slots(c, s->H, s->L), cdiv(rows, 16 * rt), (float*)workspace};
+    const Cut cut = attn_cut(c, s->H, s->L);
+    AttnArgs a{*c, *s, q, o, s->bias_len > 0 ? bias : nullptr, q_len, cut.slots, cut.min_part, cdiv(rows, 16 * rt), (float*)workspace};
     STAR_REQUIRE((int64_t)a.slots * c->Hkv * a.nrg < (1ll << 24), "star_kv8_attn: %d parts x %d heads x %d groups of rows", a.slots, c->Hkv, a.nrg);
     STAR_REQUIRE(!(s->bias_len > 0 && !bias), "star_kv8_attn: bias_len > 0 but bias is null");
     if (workspace_bytes < star_kv8_attn_workspace(c, s->H, s->L) || (a.slots > c->B && !workspace)) {

@@ -1707,7 +1707,7 @@ def _causal_forward(q, k, v, plan, s, want_lse):
         if plan.q_used != rows:
             lse.fill_(-math.inf)
     # (only launches of few workgroups over many keys are cut along the keys)
-    need = lib().star_causal_fwd_workspace(s) if plan.max_k > 960 and plan.n_q_tiles * s.H < 256 else 0
+    need = lib().star_causal_fwd_workspace(s) if plan.max_k > 320 and plan.n_q_tiles * s.H < 256 else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
     _launch(lib().star_causal_fwd, "star_causal_fwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.q_tiles_ptr, s,
             o.data_ptr(), ptr(lse), ptr(ws), need)

@@ -93,6 +93,10 @@ SHAPES = [  # keys, queries (None: the same), H, Hkv, hd, dtype
     ([3001], [30], 2, 2, 64, FP),
     ([2000, 100], [130, 100], 2, 1, 96, BF),
     ([10, 1500], [200, 60], 1, 1, 128, FP),
+    ([450, 20], [40, 20], 2, 2, 128, BF),
+    ([2600] * 11, [2] * 11, 12, 12, 64, FP),                   # two workgroups a CU, three parts
+    ([20000, 0], [16, 3], 1, 1, 128, BF),                      # so many parts that four waves join a row
+    ([185000], [3], 1, 1, 64, FP),                             # more parts a wave than lanes
 ]
 
 
@@ -525,6 +529,10 @@ CACHED = [  # lens, L, H, Hkv, hd, dtype, capacity
     ([300, 64], 5, 12, 2, 64, FP, 320),                       # 30 rows: two tiles
     ([5000, 4096, 100], 1, 32, 8, 128, FP, 5056),             # cut into parts and joined
     ([30000], 2, 2, 1, 96, BF, 30016),
+    ([60000] + [1] * 15, 1, 1, 1, 64, BF, 60032),             # more parts of a row than lanes
+    ([300000], 1, 2, 1, 64, FP, 300032),                      # more than threads
+    ([2150, 7] * 20, 1, 8, 8, 128, BF, 2176),                 # the card full without parts, long sequences cut all the same
+    ([1500, 1], 8, 8, 1, 64, FP, 1536),                       # 64 rows: cut from 1024 tokens of capacity on
     ([64 * (i % 9) + i for i in range(70)], 1, 2, 2, 64, BF, 640),   # more sequences than lanes
 ]
 
@@ -709,7 +717,8 @@ def test_the_library_checks_sizes_before_any_launch():
     assert L.star_causal_fwd(None, None, None, None, S(H=4, Hkv=2, hd=64, dtype=0, scale=1), None, None, None, 0, None) == 0
     # cut along the keys: few query tiles, many keys
     need = lambda nq, n, nk: L.star_causal_fwd_workspace(S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=n, max_q=nq, max_k=nk))  # noqa: E731
-    assert need(16, 1, 960) == 0 and need(16, 1, 1024) == 4 * 2 * 16 * 66 * 4 and need(16, 64, 100000) == 0
+    assert need(16, 1, 832) == 0 and need(16, 1, 833) == 4 * 14 * 16 * 66 * 4 and need(16, 64, 100000) == 0
+    assert need(33, 1, 320) == 0 and need(33, 1, 321) == 4 * 6 * 128 * 66 * 4
     assert need(17, 2, 10 ** 6) == 2 * 4 * 64 * 32 * 66 * 4 and need(33, 63, 10 ** 6) == 63 * 4 * 2 * 128 * 66 * 4
     s = S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1, max_q=16, max_k=4096)
     assert fwd(s) == -3 and b"workspace" in L.star_last_error() and fwd(s, ws=16, n=100) == -3 and fwd(s, ws=24, n=1 << 30) == -3
