@@ -214,6 +214,7 @@ struct AttnArgs {
     const int32_t* q_len;
     int slots;                 // (sequence, part) pairs that the grid has room for, >= B
     int min_part;              // blocks of a part at least
+    int even;                  // 1: sequences of much the same length stay whole
     int nrg;                   // groups of 16 * RT rows
     float* part;               // [slots][Hkv][rows][HD] partial sums, [slots][Hkv][rows][2] maximum and sum behind them
 };
@@ -235,11 +236,18 @@ struct Parts { int per; };
 __device__ __forceinline__ Parts cut(const AttnArgs& a, int lane) {
     if (a.slots == a.c.B) return Parts{0x7fffffff};
     int64_t total = 0;
+    int top = 0;
     for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-        const int b = b0 + lane;
-        total += b < a.c.B ? blocks_of(a, b) : 0;
+        const int b = b0 + lane, nb = b < a.c.B ? blocks_of(a, b) : 0;
+        total += nb;
+        top = max(top, nb);
     }
     total = wave_sum(total);
+    if (a.even) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+        if (2 * (int64_t)top * a.c.B <= 3 * total) return Parts{0x7fffffff};
+    }
     const int64_t room = a.slots - a.c.B;
     return Parts{(int)max((int64_t)a.min_part, (total + room - 1) / room)};
 }
@@ -655,18 +663,20 @@ static int row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 // whole CU's registers: few sequences are cut into parts that fill these places once (8 queries, 64 rows a key head of 64,
 // over 32000 tokens: 32 us with 512 workgroups, 20 with 256); where the sequences alone make half of them or more, there is
 // room for three times as many parts besides, so that a sequence much longer than the others does not run alone at the end.
+// Sequences that fill three quarters of the places and of which none is longer than 1.5 times their mean stay whole (53
+// of 2590 to 2908 tokens, 8 key heads of 128, 5 queries: 97 us in parts, 73 whole).
 // A part has 4 blocks (256 tokens) at least, one per wave, or 24 where the card is full without it.  The join is a launch of
 // its own, 3.4 us, which a short cache does not repay (one query, 8 heads of 128: 10.1 us whole and 12.5 in parts for 1024
 // tokens, 15.0 and 12.9 for 1536, 204 and 21 for 32000; 64 rows a key head of 64: 17.2 and 17.4 for 1024).
-struct Cut { int slots, min_part; };
+struct Cut { int slots, min_part, even; };
 static Cut attn_cut(const star_kv8_cache* c, int H, int L) {
     const int rows = H / c->Hkv * L, rt = row_tiles(rows), nrg = cdiv(rows, 16 * rt), blocks = c->T / KB;
     const int64_t places = (rt * c->hd <= 192 ? 512 : 256) / ((int64_t)c->Hkv * nrg);
     const bool full = places < 2 * c->B;
     const int min_part = full ? 24 : 4;
-    if (full ? blocks <= 32 : blocks * c->hd <= (rt == 4 ? 8 : 18) * 128) return Cut{c->B, min_part};
+    if (full ? blocks <= 32 : blocks * c->hd <= (rt == 4 ? 8 : 18) * 128) return Cut{c->B, min_part, 0};
     const int64_t most = (int64_t)c->B * cdiv(blocks, min_part), s = full ? c->B + 3 * (places > 1 ? places : 1) : places;
-    return Cut{(int)(s < most ? s : most), min_part};
+    return Cut{(int)(s < most ? s : most), min_part, 4 * c->B >= 3 * places};
 }
 
 #define KV8_BY_TYPE(DT, HDIM, CALL)                                                        \
@@ -743,7 +753,7 @@ extern "C" int star_kv8_attn(const star_kv8_cache* c, const void* q, const float
     STAR_REQUIRE((int64_t)c->B * s->H * s->L < (1ll << 24), "star_kv8_attn: %d sequences x %d heads x %d queries", c->B, s->H, s->L);
     const int rows = s->H / c->Hkv * s->L, rt = row_tiles(rows);
     const Cut cut = attn_cut(c, s->H, s->L);
-    AttnArgs a{*c, *s, q, o, s->bias_len > 0 ? bias : nullptr, q_len, cut.slots, cut.min_part, cdiv(rows, 16 * rt), (float*)workspace};
+    AttnArgs a{*c, *s, q, o, s->bias_len > 0 ? bias : nullptr, q_len, cut.slots, cut.min_part, cut.even, cdiv(rows, 16 * rt), (float*)workspace};
     STAR_REQUIRE((int64_t)a.slots * c->Hkv * a.nrg < (1ll << 24), "star_kv8_attn: %d parts x %d heads x %d groups of rows", a.slots, c->Hkv, a.nrg);
     STAR_REQUIRE(!(s->bias_len > 0 && !bias), "star_kv8_attn: bias_len > 0 but bias is null");
     if (workspace_bytes < star_kv8_attn_workspace(c, s->H, s->L) || (a.slots > c->B && !workspace)) {
