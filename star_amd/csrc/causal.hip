@@ -24,6 +24,16 @@ __device__ __forceinline__ Work work_of(const int32_t* tiles, int t) {
     return Work{w[0], w[1], w[2], w[3], w[4]};
 }
 
+// keys that the queries of a tile see
+__device__ __forceinline__ int keys_seen(const Work& w) { return max(0, min(w.nk, min(w.first + CT, w.nq) + w.nk - w.nq)); }
+// tiles of CQ queries that see keys of a tile, per head, and the first of them
+constexpr int CQ = 32;
+struct Walk { int first, n; };
+__device__ __forceinline__ Walk queries_of(const Work& w) {
+    const int first = max(0, w.first - (w.nk - w.nq)) / CQ;
+    return Walk{first, max(0, (w.nq + CQ - 1) / CQ - first)};
+}
+
 // Few query tiles over long keys are cut along the keys: part p of `parts` walks its share of a tile's key tiles and
 // leaves its softmax state, sums[tile][head][part][row][HD], then maximum and sum [tile][head][part][row][2].
 struct KeyTiles { int first, end; };
@@ -436,12 +446,14 @@ __global__ __launch_bounds__(256) void causal_join_kernel(const int32_t* __restr
 // sees few keys and |o| is not small against |V|: with o's delta the error of dQ and dK was 1.55 times that of rounding
 // the exact gradients once.  A workgroup that sees at most two tiles of keys therefore walks them twice, first for
 // delta = sum_j P dP in 32 bits; its walk is the shortest there is.
+// A launch of few workgroups or very unequal ones is cut: part p takes tiles p * per .. of a walk, and a walk of more than
+// one part leaves fp32 sums, which causal_dq_sum_kernel adds up in order.
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                           const T* __restrict__ V, const T* __restrict__ O,
                                                           const T* __restrict__ dO, const float* __restrict__ lse,
-                                                          const int32_t* __restrict__ tiles, star_causal_shape s,
-                                                          T* __restrict__ dQ, float* __restrict__ delta) {
+                                                          const int32_t* __restrict__ tiles, star_causal_shape s, int parts, int per,
+                                                          float* __restrict__ sums, T* __restrict__ dQ, float* __restrict__ delta) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
     using Ti = Tile<T, HD>;
@@ -451,11 +463,13 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
-    const int hi = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const int hi = blockIdx.x % s.H, part = blockIdx.x / s.H % parts, t = blockIdx.x / s.H / parts;
     const int hk = hi % s.Hkv, h = hk * (s.H / s.Hkv) + hi / s.Hkv;
     const Work sq = work_of(tiles, t);
     const int i0 = sq.first;
     const int off = sq.nk - sq.nq;
+    const int end = keys_seen(sq), ntile = (end + CK - 1) / CK, t0 = part * per, t1 = min(ntile, t0 + per);
+    if (part > 0 && t0 >= ntile) return;
     const T* Kh = K + (int64_t)sq.k0 * s.k_sr + (int64_t)hk * s.k_sh;
     const T* Vh = V + (int64_t)sq.k0 * s.v_sr + (int64_t)hk * s.v_sh;
 
@@ -487,7 +501,6 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
     }
     const int all_see = w0 + 32 <= sq.nq ? max(0, min(sq.nk, w0 + off + 1)) : 0;
     const int wave_end = w0 < sq.nq ? max(0, min(sq.nk, min(w0 + 32, sq.nq) + off)) : 0;
-    const int end = max(0, min(sq.nk, min(i0 + CT, sq.nq) + off));
     const float c2 = s.scale * A_LOG2E;
 
     f32x4 acc[2][NT];
@@ -497,12 +510,11 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
         for (int nt = 0; nt < NT; ++nt) acc[qb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
     TileLoad<T, HD, CK, 256> kl, vl;
-    const int ntile = (end + CK - 1) / CK;
     kl.place(s.k_sr, tid);
     vl.place(s.v_sr, tid);
     if (ntile > 0) {
-        kl.load(Kh, s.k_sr, 0, sq.nk, tid);
-        vl.load(Vh, s.v_sr, 0, sq.nk, tid);
+        kl.load(Kh, s.k_sr, t0 * CK, sq.nk, tid);
+        vl.load(Vh, s.v_sr, t0 * CK, sq.nk, tid);
     }
     if (ntile <= 2) {                                              // both tiles stay in LDS, each in its own half
         float d[2] = {0.f, 0.f};
@@ -551,7 +563,7 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
         const int i = w0 + 16 * qb + r16;
-        if (g == 0 && i < sq.nq) delta[(int64_t)h * s.lse_stride + sq.q0 + i] = dl[qb];
+        if (g == 0 && i < sq.nq && part == 0) delta[(int64_t)h * s.lse_stride + sq.q0 + i] = dl[qb];
     }
     auto step = [&](int tile, const uint8_t* kt, const uint8_t* vt) {
         const int key0 = tile * CK;
@@ -615,13 +627,13 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
         for (int tile = 0; tile < ntile; ++tile) step(tile, smem + tile * 2 * TB, smem + tile * 2 * TB + TB);
     } else {
 #pragma unroll 1
-        for (int tile = 0; tile < ntile; ++tile) {
+        for (int tile = t0; tile < t1; ++tile) {
             uint8_t* kt = smem + (tile & 1) * 2 * TB;
             uint8_t* vt = kt + TB;
             kl.store(kt, tid);
             vl.store(vt, tid);
             __syncthreads();
-            if (tile + 1 < ntile) {
+            if (tile + 1 < t1) {
                 kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
                 vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
             }
@@ -632,6 +644,12 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
     for (int qb = 0; qb < 2; ++qb) {
         const int i = w0 + 16 * qb + r16;
         if (i >= sq.nq) continue;
+        if (ntile > per) {
+            float* row = sums + (((int64_t)part * s.lse_stride + sq.q0 + i) * s.H + h) * HD + 4 * g;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) *(f32x4*)(row + 16 * nt) = acc[qb][nt];
+            continue;
+        }
         T* row = dQ + (int64_t)(sq.q0 + i) * s.dq_sr + h * HD + 4 * g;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -643,21 +661,39 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
     }
 }
 
+// the fp32 sums of 16 rows -> dQ
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void causal_dq_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ tiles, star_causal_shape s, int per,
+                                                           T* __restrict__ dQ) {
+    const int h = blockIdx.x % s.H, t = blockIdx.x / s.H;
+    const Work sq = work_of(tiles, t);
+    const int np = ((keys_seen(sq) + CK - 1) / CK + per - 1) / per, i0 = sq.first + 16 * blockIdx.y, rows = min(16, sq.nq - i0);
+    if (np <= 1) return;
+    const int64_t one = s.lse_stride * s.H * HD;
+    for (int c = threadIdx.x; c < rows * (HD / 4); c += 256) {
+        const int64_t row = sq.q0 + i0 + c / (HD / 4), d = h * HD + 4 * (c % (HD / 4));
+        f32x4 sum = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int p = 0; p < np; ++p) sum += *(const f32x4*)(sums + p * one + row * s.H * HD + d);
+        *(typename Vec<T>::x4*)(dQ + row * s.dq_sr + d) = pack4<T>(sum * s.scale);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------ gradients of K, V
 // One workgroup: 128 keys of one key head, 32 per wave with K, dK^T and dV^T in registers and V in LDS (with V in
 // registers too only one wave would fit a SIMD, and nothing would cover its LDS and exponential latencies); it walks the
 // queries of its query heads in tiles of 32.  The key is on the MFMA column, so P and dS come out as the operands of
 // dV^T += dO^T P and dK^T += Q^T dS.
-// A launch with few key tiles is cut by query heads (`parts` > 1): part p takes heads p * grp / parts .. of the group and
-// leaves fp32 sums, which causal_dkv_sum_kernel adds up in order.
-constexpr int CQ = 32;
+// A launch of few workgroups is cut, first by query heads: part p of hp takes heads p * grp / hp .. of the group (an XCD
+// then reads few heads); if that is not enough, each of these walks by its steps, `per` to a piece.  Where a tile
+// has more than one part or piece they leave fp32 sums, which causal_dkv_sum_kernel adds up in order.
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                            const T* __restrict__ V, const T* __restrict__ dO,
                                                            const float* __restrict__ lse, const float* __restrict__ delta,
                                                            const int32_t* __restrict__ tiles, star_causal_shape s,
-                                                           int parts, float* __restrict__ sums, T* __restrict__ dK,
-                                                           T* __restrict__ dV) {
+                                                           int hp, int pieces, int per, float* __restrict__ sums,
+                                                           T* __restrict__ dK, T* __restrict__ dV) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
     using Ti = Tile<T, HD>;
@@ -667,9 +703,12 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
 
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % s.Hkv, part = blockIdx.x / s.Hkv % parts, t = blockIdx.x / s.Hkv / parts;
-    const int heads = s.H / s.Hkv / parts, h0 = hk * (s.H / s.Hkv) + part * heads;
+    const int hk = blockIdx.x % s.Hkv, part = blockIdx.x / s.Hkv % (hp * pieces), t = blockIdx.x / s.Hkv / (hp * pieces);
+    const int piece = part / hp, heads = s.H / s.Hkv / hp;
     const Work sq = work_of(tiles, t);
+    const Walk walk = queries_of(sq);
+    const int total = walk.n * heads, n0 = piece * per, ntile = min(per, total - n0);
+    if (piece > 0 && ntile <= 0) return;
     const int j0 = sq.first, w0 = j0 + 32 * wid;           // first key of the workgroup, of the wave
     const int off = sq.nk - sq.nq;
     uint8_t* vt = smem + 32 * wid * Ti::ROWB;                      // the wave's rows of V
@@ -695,13 +734,18 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) dk[kb][nt] = dv[kb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const float c2 = s.scale * A_LOG2E;
-    const int first = max(0, j0 - off) / CQ;                       // query tiles before it see none of these keys
-    const int nper = max(0, (sq.nq + CQ - 1) / CQ - first);        // tiles per head
+    const int first = walk.first;
     const int all_see = w0 + 31 - off;                             // from this query on every key of the wave is visible
 
     TileLoad<T, HD, CQ, 256> ql, gl;
     float lr = 0.f;
-    int lh = h0, lq = first * CQ;                                  // head and first query of the next tile to load
+    // head and first query of the next tile to load
+    int lh = hk * (s.H / s.Hkv) + part % hp * heads, lq = first * CQ;
+    if (n0 > 0) {
+        const int skip = __builtin_amdgcn_readfirstlane(n0 / walk.n);
+        lh += skip;
+        lq += (n0 - skip * walk.n) * CQ;
+    }
     auto load = [&]() {
         ql.load(Q + (int64_t)sq.q0 * s.q_sr + (int64_t)lh * s.q_sh, s.q_sr, lq, sq.nq, tid);
         gl.load(dO + (int64_t)sq.q0 * s.o_sr + (int64_t)lh * s.o_sh, s.o_sr, lq, sq.nq, tid);
@@ -714,8 +758,7 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     };
     ql.place(s.q_sr, tid);
     gl.place(s.o_sr, tid);
-    const int ntile = nper * heads;
-    int q0 = first * CQ;
+    int q0 = lq;
     if (ntile > 0) load();
 #pragma unroll 1
     for (int n = 0; n < ntile; ++n) {
@@ -817,7 +860,7 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
         const int j = w0 + 16 * kb + r16;
         if (j >= sq.nk) continue;
         const int64_t at = (int64_t)(sq.k0 + j) * s.dkv_sr + hk * HD + 4 * g;
-        if (parts > 1) {
+        if (hp > 1 || total > per) {
             float* sk = sums + ((int64_t)part * 2 * s.k_rows + sq.k0 + j) * s.Hkv * HD + hk * HD + 4 * g;
             float* sv = sk + s.k_rows * s.Hkv * HD;
 #pragma unroll
@@ -841,14 +884,14 @@ __global__ __launch_bounds__(256, 2) void causal_dkv_kernel(const T* __restrict_
     }
 }
 
-// parts fp32 sums of 16 keys -> dK, dV
+// the fp32 sums of 16 keys -> dK, dV
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ tiles, star_causal_shape s, int parts,
+__global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __restrict__ sums, const int32_t* __restrict__ tiles, star_causal_shape s, int hp, int per,
                                                             T* __restrict__ dK, T* __restrict__ dV) {
-    typedef typename Vec<T>::x4 x4;
     const int hk = blockIdx.x % s.Hkv, t = blockIdx.x / s.Hkv;
     const Work sq = work_of(tiles, t);
-    const int j0 = sq.first + 16 * blockIdx.y, rows = min(16, sq.nk - j0);
+    const int np = hp * max(1, (queries_of(sq).n * (s.H / s.Hkv / hp) + per - 1) / per), j0 = sq.first + 16 * blockIdx.y, rows = min(16, sq.nk - j0);
+    if (np <= 1) return;
     const int64_t one = s.k_rows * s.Hkv * HD;
     for (int c = threadIdx.x; c < 2 * 16 * (HD / 4); c += 256) {
         const int which = c / (16 * (HD / 4)), cc = c % (16 * (HD / 4));
@@ -856,27 +899,42 @@ __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __rest
         const int64_t row = sq.k0 + j0 + cc / (HD / 4), d = hk * HD + 4 * (cc % (HD / 4)), at = row * s.Hkv * HD + d;
         f32x4 sum = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int p = 0; p < parts; ++p) sum += *(const f32x4*)(sums + (2 * p + which) * one + at);
-        x4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (T)(which ? sum[e] : sum[e] * s.scale);
-        *(x4*)((which ? dV : dK) + row * s.dkv_sr + d) = o;
+        for (int p = 0; p < np; ++p) sum += *(const f32x4*)(sums + (2 * p + which) * one + at);
+        *(typename Vec<T>::x4*)((which ? dV : dK) + row * s.dkv_sr + d) = pack4<T>(which ? sum : sum * s.scale);
     }
 }
 
-// Parts of the query heads of a group: 1 when the longest walk is short (under 16 tiles of 32 queries over all heads), or
-// the key tiles alone fill the 512 places (two workgroups a CU) once -- twice where walks go from 1 tile to 32 and more,
-// which leave no balance to a single round; otherwise the fewest that do.  Forward and backward of 2 sequences of up to 622
-// tokens, 16 heads on 2 of 96: 75 us, 217 in one part; 25 of up to 131, 32 heads on 4 of 64: 61 and 81; 8191 tokens, 16
-// heads on 4 of 128: 1223 for 1024 workgroups, 1422 for 512.
-static int dkv_parts(const star_causal_shape* s) {
+// Pieces of the walks of a launch of wgs workgroups, `longest` steps at most and `mean` on average (a causal walk is
+// anything up to the longest): steps of `per`, so that wgs * (mean / per + 1/2) pieces, which is what such walks come to, fill
+// the 512 places (two a CU) once.  From 320 workgroups on, and from 256 with walks of middle length, a walk in one piece is as good or better: two rounds of pieces
+// and the sums' way through memory cost what the idle CUs did.  Forward and backward, 8 heads of 128: one sequence of 1500
+// tokens 151 -> 95 us, 3000 tokens 294 -> 182, 5000 tokens (320 workgroups) 522 -> 384; 6 of 800 to 1300 (400) 162 -> 196.
+struct Pieces { int hp, pieces, per; };                            // parts by heads, pieces of the longest walk, steps of a piece
+static Pieces pieces(int hp, int64_t wgs, int64_t longest, int64_t mean, int least) {
+    const int64_t room = 512 - wgs / 2;
+    if (wgs < 1 || wgs > 320 || 2 * longest <= (wgs > 256 ? 12 : 3) * least) return Pieces{hp, 1, 0x3fffffff};
+    const int64_t per = max((int64_t)least, (wgs * mean + room - 1) / room);
+    if (per >= longest) return Pieces{hp, 1, 0x3fffffff};
+    return Pieces{hp, (int)((longest + per - 1) / per), (int)per};
+}
+static Pieces dq_pieces(const star_causal_shape* s) {
+    const int64_t n = cdiv(s->max_k, CK);
+    return pieces(1, (int64_t)s->n_q_tiles * s->H, n, max((int64_t)1, n - cdiv(min(s->max_q, s->max_k), CT)), 4);
+}
+// By query heads: into 1 when the longest walk is short (under 16 tiles of 32 queries over all heads), or the key tiles
+// alone fill the 512 places once -- twice where walks go from 1 tile to 32 and more, which leave no balance to a
+// single round; otherwise into the fewest that do.  Forward and backward of 2 sequences of up to 622 tokens, 16 heads on
+// 2 of 96: 75 us, 217 in one part; 25 of up to 131, 32 heads on 4 of 64: 61 and 81; 8191 tokens, 16 heads on 4 of 128: 1223
+// for 1024 workgroups, 1422 for 512 -- and 1650 for as many pieces of the whole walk.
+static Pieces dkv_pieces(const star_causal_shape* s) {
     const int grp = s->H / s->Hkv, walk = cdiv(s->max_q, CQ);
-    int parts = 1;
+    int hp = 1;
     if ((int64_t)grp * walk >= 16)
-        while (parts < grp && (int64_t)s->n_k_tiles * s->Hkv * parts < (walk >= 32 ? 1024 : 512)) {
-            do ++parts; while (grp % parts);
+        while (hp < grp && (int64_t)s->n_k_tiles * s->Hkv * hp < (walk >= 32 ? 1024 : 512)) {
+            do ++hp; while (grp % hp);
         }
-    return parts;
+    const int64_t heads = grp / hp, mean = max(1, walk - cdiv(min(s->max_q, s->max_k), 2 * CQ));
+    return pieces(hp, (int64_t)s->n_k_tiles * s->Hkv * hp, heads * walk, heads * mean, 8);
 }
 
 // ------------------------------------------------------------------------------------------------------ host side
@@ -951,8 +1009,9 @@ static int launch_causal_fwd(const void* q, const void* k, const void* v, const 
 }
 
 static int64_t causal_bwd_bytes(const star_causal_shape* s) {
-    const int parts = dkv_parts(s);
-    return parts == 1 ? 0 : (int64_t)parts * 2 * s->k_rows * s->Hkv * s->hd * 4;
+    const Pieces k = dkv_pieces(s);
+    const int64_t pq = dq_pieces(s).pieces, pk = (int64_t)k.hp * k.pieces;
+    return max(pq == 1 ? 0 : pq * s->lse_stride * s->H, pk == 1 ? 0 : pk * 2 * s->k_rows * s->Hkv) * s->hd * 4;
 }
 
 template <typename T, int HD>
@@ -968,17 +1027,23 @@ static int launch_causal_bwd(const void* q, const void* k, const void* v, const 
         set_error("star_causal_bwd: cannot reserve %d bytes of LDS", smem_k);
         return STAR_ERR_LAUNCH;
     }
-    if (s->n_q_tiles > 0)
-        hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3((unsigned)s->n_q_tiles * s->H), dim3(256), smem_q, st, (const T*)q,
-                           (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, q_tiles, *s, (T*)dq, delta);
+    if (s->n_q_tiles > 0) {
+        const Pieces p = dq_pieces(s);
+        const unsigned wgs = (unsigned)s->n_q_tiles * s->H;
+        hipLaunchKernelGGL((causal_dq_kernel<T, HD>), dim3(wgs * p.pieces), dim3(256), smem_q, st, (const T*)q,
+                           (const T*)k, (const T*)v, (const T*)o, (const T*)do_, lse, q_tiles, *s, p.pieces, p.per, sums, (T*)dq, delta);
+        if (p.pieces > 1)
+            hipLaunchKernelGGL((causal_dq_sum_kernel<T, HD>), dim3(wgs, CT / 16), dim3(256), 0, st, (const float*)sums, q_tiles, *s, p.per, (T*)dq);
+    }
     if (s->n_k_tiles > 0) {
-        const int parts = dkv_parts(s);
-        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3((unsigned)s->n_k_tiles * s->Hkv * parts), dim3(256), smem_k, st,
+        const Pieces p = dkv_pieces(s);
+        const unsigned wgs = (unsigned)s->n_k_tiles * s->Hkv;
+        hipLaunchKernelGGL((causal_dkv_kernel<T, HD>), dim3(wgs * p.hp * p.pieces), dim3(256), smem_k, st,
                            (const T*)q, (const T*)k, (const T*)v, (const T*)do_, lse, (const float*)delta, k_tiles, *s,
-                           parts, sums, (T*)dk, (T*)dv);
-        if (parts > 1)
-            hipLaunchKernelGGL((causal_dkv_sum_kernel<T, HD>), dim3((unsigned)s->n_k_tiles * s->Hkv, CT / 16), dim3(256), 0, st,
-                               (const float*)sums, k_tiles, *s, parts, (T*)dk, (T*)dv);
+                           p.hp, p.pieces, p.per, sums, (T*)dk, (T*)dv);
+        if (p.hp * p.pieces > 1)
+            hipLaunchKernelGGL((causal_dkv_sum_kernel<T, HD>), dim3(wgs, CT / 16), dim3(256), 0, st,
+                               (const float*)sums, k_tiles, *s, p.hp, p.per, (T*)dk, (T*)dv);
     }
     return STAR_OK;
 }

@@ -1722,7 +1722,8 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
     if g.data_ptr() % 16:
         g = g.clone()
     delta = torch.empty_like(lse)
-    need = lib().star_causal_bwd_workspace(s) if s.H != s.Hkv else 0
+    # (heads that do not share keys over short sequences are never cut)
+    need = lib().star_causal_bwd_workspace(s) if s.H != s.Hkv or max(plan.max_q, plan.max_k) > 256 else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     _launch(lib().star_causal_bwd, "star_causal_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
             g.data_ptr(), lse.data_ptr(), plan.q_tiles_ptr, plan.k_tiles_ptr, s, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),

@@ -97,6 +97,11 @@ SHAPES = [  # keys, queries (None: the same), H, Hkv, hd, dtype
     ([2600] * 11, [2] * 11, 12, 12, 64, FP),                   # two workgroups a CU, three parts
     ([20000, 0], [16, 3], 1, 1, 128, BF),                      # so many parts that four waves join a row
     ([185000], [3], 1, 1, 64, FP),                             # more parts a wave than lanes
+    # gradients in pieces: of long walks, beside short and empty ones, of the heads' parts, with more queries than keys
+    ([2100], None, 2, 1, 64, BF),
+    ([1200, 0, 5, 300, 0], [700, 3, 400, 300, 0], 2, 2, 128, FP),
+    ([900, 130], None, 6, 2, 96, BF),
+    ([200, 1], [1500, 700], 1, 1, 64, BF),
 ]
 
 
@@ -723,8 +728,8 @@ def test_the_library_checks_sizes_before_any_launch():
     s = S(H=4, Hkv=2, hd=64, dtype=0, scale=1, n_q_tiles=1, max_q=16, max_k=4096)
     assert fwd(s) == -3 and b"workspace" in L.star_last_error() and fwd(s, ws=16, n=100) == -3 and fwd(s, ws=24, n=1 << 30) == -3
     # cut by query heads: few key tiles, long walks
-    s = S(H=4, Hkv=1, hd=64, dtype=0, k_rows=2000, scale=1, dq_sr=256, dkv_sr=64, n_k_tiles=16, max_q=2000)
-    assert L.star_causal_bwd_workspace(s) == 4 * 2 * 2000 * 64 * 4
+    s = S(H=4, Hkv=1, hd=64, dtype=0, k_rows=2000, scale=1, dq_sr=256, dkv_sr=64, n_k_tiles=16, max_q=2000, max_k=2000)
+    assert L.star_causal_bwd_workspace(s) == 4 * 8 * 2 * 2000 * 64 * 4     # and each of the 4 heads' walks into 8 pieces
     assert bwd(s) == -3 and b"workspace" in L.star_last_error()
     s.dq_sr = 128
     assert bwd(s) == -1 and b"gradient row" in L.star_last_error()
@@ -733,6 +738,12 @@ def test_the_library_checks_sizes_before_any_launch():
     s.n_k_tiles = 1024
     assert L.star_causal_bwd_workspace(s) == 0
     s.n_k_tiles, s.max_q = 16, 96
+    assert L.star_causal_bwd_workspace(s) == 0
+    # the queries' gradient by tiles of keys: 16 of 16 tiles in pieces of 4 (mean 8; 32 workgroups)
+    s.n_q_tiles, s.n_k_tiles, s.H, s.Hkv, s.max_q, s.max_k, s.lse_stride, s.k_rows = 8, 0, 4, 4, 1024, 1024, 1024, 1024
+    s.dq_sr, s.dkv_sr = 256, 256
+    assert L.star_causal_bwd_workspace(s) == 4 * 1024 * 4 * 64 * 4
+    s.max_q = s.max_k = 384
     assert L.star_causal_bwd_workspace(s) == 0
     c = _lib.KV8Cache(B=1, Hkv=2, T=100, hd=64, dtype=0)
     assert L.star_kv8_append(c, 16, 16, 0, 0, 0, 0, 0, 0, None, None, 1, None, 1, None) == -1 and b"capacity 100" in L.star_last_error()
