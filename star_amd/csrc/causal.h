@@ -168,4 +168,46 @@ struct PartSum {
     }
 };
 
+// A tile on its way through buffer loads, one 16-byte piece of a thread at a time and without a branch, so that the pieces
+// can be asked for between other instructions: a load holds its wave for 64 clocks when the four waves of a workgroup
+// ask at once, and eight in a row hold it longer than the products of a tile take.  Rows at or past `limit` are zeros
+// by the range check (their weights are exact zeros as well), so a tile behind the last one is asked for like any other.
+template <typename T, int HD, int ROWS, int NTH>
+struct TileBuf {
+    static constexpr int CHUNKS = HD / 8, TOTAL = ROWS * CHUNKS, N = (TOTAL + NTH - 1) / NTH;
+    static constexpr bool EVEN = NTH % CHUNKS == 0 && TOTAL % NTH == 0;
+    u32x4 v[N];
+    uint32_t at[EVEN ? 1 : N];
+    __device__ __forceinline__ void place(int64_t sr, int tid) {
+#pragma unroll
+        for (int i = 0; i < (EVEN ? 1 : N); ++i) {
+            const int c = min(tid + i * NTH, TOTAL - 1);
+            at[i] = (uint32_t)(c / CHUNKS) * (uint32_t)(sr * 2) + (uint32_t)(c % CHUNKS) * 16;
+        }
+    }
+    // the rows from row0 on (at most (ROWS - 1) * 2^24 + HD * 2 bytes: row strides are below 2^23 values)
+    __device__ static __forceinline__ auto rows(const T* g, int64_t sr, int row0, int limit) {
+        const int n = max(0, min(ROWS, limit - row0));
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(g + (int64_t)row0 * sr), 0, n > 0 ? (n - 1) * (int)(sr * 2) + HD * 2 : 0, 0x00020000);
+    }
+    template <typename R>
+    __device__ __forceinline__ void load(R rows, int64_t sr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t off = EVEN ? at[0] + i * (NTH / CHUNKS) * (uint32_t)(sr * 2) : at[i];
+            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, off, 0, 0));
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + i * NTH;
+            if (TOTAL % NTH == 0 || c < TOTAL) *(u32x4*)(tile + c / CHUNKS * Tile<T, HD>::ROWB + (c % CHUNKS) * 16) = v[i];
+        }
+    }
+};
+
+// what __builtin_amdgcn_sched_group_barrier(kind, how many, 0) puts in order, one call after another, within a block of code
+constexpr int SG_VALU = 0x2, SG_MFMA = 0x8, SG_VMEM_READ = 0x20, SG_DS_READ = 0x100, SG_DS_WRITE = 0x200;
+
 }  // namespace star

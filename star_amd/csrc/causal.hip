@@ -100,28 +100,34 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
         l[qb] = 0.f;
     }
 
-    TileLoad<T, HD, CK, 256> kl, vl;
+    using Load = TileBuf<T, HD, CK, 256>;
+    Load kl, vl;
     const KeyTiles kt_ = key_tiles(end, part, parts);
-    const int ntile = kt_.end;
+    const int ntile = kt_.end, mine = min(ntile, (wave_end + CK - 1) / CK);    // (tiles that the wave's queries see)
     kl.place(s.k_sr, tid);
     vl.place(s.v_sr, tid);
-    if (kt_.first < ntile) {
-        kl.load(Kh, s.k_sr, kt_.first * CK, sq.nk, tid);
-        vl.load(Vh, s.v_sr, kt_.first * CK, sq.nk, tid);
-    }
-#pragma unroll 1
-    for (int tile = kt_.first; tile < ntile; ++tile) {
+    auto ask = [&](int tile) {
+        const int limit = tile < ntile ? sq.nk : 0;
+        kl.load(Load::rows(Kh, s.k_sr, tile * CK, limit), s.k_sr);
+        vl.load(Load::rows(Vh, s.v_sr, tile * CK, limit), s.v_sr);
+    };
+    auto put = [&](int tile) {
         uint8_t* kt = smem + (tile & 1) * 2 * TB;
-        uint8_t* vt = kt + TB;
-        kl.store(kt, tid);                                         // (the tile two before is done: barrier of the last step)
-        vl.store(vt, tid);
-        __syncthreads();
-        if (tile + 1 < ntile) {
-            kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
-            vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
-        }
+        kl.store(kt, tid);
+        vl.store(kt + TB, tid);
+    };
+    // A step multiplies S, forms the weights while the next tile goes from registers to LDS, and multiplies O while the one
+    // after it is asked for.  The order of the instructions is given: with loads and stores in front of the step
+    // 12001 tokens took 562 us, 523 so.
+    int tile = kt_.first;
+    ask(tile);
+    put(tile);
+    ask(tile + 1);
+#pragma unroll 1
+    for (; tile < mine; ++tile) {
+        const uint8_t *kt = smem + (tile & 1) * 2 * TB, *vt = kt + TB;
+        __syncthreads();                                           // the tile is there, the one before is done with
         const int key0 = tile * CK;
-        if (key0 >= wave_end) continue;                            // (wave-uniform)
 
         f32x4 sc[2][4];
 #pragma unroll
@@ -135,6 +141,12 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) sc[qb][kt4] = mfma16(kf[ks], qf[qb][ks], sc[qb][kt4]);
             }
+        }
+        __builtin_amdgcn_sched_group_barrier(SG_DS_READ, 4, 0);
+#pragma unroll
+        for (int j = 0; j < 4 * KS; ++j) {
+            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+            if (j + 4 < 4 * KS) __builtin_amdgcn_sched_group_barrier(SG_DS_READ, 1, 0);
         }
         if (key0 + CK > all_see) {                                 // (wave-uniform) some query does not see the whole tile
 #pragma unroll
@@ -165,8 +177,14 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
                 pf[qb][hf] = pack_b<T>(p[0], p[1]);
             }
         };
+        put(tile + 1);
         weights(0);
         weights(1);
+#pragma unroll
+        for (int i = 0; i < 2 * Load::N; ++i) {
+            __builtin_amdgcn_sched_group_barrier(SG_VALU, 16, 0);
+            __builtin_amdgcn_sched_group_barrier(SG_DS_WRITE, 1, 0);
+        }
         if (!__all(sum[0] < M_MOST && sum[1] < M_MOST)) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
@@ -193,6 +211,7 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
         }
         l[0] += sum[0];
         l[1] += sum[1];
+        ask(tile + 2);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -201,6 +220,19 @@ __global__ __launch_bounds__(256, 2) void causal_fwd_kernel(const T* __restrict_
 #pragma unroll
                 for (int qb = 0; qb < 2; ++qb) oacc[qb][nt] = mfma16(vf, pf[qb][hf], oacc[qb][nt]);
             }
+        __builtin_amdgcn_sched_group_barrier(SG_DS_READ, 8, 0);    // (two reads a fragment)
+#pragma unroll
+        for (int j = 0; j < 2 * NT; ++j) {
+            __builtin_amdgcn_sched_group_barrier(SG_MFMA, 2, 0);
+            if (j + 4 < 2 * NT) __builtin_amdgcn_sched_group_barrier(SG_DS_READ, 2, 0);
+            if (j % (NT / Load::N) == 0) __builtin_amdgcn_sched_group_barrier(SG_VMEM_READ, 1, 0);
+        }
+    }
+#pragma unroll 1
+    for (; tile < ntile; ++tile) {                                 // tiles for other waves
+        __syncthreads();
+        put(tile + 1);
+        ask(tile + 2);
     }
 
 #pragma unroll
