@@ -187,8 +187,8 @@ struct TileBuf {
     }
     // the rows from row0 on (at most (ROWS - 1) * 2^24 + HD * 2 bytes: row strides are below 2^23 values)
     __device__ static __forceinline__ auto rows(const T* g, int64_t sr, int row0, int limit) {
-        const int n = max(0, min(ROWS, limit - row0));
-        return __builtin_amdgcn_make_buffer_rsrc((void*)(g + (int64_t)row0 * sr), 0, n > 0 ? (n - 1) * (int)(sr * 2) + HD * 2 : 0, 0x00020000);
+        const int n = max(0, min(ROWS, limit - row0)), bytes = ((n - 1) * (int)(sr * 2) + HD * 2) & (-n >> 31);   // (no branch)
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(g + (int64_t)row0 * sr), 0, bytes, 0x00020000);
     }
     template <typename R>
     __device__ __forceinline__ void load(R rows, int64_t sr) {

@@ -12,6 +12,7 @@
 // transposed from the same copy (Tile in causal.h).  The softmax side has the query on the MFMA column, so maximum and
 // sum of a row are in-lane but for two shuffles, and the accumulator of S^T is, packed to 16 bits, the next operand.
 #include "causal.h"
+#include <type_traits>
 
 namespace star {
 
@@ -541,26 +542,25 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) acc[qb][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    TileLoad<T, HD, CK, 256> kl, vl;
+    using Load = TileBuf<T, HD, CK, 256>;
+    Load kl, vl;
     kl.place(s.k_sr, tid);
     vl.place(s.v_sr, tid);
-    if (ntile > 0) {
-        kl.load(Kh, s.k_sr, t0 * CK, sq.nk, tid);
-        vl.load(Vh, s.v_sr, t0 * CK, sq.nk, tid);
-    }
+    auto ask_k = [&](int tile) { kl.load(Load::rows(Kh, s.k_sr, tile * CK, tile < t1 ? sq.nk : 0), s.k_sr); };
+    auto ask_v = [&](int tile) { vl.load(Load::rows(Vh, s.v_sr, tile * CK, tile < t1 ? sq.nk : 0), s.v_sr); };
+    auto k_tile = [&](int tile) { return smem + (tile & 1) * 2 * TB; };
+    ask_k(t0);
+    ask_v(t0);
     if (ntile <= 2) {                                              // both tiles stay in LDS, each in its own half
         float d[2] = {0.f, 0.f};
 #pragma unroll 1
         for (int tile = 0; tile < ntile; ++tile) {
-            uint8_t* kt = smem + tile * 2 * TB;
-            uint8_t* vt = kt + TB;
+            uint8_t *kt = k_tile(tile), *vt = kt + TB;
             kl.store(kt, tid);
             vl.store(vt, tid);
             __syncthreads();
-            if (tile + 1 < ntile) {
-                kl.load(Kh, s.k_sr, CK, sq.nk, tid);
-                vl.load(Vh, s.v_sr, CK, sq.nk, tid);
-            }
+            ask_k(tile + 1);
+            ask_v(tile + 1);
 #pragma unroll 1
             for (int k4 = 0; k4 < 4; ++k4) {
                 f32x4 sc[2], dp[2];
@@ -597,10 +597,10 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
         const int i = w0 + 16 * qb + r16;
         if (g == 0 && i < sq.nq && part == 0) delta[(int64_t)h * s.lse_stride + sq.q0 + i] = dl[qb];
     }
-    auto step = [&](int tile, const uint8_t* kt, const uint8_t* vt) {
+    // one tile; `on`: the next one goes from registers to LDS and the one after it is asked for among the instructions
+    auto step = [&](int tile, auto masked, auto on) {
+        uint8_t *kt = k_tile(tile), *vt = kt + TB;
         const int key0 = tile * CK;
-        if (key0 >= wave_end) return;
-        const bool masked = key0 + CK > all_see;                   // (wave-uniform)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {                           // 32 keys at a time
             x4 ds[2][2];
@@ -619,29 +619,29 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
                         dp[qb] = mfma16(vf, gf[qb][ks], dp[qb]);
                     }
                 }
-#pragma unroll
-                for (int qb = 0; qb < 2; ++qb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        sc[qb][i] = __builtin_fmaf(sc[qb][i], c2, -l2[qb]);
-                        dp[qb][i] -= dl[qb];
-                    }
-                if (masked) {
-#pragma unroll
-                    for (int qb = 0; qb < 2; ++qb)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool vis = key0 + 32 * hf + 16 * k2 + 4 * g + i < lim[qb];
-                            sc[qb][i] = vis ? sc[qb][i] : -INFINITY;
-                            dp[qb][i] = vis ? dp[qb][i] : 0.f;
-                        }
+                if constexpr (on.value) {
+                    if (hf == 0 && k2 == 0) kl.store(k_tile(tile + 1), tid);
+                    if (hf == 0 && k2 == 1) vl.store(k_tile(tile + 1) + TB, tid);
                 }
 #pragma unroll
                 for (int qb = 0; qb < 2; ++qb) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) dp[qb][i] *= __builtin_amdgcn_exp2f(sc[qb][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        sc[qb][i] = __builtin_fmaf(sc[qb][i], c2, -l2[qb]);
+                        dp[qb][i] -= dl[qb];
+                        if constexpr (masked.value) {
+                            const bool vis = key0 + 32 * hf + 16 * k2 + 4 * g + i < lim[qb];
+                            sc[qb][i] = vis ? sc[qb][i] : -INFINITY;
+                            dp[qb][i] = vis ? dp[qb][i] : 0.f;
+                        }
+                        dp[qb][i] *= __builtin_amdgcn_exp2f(sc[qb][i]);
+                    }
                     ds[qb][k2] = pack4<T>(dp[qb]);
                 }
+            }
+            if constexpr (on.value) {
+                if (hf == 0) ask_k(tile + 2);
+                else ask_v(tile + 2);
             }
             x8 df[2];
 #pragma unroll
@@ -652,24 +652,38 @@ __global__ __launch_bounds__(256, 2) void causal_dq_kernel(const T* __restrict__
 #pragma unroll
                 for (int qb = 0; qb < 2; ++qb) acc[qb][nt] = mfma16(kf, df[qb], acc[qb][nt]);
             }
+            if (hf == 0) __builtin_amdgcn_sched_barrier(0);        // (the halves mixed: 1219 us for 8191 grouped tokens, 1176 so)
         }
     };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
     if (ntile <= 2) {
 #pragma unroll 1
-        for (int tile = 0; tile < ntile; ++tile) step(tile, smem + tile * 2 * TB, smem + tile * 2 * TB + TB);
+        for (int tile = 0; tile < min(ntile, (wave_end + CK - 1) / CK); ++tile) step(tile, yes, no);
     } else {
+        int tile = t0;
+        kl.store(k_tile(tile), tid);
+        vl.store(k_tile(tile) + TB, tid);
+        ask_k(tile + 1);
+        ask_v(tile + 1);
+        const int mine = min(t1, (wave_end + CK - 1) / CK), clear = min(mine, all_see / CK);   // tiles that the wave sees, sees whole
 #pragma unroll 1
-        for (int tile = t0; tile < t1; ++tile) {
-            uint8_t* kt = smem + (tile & 1) * 2 * TB;
-            uint8_t* vt = kt + TB;
-            kl.store(kt, tid);
-            vl.store(vt, tid);
+        for (; tile < clear; ++tile) {
             __syncthreads();
-            if (tile + 1 < t1) {
-                kl.load(Kh, s.k_sr, (tile + 1) * CK, sq.nk, tid);
-                vl.load(Vh, s.v_sr, (tile + 1) * CK, sq.nk, tid);
-            }
-            step(tile, kt, vt);
+            step(tile, no, yes);
+        }
+#pragma unroll 1
+        for (; tile < mine; ++tile) {
+            __syncthreads();
+            step(tile, yes, yes);
+        }
+#pragma unroll 1
+        for (; tile < t1; ++tile) {                                // tiles for other waves
+            __syncthreads();
+            kl.store(k_tile(tile + 1), tid);
+            vl.store(k_tile(tile + 1) + TB, tid);
+            ask_k(tile + 2);
+            ask_v(tile + 2);
         }
     }
 #pragma unroll
