@@ -952,9 +952,10 @@ __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __rest
 
 // Pieces of the walks of a launch of wgs workgroups, `longest` steps at most and `mean` on average (a causal walk is
 // anything up to the longest): steps of `per`, so that wgs * (mean / per + 1/2) pieces, which is what such walks come to, fill
-// the 512 places (two a CU) once.  From 320 workgroups on, and from 256 with walks of middle length, a walk in one piece is as good or better: two rounds of pieces
-// and the sums' way through memory cost what the idle CUs did.  Forward and backward, 8 heads of 128: one sequence of 1500
-// tokens 151 -> 95 us, 3000 tokens 294 -> 182, 5000 tokens (320 workgroups) 522 -> 384; 6 of 800 to 1300 (400) 162 -> 196.
+// the 512 places (two a CU) once.  From 320 workgroups on, and from 256 with walks of middle length, a walk in one piece
+// is as good or better: two rounds of pieces and the sums' way through memory cost what the idle CUs did.  Forward
+// and backward, 8 heads of 128: one sequence of 1500 tokens 137 -> 91 us, 3000 tokens 260 -> 170, 5000 tokens (320 workgroups)
+// 460 -> 352; 6 of 800 to 1300 (400) 147 -> 186.
 struct Pieces { int hp, pieces, per; };                            // parts by heads, pieces of the longest walk, steps of a piece
 static Pieces pieces(int hp, int64_t wgs, int64_t longest, int64_t mean, int least) {
     const int64_t room = 512 - wgs / 2;
@@ -969,18 +970,19 @@ static Pieces dq_pieces(const star_causal_shape* s) {
 }
 // By query heads: into 1 when the longest walk is short (under 16 tiles of 32 queries over all heads), or the key tiles
 // alone fill the 512 places once -- twice where walks go from 1 tile to 32 and more, which leave no balance to a
-// single round; otherwise into the fewest that do.  Forward and backward of 2 sequences of up to 622 tokens, 16 heads on
-// 2 of 96: 75 us, 217 in one part; 25 of up to 131, 32 heads on 4 of 64: 61 and 81; 8191 tokens, 16 heads on 4 of 128: 1223
-// for 1024 workgroups, 1422 for 512 -- and 1650 for as many pieces of the whole walk.
+// single round; otherwise into the fewest that do.  Forward and backward of 8191 tokens, 16 heads on 4 of 128: 1144 us for
+// 1024 workgroups, 1346 for 512 by heads, 1223 by steps alone; 2 sequences of up to 622, 16 heads on 2 of 96: 68 us, 217 in
+// one part.
 static Pieces dkv_pieces(const star_causal_shape* s) {
     const int grp = s->H / s->Hkv, walk = cdiv(s->max_q, CQ);
+    const int64_t wgs = (int64_t)s->n_k_tiles * s->Hkv, want = walk >= 32 ? 1024 : 512;
     int hp = 1;
     if ((int64_t)grp * walk >= 16)
-        while (hp < grp && (int64_t)s->n_k_tiles * s->Hkv * hp < (walk >= 32 ? 1024 : 512)) {
+        while (hp < grp && wgs * hp < want) {
             do ++hp; while (grp % hp);
         }
     const int64_t heads = grp / hp, mean = max(1, walk - cdiv(min(s->max_q, s->max_k), 2 * CQ));
-    return pieces(hp, (int64_t)s->n_k_tiles * s->Hkv * hp, heads * walk, heads * mean, 8);
+    return pieces(hp, wgs * hp, heads * walk, heads * mean, 8);
 }
 
 // ------------------------------------------------------------------------------------------------------ host side

@@ -537,6 +537,7 @@ CACHED = [  # lens, L, H, Hkv, hd, dtype, capacity
     ([60000] + [1] * 15, 1, 1, 1, 64, BF, 60032),             # more parts of a row than lanes
     ([300000], 1, 2, 1, 64, FP, 300032),                      # more than threads
     ([2150, 7] * 20, 1, 8, 8, 128, BF, 2176),                 # the card full without parts, long sequences cut all the same
+    ([2150 - 9 * i for i in range(40)], 2, 8, 8, 64, BF, 2176),     # much the same length: whole
     ([1500, 1], 8, 8, 1, 64, FP, 1536),                       # 64 rows: cut from 1024 tokens of capacity on
     ([64 * (i % 9) + i for i in range(70)], 1, 2, 2, 64, BF, 640),   # more sequences than lanes
 ]
