@@ -274,15 +274,18 @@ __device__ __forceinline__ f16x8 widen<_Float16>(uint32_t lo, uint32_t hi, float
 template <typename T> struct VHalf { static constexpr float by = 1.f; };
 template <> struct VHalf<_Float16> { static constexpr float by = 0.5f; };
 
-// The codes are read once: past the caches (four sequences of up to 131072 tokens, 1.0 GB: 183 -> 161 us)
-template <typename V>
-__device__ __forceinline__ V once(const V* p) { return __builtin_nontemporal_load(p); }
+// Codes that one workgroup alone reads pass the caches by (four sequences of up to 131072 tokens, 1.0 GB: 183 -> 161 us)
+template <bool ONCE, typename V>
+__device__ __forceinline__ V codes(const V* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+}
 
 // Wave w of a workgroup takes the blocks w, w + 4, ... of its part for RT * 16 rows (a row is one query of one head of
 // the group); the four softmax states are joined through LDS at the end.  Token of the MFMA: row rho of K tile t is
 // token 16 * (rho / 4) + 4 t + rho % 4, so lane group g ends up with the weights of the tokens 16 g .. 16 g + 15, which
 // are the 16 bytes it loads from each row of V.
-template <typename T, int HD, int RT>
+template <typename T, int HD, int RT, bool ONCE>
 __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int KS = HD / 32, NT = HD / 16, C64 = HD / 64;
@@ -420,11 +423,11 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int cc = 0; cc < C64; ++cc) kr[t][cc] = once((const u32x4*)(kb + (krow + 4 * t) * HD + 64 * cc + 16 * g));
-            if constexpr (ODD) ko[t] = once((const u32x2*)(kb + (krow + 4 * t) * HD + 64 * C64 + 8 * g));
+            for (int cc = 0; cc < C64; ++cc) kr[t][cc] = codes<ONCE>((const u32x4*)(kb + (krow + 4 * t) * HD + 64 * cc + 16 * g));
+            if constexpr (ODD) ko[t] = codes<ONCE>((const u32x2*)(kb + (krow + 4 * t) * HD + 64 * C64 + 8 * g));
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) vr[nt] = once((const u32x4*)(vb + (16 * nt + r16) * KB + 16 * g));
+        for (int nt = 0; nt < NT; ++nt) vr[nt] = codes<ONCE>((const u32x4*)(vb + (16 * nt + r16) * KB + 16 * g));
         ks_ = ksc[blk];
         vs_ = vsc[blk];
     };
@@ -657,24 +660,27 @@ static int check_cache(const star_kv8_cache* c, const char* who) {
     return STAR_OK;
 }
 
-// rows of one workgroup: 16 while they suffice, else as many as keep the codes' conversion cheap against the products
-static int row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// tiles of 16 rows of one workgroup.  Four would read and convert the codes half as often, with one wave a SIMD and, at head
+// dim 128, half of the state in accumulation registers: 25 sequences of up to 15442 tokens, 40 rows a key head of 64, 177 us
+// with four and 131 with two; 16 of 2000, 64 rows of 128, 43 and 25; four of up to 131072, 64 rows of 128, 199 and 209.
+static int row_tiles(int rows) { return rows <= 16 ? 1 : 2; }
 // (sequence, part) pairs that the grid has room for.  512 workgroups (two a CU) run at once, 256 where the rows take a
-// whole CU's registers: few sequences are cut into parts that fill these places once (8 queries, 64 rows a key head of 64,
-// over 32000 tokens: 32 us with 512 workgroups, 20 with 256); where the sequences alone make half of them or more, there is
+// whole CU's registers: few sequences are cut into parts that fill these places once (four of 8000 tokens, 64 rows a key
+// head of 128: 36 us with 512 workgroups, 25 with 256); where the sequences alone make half of them or more, there is
 // room for three times as many parts besides, so that a sequence much longer than the others does not run alone at the end.
 // Sequences that fill three quarters of the places and of which none is longer than 1.5 times their mean stay whole (53
 // of 2590 to 2908 tokens, 8 key heads of 128, 5 queries: 97 us in parts, 73 whole).
 // A part has 4 blocks (256 tokens) at least, one per wave, or 24 where the card is full without it.  The join is a launch of
 // its own, 3.4 us, which a short cache does not repay (one query, 8 heads of 128: 10.1 us whole and 12.5 in parts for 1024
-// tokens, 15.0 and 12.9 for 1536, 204 and 21 for 32000; 64 rows a key head of 64: 17.2 and 17.4 for 1024).
+// tokens, 15.0 and 12.9 for 1536, 204 and 21 for 32000; 64 rows a key head of 64: 12.1 and 13.4
+// for 1280, 16.8 and 13.5 for 2048).
 struct Cut { int slots, min_part, even; };
 static Cut attn_cut(const star_kv8_cache* c, int H, int L) {
     const int rows = H / c->Hkv * L, rt = row_tiles(rows), nrg = cdiv(rows, 16 * rt), blocks = c->T / KB;
     const int64_t places = (rt * c->hd <= 192 ? 512 : 256) / ((int64_t)c->Hkv * nrg);
     const bool full = places < 2 * c->B;
     const int min_part = full ? 24 : 4;
-    if (full ? blocks <= 32 : blocks * c->hd <= (rt == 4 ? 8 : 18) * 128) return Cut{c->B, min_part, 0};
+    if (full ? blocks <= 32 : rt == 1 ? blocks * c->hd <= 18 * 128 : blocks <= 22) return Cut{c->B, min_part, 0};
     const int64_t most = (int64_t)c->B * cdiv(blocks, min_part), s = full ? c->B + 3 * (places > 1 ? places : 1) : places;
     return Cut{(int)(s < most ? s : most), min_part, 4 * c->B >= 3 * places};
 }
@@ -695,9 +701,9 @@ static Cut attn_cut(const star_kv8_cache* c, int H, int L) {
 template <typename T, int HD>
 static void launch_attn(const AttnArgs& a, int rt, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.slots * a.c.Hkv * a.nrg));
-    if (rt == 1) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 1>), grid, dim3(256), 0, st, a);
-    else if (rt == 2) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 4>), grid, dim3(256), 0, st, a);
+    if (rt == 1) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 1, true>), grid, dim3(256), 0, st, a);
+    else if (a.nrg == 1) hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 2, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_attn_kernel<T, HD, 2, false>), grid, dim3(256), 0, st, a);
     if (a.slots == a.c.B) return;
     // (one wave has 16 parts, 32 at hd 64, on their way at once: up to 32 the two take the same time, beyond it 64 parts 1 us more)
     const int64_t rows = (int64_t)a.c.B * a.s.H * a.s.L;

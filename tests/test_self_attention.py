@@ -530,7 +530,7 @@ CACHED = [  # lens, L, H, Hkv, hd, dtype, capacity
     ([375], 1, 8, 8, 128, BF, 384),
     ([0, 1, 63, 64, 65, 129], 1, 4, 2, 64, BF, 192),
     ([700, 64, 5, 1023], 3, 6, 2, 96, FP, 1024),
-    ([2000, 17], 16, 8, 1, 128, BF, 2048),                    # 128 rows: four tiles of 16 in a workgroup, two groups
+    ([2000, 17], 16, 8, 1, 128, BF, 2048),                    # 128 rows: two tiles of 16 in a workgroup, four groups
     ([300, 64], 5, 12, 2, 64, FP, 320),                       # 30 rows: two tiles
     ([5000, 4096, 100], 1, 32, 8, 128, FP, 5056),             # cut into parts and joined
     ([30000], 2, 2, 1, 96, BF, 30016),
@@ -538,7 +538,7 @@ CACHED = [  # lens, L, H, Hkv, hd, dtype, capacity
     ([300000], 1, 2, 1, 64, FP, 300032),                      # more than threads
     ([2150, 7] * 20, 1, 8, 8, 128, BF, 2176),                 # the card full without parts, long sequences cut all the same
     ([2150 - 9 * i for i in range(40)], 2, 8, 8, 64, BF, 2176),     # much the same length: whole
-    ([1500, 1], 8, 8, 1, 64, FP, 1536),                       # 64 rows: cut from 1024 tokens of capacity on
+    ([1500, 1], 8, 8, 1, 64, FP, 1536),                       # 64 rows: cut from 23 blocks of capacity on
     ([64 * (i % 9) + i for i in range(70)], 1, 2, 2, 64, BF, 640),   # more sequences than lanes
 ]
 
