@@ -291,6 +291,9 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
     constexpr int KS = HD / 32, NT = HD / 16, C64 = HD / 64;
     constexpr bool ODD = HD % 64 != 0;                              // head dim 96: 64 + 32
     constexpr int OP = HD + 4;
+    // 32 rows of 128: V is widened only where it is used and the next block's V asked for after that, 60 registers fewer, so that
+    // two waves fit a SIMD (four sequences of up to 131072 tokens, 64 rows: 210 -> 189 us; 16 rows, 161 -> 163, are not)
+    constexpr bool LATE = RT * HD > 192;
     __shared__ __attribute__((aligned(16))) float osh[4 * 16 * OP];
     __shared__ float msh[4 * 16], lsh[4 * 16];
 
@@ -417,22 +420,27 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
     u32x4 kr[4][C64], vr[NT];
     u32x2 ko[4];
     float ks_ = 0.f, vs_ = 0.f;
-    auto load = [&](int blk) {
+    auto load_k = [&](int blk) {
         const uint8_t* kb = kc + (int64_t)blk * KB * HD;
-        const uint8_t* vb = vc + (int64_t)blk * KB * HD;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int cc = 0; cc < C64; ++cc) kr[t][cc] = codes<ONCE>((const u32x4*)(kb + (krow + 4 * t) * HD + 64 * cc + 16 * g));
             if constexpr (ODD) ko[t] = codes<ONCE>((const u32x2*)(kb + (krow + 4 * t) * HD + 64 * C64 + 8 * g));
         }
+        ks_ = ksc[blk];
+    };
+    auto load_v = [&](int blk) {
+        const uint8_t* vb = vc + (int64_t)blk * KB * HD;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) vr[nt] = codes<ONCE>((const u32x4*)(vb + (16 * nt + r16) * KB + 16 * g));
-        ks_ = ksc[blk];
         vs_ = vsc[blk];
     };
     const int full1 = min(blk1, open);                              // complete blocks end here
-    if (blk0 + wid < full1) load(blk0 + wid);
+    if (blk0 + wid < full1) {
+        load_k(blk0 + wid);
+        load_v(blk0 + wid);
+    }
 #pragma unroll 1
     for (int blk = blk0 + wid; blk < full1; blk += 4) {
         f32x4 sc[RT][4];
@@ -452,23 +460,30 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
                 for (int ks = 0; ks < KS; ++ks) sc[rt][t] = mfma16(kf[ks], qf[rt][ks], sc[rt][t]);
             }
         }
-        x8 vf[NT][2];
-        const float vs = vs_ * VHalf<T>::by, kscale = ks_ * c2;
+        const float kscale = ks_ * c2, vs = vs_ * VHalf<T>::by;
+        auto v_half = [&](int nt, int hf) { return widen<T>(vr[nt][2 * hf], vr[nt][2 * hf + 1], vs); };
+        x8 vf[LATE ? 1 : NT][2];
+        if constexpr (!LATE) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            vf[nt][0] = widen<T>(vr[nt][0], vr[nt][1], vs);
-            vf[nt][1] = widen<T>(vr[nt][2], vr[nt][3], vs);
+            for (int nt = 0; nt < NT; ++nt) vf[nt][0] = v_half(nt, 0), vf[nt][1] = v_half(nt, 1);
         }
-        if (blk + 4 < full1) load(blk + 4);                         // in flight during the softmax and the product with V
+        if (blk + 4 < full1) {                                      // in flight during the softmax and the product with V
+            load_k(blk + 4);
+            if constexpr (!LATE) load_v(blk + 4);
+        }
         x8 pf[RT][2];
         softmax(sc, kscale, blk, pf);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                acc[rt][nt] = mfma16(vf[nt][0], pf[rt][0], acc[rt][nt]);
-                acc[rt][nt] = mfma16(vf[nt][1], pf[rt][1], acc[rt][nt]);
+            for (int hf = 0; hf < 2; ++hf) {
+                const x8 v = LATE ? v_half(nt, hf) : vf[LATE ? 0 : nt][hf];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][nt] = mfma16(v, pf[rt][hf], acc[rt][nt]);
             }
+        if constexpr (LATE) {
+            if (blk + 4 < full1) load_v(blk + 4);
+        }
     }
     if (open < blk1 && open >= blk0 && (open - blk0) % 4 == wid) {  // the open block, in 16 bits
         const T* kt = (const T*)c.k_tail + bh * KB * HD;
@@ -662,12 +677,13 @@ static int check_cache(const star_kv8_cache* c, const char* who) {
 
 // tiles of 16 rows of one workgroup.  Four would read and convert the codes half as often, with one wave a SIMD and, at head
 // dim 128, half of the state in accumulation registers: 25 sequences of up to 15442 tokens, 40 rows a key head of 64, 177 us
-// with four and 131 with two; 16 of 2000, 64 rows of 128, 43 and 25; four of up to 131072, 64 rows of 128, 199 and 209.
+// with four and 131 with two; 16 of 2000, 64 rows of 128, 43 and 26; four of up to 131072, 64 rows of 128, 199 and 189.
 static int row_tiles(int rows) { return rows <= 16 ? 1 : 2; }
-// (sequence, part) pairs that the grid has room for.  512 workgroups (two a CU) run at once, 256 where the rows take a
-// whole CU's registers: few sequences are cut into parts that fill these places once (four of 8000 tokens, 64 rows a key
-// head of 128: 36 us with 512 workgroups, 25 with 256); where the sequences alone make half of them or more, there is
-// room for three times as many parts besides, so that a sequence much longer than the others does not run alone at the end.
+// (sequence, part) pairs that the grid has room for.  512 workgroups (two a CU) run at once: few sequences are cut into
+// parts that fill these places once; where the sequences alone make half of them or more, there is room for three times
+// as many parts besides, so that a sequence much longer than the others does not run alone at the end.  32 rows of 128 keep a
+// CU busy almost alone, so that for them half of the places counts as all (40 sequences of 2000 tokens, 64 rows: 26 us
+// whole, 30 in parts).
 // Sequences that fill three quarters of the places and of which none is longer than 1.5 times their mean stay whole (53
 // of 2590 to 2908 tokens, 8 key heads of 128, 5 queries: 97 us in parts, 73 whole).
 // A part has 4 blocks (256 tokens) at least, one per wave, or 24 where the card is full without it.  The join is a launch of
@@ -677,12 +693,12 @@ static int row_tiles(int rows) { return rows <= 16 ? 1 : 2; }
 struct Cut { int slots, min_part, even; };
 static Cut attn_cut(const star_kv8_cache* c, int H, int L) {
     const int rows = H / c->Hkv * L, rt = row_tiles(rows), nrg = cdiv(rows, 16 * rt), blocks = c->T / KB;
-    const int64_t places = (rt * c->hd <= 192 ? 512 : 256) / ((int64_t)c->Hkv * nrg);
-    const bool full = places < 2 * c->B;
+    const int64_t places = 512 / ((int64_t)c->Hkv * nrg), fill = rt * c->hd > 192 ? places / 2 : places;
+    const bool full = fill < 2 * c->B;
     const int min_part = full ? 24 : 4;
     if (full ? blocks <= 32 : rt == 1 ? blocks * c->hd <= 18 * 128 : blocks <= 22) return Cut{c->B, min_part, 0};
     const int64_t most = (int64_t)c->B * cdiv(blocks, min_part), s = full ? c->B + 3 * (places > 1 ? places : 1) : places;
-    return Cut{(int)(s < most ? s : most), min_part, 4 * c->B >= 3 * places};
+    return Cut{(int)(s < most ? s : most), min_part, 4 * c->B >= 3 * fill};
 }
 
 #define KV8_BY_TYPE(DT, HDIM, CALL)                                                        \
