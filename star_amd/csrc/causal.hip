@@ -969,13 +969,14 @@ static Pieces dq_pieces(const star_causal_shape* s) {
     return pieces(1, (int64_t)s->n_q_tiles * s->H, n, max((int64_t)1, n - cdiv(min(s->max_q, s->max_k), CT)), 4);
 }
 // By query heads: into 1 when the longest walk is short (under 16 tiles of 32 queries over all heads), or the key tiles
-// alone fill the 512 places once -- twice where walks go from 1 tile to 32 and more, which leave no balance to a
-// single round; otherwise into the fewest that do.  Forward and backward of 8191 tokens, 16 heads on 4 of 128: 1144 us for
-// 1024 workgroups, 1346 for 512 by heads, 1223 by steps alone; 2 sequences of up to 622, 16 heads on 2 of 96: 68 us, 217 in
+// alone give every CU a workgroup -- two from walks of 16 tiles a head on, four from 32, which go from 1 tile to 32 and more
+// and leave no balance to a single round; otherwise into the fewest that do.  Forward and backward of 8191 tokens, 16
+// heads on 4 of 128: 1144 us for 1024 workgroups, 1346 for 512 by heads, 1223 by steps alone; 4 sequences of 500 to 900, 32 on
+// 4 of 128: 155 for 512, 183 for 256; 53 of 200 to 210, 8 on 2 of 128: 126 and 113; 2 of up to 622, 16 on 2 of 96: 68, 217 in
 // one part.
 static Pieces dkv_pieces(const star_causal_shape* s) {
     const int grp = s->H / s->Hkv, walk = cdiv(s->max_q, CQ);
-    const int64_t wgs = (int64_t)s->n_k_tiles * s->Hkv, want = walk >= 32 ? 1024 : 512;
+    const int64_t wgs = (int64_t)s->n_k_tiles * s->Hkv, want = walk >= 32 ? 1024 : walk >= 16 ? 512 : 256;
     int hp = 1;
     if ((int64_t)grp * walk >= 16)
         while (hp < grp && wgs * hp < want) {
