@@ -534,6 +534,9 @@ class NuggetSelfAttention(nn.Module):
         self.resid_dropout = nn.Dropout(resid_pdrop)
         self._plan = None            # ((B, T, device), plan) of the last unpadded batch
 
+    def __getstate__(self):
+        return {**self.__dict__, "_plan": None}         # (a copied or saved module makes its plans itself)
+
     def new_cache(self, batch: int, max_tokens: int, device=None, dtype=torch.bfloat16):
         """An empty 8-bit cache for this layer."""
         return ops.KVCache8(batch, self.kv_heads, max_tokens, self.head_dim, device or self.c_attn.weight.device, dtype)

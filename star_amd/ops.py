@@ -1682,14 +1682,29 @@ class PackedSeqs:
         kt = tiles(nk, lambda s, j: nq[s] - np.clip(j - (nk[s] - nq[s]), 0, nq[s]))
         seqs = np.stack([q0, nq, k0, nk], 1)
         flat = np.concatenate([qt.ravel(), kt.ravel(), seqs.ravel()]).astype(np.int32)
-        buf = torch.from_numpy(flat).to(device)
+        self._buf, self._cuts = torch.from_numpy(flat).to(device), (qt.size, qt.size + kt.size)
+        self._views()
+
+    def _views(self):
+        """The parts of the one device buffer, and where they lie."""
+        buf, (a, b) = self._buf, self._cuts
         self.device = buf.device
-        a, b = qt.size, qt.size + kt.size
         self.q_tiles, self.k_tiles, self.seqs = buf[:a].view(-1, 8), buf[a:b].view(-1, 8), buf[b:].view(-1, 4)
         self.starts, self.counts = self.seqs[:, 2], self.seqs[:, 3]
-        self.n_q_tiles, self.n_k_tiles = len(qt), len(kt)
+        self.n_q_tiles, self.n_k_tiles = len(self.q_tiles), len(self.k_tiles)
         self.q_tiles_ptr, self.k_tiles_ptr = self.q_tiles.data_ptr(), self.k_tiles.data_ptr()
         self.starts_ptr, self.counts_ptr = self.starts.data_ptr(), self.counts.data_ptr()
+
+    _OF_BUFFER = ("device", "q_tiles", "k_tiles", "seqs", "starts", "counts", "n_q_tiles", "n_k_tiles",
+                  "q_tiles_ptr", "k_tiles_ptr", "starts_ptr", "counts_ptr")
+
+    # (a copy or a loaded plan has a buffer of its own: its addresses are formed from that)
+    def __getstate__(self):
+        return {n: x for n, x in self.__dict__.items() if n not in self._OF_BUFFER}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._views()
 
 
 def _rows_like(rows, used, heads, hd, t):
