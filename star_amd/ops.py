@@ -1733,7 +1733,9 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
     """Gradients into dq, dk and dv, whose rows are s.dq_sr and s.dkv_sr values apart."""
     if torch.is_grad_enabled():
         raise _lib.StarNuggetError("causal_attn has no second derivative (backward with create_graph=True)")
-    g = g.to(q.dtype).contiguous()
+    if g.dtype != q.dtype:
+        g = g.to(q.dtype)
+    g = g.contiguous()
     if g.data_ptr() % 16:
         g = g.clone()
     delta = torch.empty_like(lse)
@@ -1745,6 +1747,22 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
             ptr(ws), need)
 
 
+def _causal_saved(ctx, q, k, v, o, lse):
+    """The shape, o and lse for the backward, from the tensors that autograd gives back: hooks on saved tensors (offload,
+    compression) return a view with gaps as a dense tensor, whose strides are not those of the forward's shape."""
+    s, plan = ctx.s, ctx.plan
+    dev, n_q, n_k = plan.device, s.lse_stride * s.H, s.k_rows * s.Hkv * s.hd
+    if not (q.device == k.device == v.device == o.device == lse.device == dev and _DT16.get(q.dtype) == s.dtype
+            and q.dtype == k.dtype == v.dtype == o.dtype and lse.dtype == torch.float32 and lse.numel() == n_q
+            and q.numel() == o.numel() == n_q * s.hd and k.numel() == v.numel() == n_k):
+        raise ValueError("causal_attn: saved tensors came back with another type, size or device")
+    if ctx.strides != (q.stride(), k.stride(), v.stride()):
+        was, s = s, _causal_layout(q, k, v, plan, s.scale)
+        if (s.H, s.Hkv, s.hd) != (was.H, was.Hkv, was.hd):
+            raise ValueError("causal_attn: saved tensors came back with another shape")
+    return s, o.contiguous(), lse.contiguous()
+
+
 class _CausalAttn(torch.autograd.Function):
     """softmax(scale Q K^T, j <= i + nk - nq) V of packed sequences."""
 
@@ -1752,7 +1770,7 @@ class _CausalAttn(torch.autograd.Function):
     def forward(ctx, q, k, v, plan, s, need_lse):
         o, lse = _causal_forward(q, k, v, plan, s, True)
         ctx.save_for_backward(q, k, v, o, lse)
-        ctx.plan, ctx.s = plan, s
+        ctx.plan, ctx.s, ctx.strides = plan, s, (q.stride(), k.stride(), v.stride())
         if not need_lse:
             return o
         ctx.mark_non_differentiable(lse)
@@ -1761,9 +1779,12 @@ class _CausalAttn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g, _=None):
         q, k, v, o, lse = ctx.saved_tensors
-        plan, s = ctx.plan, ctx.s
-        dq = _rows_like(s.lse_stride, plan.q_used, s.H, s.hd, q)
-        dk, dv = (_rows_like(s.k_rows, plan.k_used, s.Hkv, s.hd, t) for t in (k, v))
+        plan = ctx.plan
+        s, o, lse = _causal_saved(ctx, q, k, v, o, lse)
+        make = torch.empty_like if s.lse_stride == plan.q_used else torch.zeros_like       # (rows in no sequence are 0)
+        dq = make(o)
+        make = torch.empty_like if s.k_rows == plan.k_used else torch.zeros_like
+        dk, dv = make(k, memory_format=torch.contiguous_format), make(v, memory_format=torch.contiguous_format)
         s.dq_sr, s.dkv_sr = s.H * s.hd, s.Hkv * s.hd
         _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv)
         return dq, dk, dv, None, None, None
@@ -1777,16 +1798,18 @@ class _CausalAttnQKV(torch.autograd.Function):
     def forward(ctx, qkv, views, plan, s):
         o, lse = _causal_forward(*views, plan, s, True)
         ctx.save_for_backward(qkv, o, lse)
-        ctx.plan, ctx.s = plan, s
+        ctx.plan, ctx.s, ctx.strides = plan, s, tuple(t.stride() for t in views)
         return o
 
     @staticmethod
     def backward(ctx, g):
         qkv, o, lse = ctx.saved_tensors
         plan, s = ctx.plan, ctx.s
+        views = _qkv_views(qkv, s.H, s.Hkv, s.hd)
+        s, o, lse = _causal_saved(ctx, *views, o, lse)
         d = _rows_like(s.lse_stride, plan.q_used, s.H + 2 * s.Hkv, s.hd, qkv)
         s.dq_sr = s.dkv_sr = (s.H + 2 * s.Hkv) * s.hd
-        _causal_backward(g, *_qkv_views(qkv, s.H, s.Hkv, s.hd), o, lse, plan, s, *_qkv_views(d.flatten(1), s.H, s.Hkv, s.hd))
+        _causal_backward(g, *views, o, lse, plan, s, *_qkv_views(d.flatten(1), s.H, s.Hkv, s.hd))
         return d.flatten(1), None, None, None
 
 
@@ -1836,6 +1859,10 @@ def _causal_shape(q, k, v, plan, scale):
     if not (k.device == dev == v.device == plan.device and q.is_cuda):
         dev = _same_device("causal_attn", q=q, k=k, v=v)
         raise ValueError(f"causal_attn: the plan is on {plan.device}, the tensors on {dev}")
+    return _causal_layout(q, k, v, plan, scale)
+
+
+def _causal_layout(q, k, v, plan, scale):
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"causal_attn: [rows, heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     rows, H, hd = q.shape
