@@ -23,12 +23,14 @@ Everything runs in the HIP kernels of libstar_nugget.so; there is no CPU path.
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional
 
 import torch
 from torch import nn
 
 from . import ops
+from ._lib import StarNuggetError
 
 
 # ------------------------------------------------------------------------------------------ a1
@@ -507,7 +509,9 @@ class NuggetSelfAttention(nn.Module):
 
     The core runs on 16-bit operands with fp32 softmax and sums, as NuggetCrossAttention's does: fp32 activations are
     rounded to bfloat16 for it.  The softmax is never padded, so no additive attention_mask is taken: give the lengths.
-    The plan of an unpadded or padded batch is made at its first call: make that before a HIP-graph capture.
+    The plan of an unpadded or padded batch is made at its first call: make that before a HIP-graph capture (a new shape is
+    refused in one).  Plans of unpadded batches are kept for the last 32 shapes, and as long as the module for a shape that
+    was captured, since a graph reads its plan at every replay.
 
         attn(x)                                  x [B,T,d], every row T frames
         attn(x, valid=frames)                    x [B,T,d] padded, frames an ops.ValidFrames; pad rows see nothing
@@ -532,10 +536,36 @@ class NuggetSelfAttention(nn.Module):
         self.c_attn = Conv1D((num_heads + 2 * self.kv_heads) * self.head_dim, hidden_size)
         self.c_proj = Conv1D(hidden_size, hidden_size)
         self.resid_dropout = nn.Dropout(resid_pdrop)
-        self._plan = None            # ((B, T, device), plan) of the last unpadded batch
+        self._plans, self._captured = {}, {}     # (B, T, device) -> (plan, streams it was used on): unpadded batches
 
     def __getstate__(self):
-        return {**self.__dict__, "_plan": None}         # (a copied or saved module makes its plans itself)
+        return {**self.__dict__, "_plans": {}, "_captured": {}}     # (a copied or saved module makes its plans itself)
+
+    _PLANS, _LOCK = 32, threading.Lock()
+
+    def _plan_of(self, B, T, device):
+        """The plan of B sequences of T frames.  One that is dropped from _plans may still be read by work on any stream it was
+        used on, which is recorded for the allocator; one that a capture has seen is never dropped."""
+        key = (B, T, device)
+        kept, capture = self._captured.get(key) or self._plans.get(key), ops.capturing(device)
+        if kept is None:
+            if capture:
+                raise StarNuggetError(f"NuggetSelfAttention: call it once with [{B},{T},{self.embed_dim}] before a HIP-graph "
+                                      "capture (the plan of a new shape is copied to the device)")
+            kept = ops.PackedSeqs([T] * B, device), set()
+            with self._LOCK:
+                while len(self._plans) >= self._PLANS:
+                    self._plans.pop(next(iter(self._plans)))
+                self._plans[key] = kept
+        plan, streams = kept
+        if capture:
+            self._captured[key] = kept
+        elif plan.device.type == "cuda":
+            raw = ops._raw_stream(plan.device.index)
+            if raw not in streams:
+                plan.record_stream(torch.cuda.current_stream(plan.device))
+                streams.add(raw)
+        return plan
 
     def new_cache(self, batch: int, max_tokens: int, device=None, dtype=torch.bfloat16):
         """An empty 8-bit cache for this layer."""
@@ -555,10 +585,7 @@ class NuggetSelfAttention(nn.Module):
                     raise ValueError(f"NuggetSelfAttention: valid is for [{valid.B},{valid.T},d], got {tuple(hidden_states.shape)}")
                 plan = valid.seqs()
             else:
-                key = (B, T, hidden_states.device)
-                if self._plan is None or self._plan[0] != key:
-                    self._plan = (key, ops.PackedSeqs([T] * B, hidden_states.device))
-                plan = self._plan[1]
+                plan = self._plan_of(B, T, hidden_states.device)
         elif valid is not None:
             raise ValueError("NuggetSelfAttention: give plan or valid, not both")
         qkv = self.c_attn(hidden_states).reshape(-1, self.c_attn.nf)

@@ -1573,6 +1573,16 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def capturing(dev) -> bool:
+    """Whether the current stream of dev is being captured into a graph."""
+    if dev.type != "cuda":
+        return False
+    if dev.index is None or _current_device() == dev.index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(dev.index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _launch(fn, what, dev, *args):
     """fn(*args, the current stream of dev), with dev as the current device for the launch."""
     index = dev.index
@@ -1626,6 +1636,10 @@ class PackedSeqs:
 
     lengths: keys of every sequence.  q_lengths: its queries where there are fewer (they are the newest positions: query
     i sees the keys j <= i + lengths[s] - q_lengths[s]); more queries than keys are allowed, the first then see nothing.
+    A captured graph reads the plan's buffer at every replay: keep the plan as long as the graph.  A plan that is used on
+    another stream than the one it was made on and dropped while that work may still run needs record_stream, as
+    tensors do.
+
     Sequences lie one behind the other; with padded_to=T sequence s starts at row s * T instead (a padded [B,T] batch,
     flattened), for the queries too; k_starts gives the first key row of every sequence instead (two sequences may then
     have rows in common, such as the same prompt; causal_attn refuses the gradients of such rows)."""
@@ -1694,6 +1708,10 @@ class PackedSeqs:
         self.n_q_tiles, self.n_k_tiles = len(self.q_tiles), len(self.k_tiles)
         self.q_tiles_ptr, self.k_tiles_ptr = self.q_tiles.data_ptr(), self.k_tiles.data_ptr()
         self.starts_ptr, self.counts_ptr = self.starts.data_ptr(), self.counts.data_ptr()
+
+    def record_stream(self, stream):
+        """torch.Tensor.record_stream for the plan's buffer."""
+        self._buf.record_stream(stream)
 
     _OF_BUFFER = ("device", "q_tiles", "k_tiles", "seqs", "starts", "counts", "n_q_tiles", "n_k_tiles",
                   "q_tiles_ptr", "k_tiles_ptr", "starts_ptr", "counts_ptr")

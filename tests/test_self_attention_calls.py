@@ -2,8 +2,12 @@
 in another layout, plans that captured graphs still read, tangents, padded prompts into a cache, empty batches, full
 caches.  Tolerances are those of test_self_attention.py, whose formulas are used."""
 import copy
+import gc
 import io
 import pickle
+import sys
+import threading
+import weakref
 
 import pytest
 import torch
@@ -56,7 +60,12 @@ def test_a_copied_module_leaves_the_plan_behind(ops, how):
     with pytest.raises(ops.StarDeviceError):                   # (the plan is made before the tensors are refused)
         m(torch.zeros(2, 5, 128))
     theirs = COPIES[how](m)
-    assert not any(isinstance(x, ops.PackedSeqs) for v in vars(theirs).values() for x in (v.values() if isinstance(v, dict) else v if isinstance(v, tuple) else [v]))
+
+    def plans(x):
+        parts = x.values() if isinstance(x, dict) else x if isinstance(x, (tuple, list)) else ()
+        return isinstance(x, ops.PackedSeqs) or any(plans(y) for y in parts)
+
+    assert plans(vars(m)) and not plans(vars(theirs))
     for a, b in zip(m.parameters(), theirs.parameters()):
         assert torch.equal(a, b) and a is not b
 
@@ -149,3 +158,108 @@ def test_gradients_of_views_under_save_on_cpu(ops, H, Hkv, whole):
     with torch.autograd.graph.save_on_cpu():
         o2, g2 = step()
     assert torch.equal(o, o2) and torch.equal(g, g2)
+
+
+# ------------------------------------------------------------------------------------------------------ kept plans
+def recording(monkeypatch, ops, seen):
+    """A module on the CPU whose core only records the plan that it was given."""
+    from star_amd import NuggetSelfAttention
+
+    def core(qkv, H, Hkv, plan, scale=None):
+        seen.append(weakref.ref(plan))
+        assert plan.q_rows == len(qkv), "a plan of other lengths"
+        return qkv[:, :128].view(-1, 2, 64)
+
+    monkeypatch.setattr(ops, "causal_attn_qkv", core)
+    return NuggetSelfAttention(128, 2).eval()
+
+
+def test_a_captured_shape_keeps_its_plan(ops, monkeypatch):
+    """A graph reads the plan's buffer at every replay: calls of other shapes between the replays must not free it."""
+    seen = []
+    m = recording(monkeypatch, ops, seen)
+    x = torch.zeros(2, 5, 128)
+    with torch.no_grad():
+        m(x)
+        monkeypatch.setattr(ops, "capturing", lambda dev: True, raising=False)
+        m(x)
+        monkeypatch.setattr(ops, "capturing", lambda dev: False)
+        for t in range(6, 80):
+            m(torch.zeros(1, t, 128))
+        gc.collect()
+        assert seen[1]() is not None and seen[0]() is seen[1]()
+        m(x)
+        assert seen[-1]() is seen[1]()
+        assert sum(r() is not None for r in seen[2:-1]) <= 32 and seen[-2]() is not None       # the others are bounded
+        monkeypatch.setattr(ops, "capturing", lambda dev: True)
+        with pytest.raises(RuntimeError, match="before a HIP-graph capture"):
+            m(torch.zeros(7, 3, 128))
+
+
+def test_threads_with_different_shapes_get_their_own_plans(ops, monkeypatch):
+    seen, failed = [], []
+    m = recording(monkeypatch, ops, seen)
+
+    def work(t):
+        try:
+            with torch.no_grad():
+                for _ in range(300):
+                    m(torch.zeros(1, t, 128))
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    every = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(t,)) for t in (3, 4, 5, 6)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(every)
+    assert not failed, failed[:1]
+
+
+@gpu
+def test_a_captured_module_replays_after_calls_of_other_shapes(ops):
+    """Forward and backward captured at one shape, more shapes than are kept in between, memory reused, on two streams."""
+    from star_amd import NuggetSelfAttention
+    torch.manual_seed(0)
+    m = NuggetSelfAttention(256, 4, kv_heads=2).to(DEV, BF)
+    x, g = rnd(1, 2, 150, 256), rnd(2, 2, 150, 256)
+
+    def step(x, g):
+        leaf = x.detach().requires_grad_()
+        y = m(leaf)
+        return (y.detach(), *torch.autograd.grad(y, [leaf, *m.parameters()], g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, g)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(x, g)
+    new = rnd(3, 3, 9, 256)
+    with pytest.raises(RuntimeError, match="before a HIP-graph capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            m(new)
+    torch.cuda.synchronize()
+    for seed in (10, 20, 30):
+        with torch.cuda.stream(side), torch.no_grad():
+            others = [m(rnd(seed, 1, t, 256)) for t in range(1, 90, 2)]
+            junk = [torch.full((64, 8), -1, dtype=torch.int32, device=DEV) for _ in range(64)]
+        torch.cuda.current_stream().wait_stream(side)
+        x.copy_(rnd(seed, 2, 150, 256))
+        g.copy_(rnd(seed + 1, 2, 150, 256))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, step(x, g)):
+            assert torch.equal(a, b)
+        with torch.no_grad():
+            for t, o in zip(range(1, 90, 2), others):
+                assert torch.equal(o, m(rnd(seed, 1, t, 256)))
+        del junk
