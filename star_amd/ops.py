@@ -12,6 +12,7 @@ from typing import Optional, Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import CausalShape, KV8Cache, KV8Query, XAttnShape, check, lib, ptr, stream_ptr
@@ -1609,6 +1610,15 @@ def _same_device(what, **ts):
     return dev
 
 
+def _refuse_tangents(what, *ts):
+    """A dual tensor does not require grad, so its tangent would be dropped without a word by a call that goes round autograd.
+    (The level is -1 outside torch.autograd.forward_ad.dual_level and torch.func.jvp.)"""
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        for t in ts:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _row_strides(what, name, t):
     """The strides of a [.., hd] operand but for hd's, after checking what the kernels' 16-byte loads need of it.  That
     of a dimension of size 1, which is never used and may be anything, is given as 0."""
@@ -1848,6 +1858,7 @@ def causal_attn(q, k, v, plan: PackedSeqs, scale: Optional[float] = None, need_l
     infinite).  An infinite or NaN v row reaches up to 94 earlier queries of its own sequence, which share a tile with it;
     so do k rows in the gradient of q, and rows of q and of o's gradient reach later keys' gradients.  Rows of other
     sequences or in no sequence reach nobody."""
+    _refuse_tangents("causal_attn", q, k, v)
     s = _causal_shape(q, k, v, plan, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if not plan.apart:
@@ -1861,6 +1872,7 @@ def causal_attn_qkv(qkv, n_heads: int, kv_heads: int, plan: PackedSeqs, scale: O
     """causal_attn on one projection qkv [rows, (n_heads + 2 kv_heads) hd], queries, keys and values side by side (GPT-2's
     c_attn): returns o [rows, n_heads, hd].  The gradients of the three parts are written straight
     into one matrix of qkv's shape."""
+    _refuse_tangents("causal_attn_qkv", qkv)
     if qkv.dim() != 2 or n_heads < 1 or kv_heads < 1 or qkv.shape[1] % (n_heads + 2 * kv_heads):
         raise ValueError(f"causal_attn_qkv: [rows, ({n_heads} + 2 * {kv_heads}) * hd] expected, got {tuple(qkv.shape)}")
     if not plan.square:
@@ -2019,6 +2031,7 @@ def kv8_append(cache: KVCache8, k, v, counts=None, plan: Optional[PackedSeqs] = 
     block it began in.  At any other position the tokens in front of it in its block are lost: do not give one.
     Nothing is differentiated through a cache.  One launch, no host sync."""
     dev, B, H, hd = cache.device, cache.batch, cache.kv_heads, cache.head_dim
+    _refuse_tangents("kv8_append", k, v)
     if not (k.device == v.device == dev):
         _same_device("kv8_append", k=k, v=v, cache=cache.lens)
     if k.shape != v.shape:
@@ -2069,6 +2082,7 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
     to 16 bits for the product with v.  An infinite or NaN v of a token reaches every query of its sequence in the call as
     soon as one of them sees a token of its block."""
     dev, B, hd = cache.device, cache.batch, cache.head_dim
+    _refuse_tangents("kv8_attn", q, bias)
     if q.device != dev or (bias is not None and bias.device != dev):
         _same_device("kv8_attn", q=q, bias=bias, cache=cache.lens)
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:

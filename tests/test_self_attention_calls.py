@@ -263,3 +263,40 @@ def test_a_captured_module_replays_after_calls_of_other_shapes(ops):
             for t, o in zip(range(1, 90, 2), others):
                 assert torch.equal(o, m(rnd(seed, 1, t, 256)))
         del junk
+
+
+# ------------------------------------------------------------------------------------------------------ tangents
+def refuses_tangents(ops, dev):
+    from types import SimpleNamespace
+    from torch.autograd import forward_ad
+    q, qkv, b = (torch.ones(n, device=dev, dtype=BF) for n in ((4, 2, 64), (4, 384), (1, 5)))
+    plan = ops.PackedSeqs([4], dev)
+    cache = SimpleNamespace(device=q.device, batch=1, kv_heads=2, head_dim=64, dtype=BF)
+    x = q[None].transpose(1, 2)
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: ops.causal_attn(dual(q), q, q, plan), lambda: ops.causal_attn(q, dual(q), q, plan),
+                 lambda: ops.causal_attn(q, q, dual(q), plan), lambda: ops.causal_attn_qkv(dual(qkv), 2, 2, plan),
+                 lambda: ops.kv8_append(cache, dual(x), x), lambda: ops.kv8_append(cache, x, dual(x)),
+                 lambda: ops.kv8_attn(dual(x), cache), lambda: ops.kv8_attn(x, cache, bias=dual(b))]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: ops.causal_attn(t, q, q, plan), (q,), (q,))
+
+
+def test_tensors_with_a_tangent_are_refused(ops):
+    refuses_tangents(ops, "cpu")
+
+
+@gpu
+def test_tensors_with_a_tangent_are_refused_on_the_gpu_and_others_beside_them_run(ops):
+    from torch.autograd import forward_ad
+    refuses_tangents(ops, DEV)
+    q, k, v, _ = packed([9, 70], None, 2, 2, 64, BF)
+    plan = ops.PackedSeqs([9, 70], DEV)
+    with forward_ad.dual_level():
+        assert torch.equal(ops.causal_attn(q, k, v, plan), ops.causal_attn(q.requires_grad_(), k, v, plan).detach())
