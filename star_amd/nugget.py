@@ -517,7 +517,11 @@ class NuggetSelfAttention(nn.Module):
         attn(x, valid=frames)                    x [B,T,d] padded, frames an ops.ValidFrames; pad rows see nothing
         attn(x, plan=plan)                       x [rows,d] packed, plan an ops.PackedSeqs
         attn(x, plan=plan, cache=cache)          the same prompt, whose keys and values also go into an ops.KVCache8
-        attn(x, cache=cache, counts=n)           x [B,L,d]: the next (at most L) tokens of every sequence of the cache"""
+        attn(x, valid=frames, cache=cache)       the same, padded; pad rows do not go into the cache
+        attn(x, cache=cache, counts=n)           x [B,L,d]: the next (at most L) tokens of every sequence of the cache
+
+    A prompt attends to itself alone: the cache must hold nothing yet of the sequences that it has rows for (those of length 0
+    keep what they have).  What follows on held tokens, a prompt's next part too, goes in by the last form."""
 
     def __init__(self, hidden_size: int, num_heads: int, layer_idx: int = 0, scale_attn_weights: bool = True,
                  scale_attn_by_inverse_layer_idx: bool = False, resid_pdrop: float = 0.0, attn_pdrop: float = 0.0,
@@ -572,7 +576,7 @@ class NuggetSelfAttention(nn.Module):
         return ops.KVCache8(batch, self.kv_heads, max_tokens, self.head_dim, device or self.c_attn.weight.device, dtype)
 
     def forward(self, hidden_states, plan=None, valid=None, cache=None, counts=None):
-        if cache is not None and plan is None:
+        if cache is not None and plan is None and valid is None:
             return self._next_tokens(hidden_states, cache, counts)
         if counts is not None:
             raise ValueError("NuggetSelfAttention: counts go with the next tokens of a cache")

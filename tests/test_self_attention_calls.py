@@ -300,3 +300,45 @@ def test_tensors_with_a_tangent_are_refused_on_the_gpu_and_others_beside_them_ru
     plan = ops.PackedSeqs([9, 70], DEV)
     with forward_ad.dual_level():
         assert torch.equal(ops.causal_attn(q, k, v, plan), ops.causal_attn(q.requires_grad_(), k, v, plan).detach())
+
+
+# ------------------------------------------------------------------------------------------------------ padded prompts
+def test_a_padded_prompt_for_a_cache_goes_by_its_lengths(ops, monkeypatch):
+    """(CPU: the core and the append only record what they are given.)"""
+    seen = []
+    m = recording(monkeypatch, ops, seen)
+    valid, given = ops.ValidFrames([3, 0, 5], 5, "cpu"), []
+    monkeypatch.setattr(ops, "kv8_append", lambda cache, k, v, counts=None, plan=None, at=None: given.append((k.shape, plan, counts)))
+    cache = type("Cache", (), dict(dtype=torch.bfloat16))()
+    with torch.no_grad():
+        m(torch.zeros(3, 5, 128), valid=valid, cache=cache)
+        assert given == [((15, 2, 64), valid.seqs(), None)] and seen[0]() is valid.seqs()
+        for kw, text in ((dict(valid=valid, plan=valid.seqs()), "not both"), (dict(valid=valid, counts=torch.ones(3)), "counts go")):
+            with pytest.raises(ValueError, match=text):
+                m(torch.zeros(3, 5, 128), cache=cache, **kw)
+        with pytest.raises(ValueError, match="valid is for"):
+            m(torch.zeros(3, 4, 128), valid=valid, cache=cache)
+
+
+@gpu
+def test_a_padded_prompt_into_a_cache_equals_the_packed_one(ops):
+    """Pad rows, NaN included, neither enter the cache nor the prompt; sequences without a row in it keep what they hold."""
+    from star_amd import NuggetSelfAttention
+    lens, T, d = [50, 0, 130, 64], 130, 256
+    torch.manual_seed(0)
+    m = NuggetSelfAttention(d, 4, kv_heads=2).to(DEV, BF).eval()
+    x = rnd(1, 4, T, d)
+    real = torch.arange(T, device=DEV)[None] < torch.tensor(lens, device=DEV)[:, None]
+    with torch.no_grad():
+        packed_cache, padded_cache = m.new_cache(4, 192), m.new_cache(4, 192)
+        held = rnd(2, 4, 2, 7, 64)
+        for cache in (packed_cache, padded_cache):
+            ops.kv8_append(cache, held, held, counts=torch.tensor([0, 7, 0, 0], device=DEV))
+        want = m(x[real], plan=ops.PackedSeqs(lens, DEV), cache=packed_cache)
+        x[~real] = float("nan")
+        got = m(x, valid=ops.ValidFrames(lens, T, DEV), cache=padded_cache)
+        assert torch.equal(got[real], want) and padded_cache.lens.tolist() == [50, 7, 130, 64]
+        for a, b in zip(packed_cache.values(), padded_cache.values()):
+            assert torch.equal(a, b)
+        x = rnd(3, 4, 2, d)
+        assert torch.equal(m(x, cache=padded_cache), m(x, cache=packed_cache))
