@@ -189,6 +189,8 @@ class StreamingEncoderKV:
         cur = [min(int(c), self.seg.kmax) for c in counts]
         if len(cur) != self.seg.B:
             raise ValueError(f"extend: {len(cur)} counts for a batch of {self.seg.B}")
+        if self.caches is not None and any(c < p for c, p in zip(cur, self._prev)):
+            raise ValueError("extend: a count went back; reset() the utterance first")
         lo, hi = min(self._prev), max(cur)
         if hi > lo:
             B, d = self.seg.B, self.seg.d
@@ -202,8 +204,6 @@ class StreamingEncoderKV:
 
     def _append(self, out, lo, hi, cur):
         """Rows [prev_b, cur_b) of every utterance, of the projected [lo, hi), into the layers' caches."""
-        if any(c < p for c, p in zip(cur, self._prev)):
-            raise ValueError("extend: a count went back; reset() the utterance first")
         plan = ops.PackedSeqs([c - p for c, p in zip(cur, self._prev)], self.seg.device,
                               k_starts=[b * (hi - lo) + p - lo for b, p in enumerate(self._prev)])
         heads = out.to(self.caches[0].dtype).view(out.shape[0], 2 * self.nl, self.h, -1)

@@ -342,3 +342,48 @@ def test_a_padded_prompt_into_a_cache_equals_the_packed_one(ops):
             assert torch.equal(a, b)
         x = rnd(3, 4, 2, d)
         assert torch.equal(m(x, cache=padded_cache), m(x, cache=packed_cache))
+
+
+# ------------------------------------------------------------------------------------------------------ streaming memory
+def streamed(B, kmax, dev, dtype=torch.bfloat16, d=128):
+    from star_amd import NuggetCrossAttention, NuggetScorer
+    from star_amd.streaming import StreamingEncoderKV, StreamingNuggetSegmenter
+    torch.manual_seed(0)
+    seg = StreamingNuggetSegmenter(NuggetScorer(d).to(dev), B, d, kmax, dev, dtype=dtype)
+    return seg, StreamingEncoderKV([NuggetCrossAttention(d, 2).to(dev, dtype)], seg, eight_bit=True)
+
+
+@pytest.mark.parametrize("before,then", [([5], [3]), ([5], [0]), ([7, 5], [4, 5]), ([7, 5], [9, 4])])
+def test_a_count_that_goes_back_is_refused_whether_or_not_a_row_is_projected(ops, monkeypatch, before, then):
+    """(CPU: the caches and the segmenter are stand-ins; what extend() takes and keeps is looked at.)"""
+    from types import SimpleNamespace
+    from star_amd.streaming import StreamingEncoderKV
+    kv, given = StreamingEncoderKV.__new__(StreamingEncoderKV), []
+    B, d = len(before), 128
+    kv.seg = SimpleNamespace(B=B, d=d, kmax=64, device=torch.device("cpu"), state=SimpleNamespace(mem=torch.zeros(B, 64, d)))
+    kv.nl, kv.h, kv.w_all, kv.b_all, kv.kv = 1, 2, torch.zeros(d, 2 * d), torch.zeros(2 * d), None
+    kv.caches, kv._prev = [SimpleNamespace(dtype=BF)], [0] * B
+    monkeypatch.setattr(ops, "kv8_append", lambda cache, k, v, plan=None: given.append(plan.counts.tolist()))
+    kv.extend(before)
+    with pytest.raises(ValueError, match="went back"):
+        kv.extend(then)
+    assert kv._prev == before and given == [before]
+    kv.extend([c + 1 for c in before])
+    assert given == [before, [1] * B]
+
+
+@gpu
+def test_a_refused_extend_leaves_the_caches_as_they_were(ops):
+    seg, kv = streamed(1, 150, DEV)
+    seg.state.mem.copy_(rnd(1, 1, 150, 128))
+    kv.extend([70])
+    for back in ([60], [0]):
+        with pytest.raises(ValueError, match="went back"):
+            kv.extend(back)
+    kv.extend([80])
+    _, whole = streamed(1, 150, DEV)
+    whole.seg.state.mem.copy_(seg.state.mem)
+    whole.extend([70])
+    whole.extend([80])
+    a, b = kv.layers()[0].cache, whole.layers()[0].cache
+    assert a.lens.tolist() == [80] and all(torch.equal(x, y) for x, y in zip(a.values(), b.values()))
