@@ -1747,8 +1747,10 @@ def _causal_forward(q, k, v, plan, s, want_lse):
     lse = None
     if want_lse:
         lse = torch.empty((s.H, rows), dtype=torch.float32, device=dev)
-        if plan.q_used != rows:
+        if plan.q_used != rows or not plan.n_k_tiles:
             lse.fill_(-math.inf)
+    if not plan.n_k_tiles:                                         # no key in the whole batch, k and v may have no memory
+        return o.zero_(), lse
     # (only launches of few workgroups over many keys are cut along the keys)
     need = lib().star_causal_fwd_workspace(s) if plan.max_k > 320 and plan.n_q_tiles * s.H < 256 else 0
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
@@ -1761,6 +1763,10 @@ def _causal_backward(g, q, k, v, o, lse, plan, s, dq, dk, dv):
     """Gradients into dq, dk and dv, whose rows are s.dq_sr and s.dkv_sr values apart."""
     if torch.is_grad_enabled():
         raise _lib.StarNuggetError("causal_attn has no second derivative (backward with create_graph=True)")
+    if not (plan.n_q_tiles and plan.n_k_tiles):                    # nobody sees anything
+        for t in (dq, dk, dv):
+            t.zero_()
+        return
     if g.dtype != q.dtype:
         g = g.to(q.dtype)
     g = g.contiguous()

@@ -387,3 +387,46 @@ def test_a_refused_extend_leaves_the_caches_as_they_were(ops):
     whole.extend([80])
     a, b = kv.layers()[0].cache, whole.layers()[0].cache
     assert a.lens.tolist() == [80] and all(torch.equal(x, y) for x, y in zip(a.values(), b.values()))
+
+
+# ------------------------------------------------------------------------------------------------------ empty batches
+EMPTY = [([0], [5]), ([0, 0], [300, 1]), ([5], [0]), ([700, 3], [0, 0]), ([0], [0]), ([], [])]
+
+
+def empty_batch(ops, keys, queries, dev, padded, monkeypatch=None):
+    """No key (query) in the whole batch: o = 0, lse = -inf, gradients 0, whether or not the tensors have rows at all."""
+    H, Hkv, hd = 4, 2, 64
+    n_q, n_k = (max(1, len(keys)) * 1000,) * 2 if padded else (sum(queries), sum(keys))
+    q, k, v = (torch.ones(n, h, hd, dtype=BF, device=dev).requires_grad_() for n, h in ((n_q, H), (n_k, Hkv), (n_k, Hkv)))
+    plan = ops.PackedSeqs(keys, dev, q_lengths=queries, padded_to=1000 if padded else None)
+    if dev == "cpu":
+        o, lse = ops._CausalAttn.apply(q, k, v, plan, ops._causal_layout(q, k, v, plan, None), True)
+    else:
+        o, lse = ops.causal_attn(q, k, v, plan, need_lse=True)
+        with torch.no_grad():
+            assert torch.equal(ops.causal_attn(q, k, v, plan), o)
+    assert o.shape == q.shape and (o == 0).all() and lse.shape == (H, n_q) and torch.isneginf(lse).all()
+    for t, g in zip((q, k, v), torch.autograd.grad(o, (q, k, v), torch.ones_like(o))):
+        assert g.shape == t.shape and (g == 0).all()
+
+
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("keys,queries", EMPTY)
+def test_a_batch_without_keys_or_without_queries_launches_nothing_that_needs_them(ops, monkeypatch, keys, queries, padded):
+    """(CPU: the memory that torch.empty gives is poisoned, and a launch may be asked for only if it has nothing to do.)"""
+    def launch(fn, what, dev, *args):
+        s = next(a for a in args if isinstance(a, ops.CausalShape))
+        assert what == "star_causal_fwd" and s.n_q_tiles == 0, (what, s.n_q_tiles, s.n_k_tiles)
+
+    make = torch.empty_like
+    monkeypatch.setattr(ops, "_launch", launch)
+    monkeypatch.setattr(torch, "empty", lambda size, dtype, device: torch.full(size, 7.0, dtype=dtype, device=device))
+    monkeypatch.setattr(torch, "empty_like", lambda t, **kw: make(t, **kw).fill_(7.0))
+    empty_batch(ops, keys, queries, "cpu", padded)
+
+
+@gpu
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("keys,queries", EMPTY)
+def test_a_batch_without_keys_or_without_queries(ops, keys, queries, padded):
+    empty_batch(ops, keys, queries, DEV, padded)
