@@ -501,7 +501,8 @@ int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, 
  * how they were split into calls.
  *   k_codes [B][Hkv][T][hd], k_scales [B][Hkv][T/64]         k_tail [B][Hkv][64][hd]  (row = token % 64)
  *   v_codes [B][Hkv][T/64][hd][64], v_scales [B][Hkv][T/64]  v_tail [B][Hkv][hd][64]  (V is transposed inside a block)
- *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written);
+ *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written), so that a sequence has
+ *       lens + dropped positions; a call with `at` counts anew;
  *   tickets [B * (1 + 2 * Hkv) * STAR_KV8_TICKET_STRIDE]: zero before the first call, zero after every call.  All base addresses multiples of 16 bytes.
  * An append must not overlap any other call on the cache (the stream orders them); attentions alone may. */
 #define STAR_KV8_BLOCK 64
@@ -531,7 +532,8 @@ int star_kv8_append(const star_kv8_cache* c, const void* k, const void* v, int64
 
 /* o = softmax(scale q k^T + bias) v over the tokens held; q [B,H,L,hd] and o by strides as above, query head h on key
  * head h / (H / Hkv).  q_len [B] or NULL: queries of sequence b (at most L; rows behind them give 0).
- *   causal: query i sees the tokens j <= lens[b] - q_len[b] + i (the queries are the newest tokens, already appended)
+ *   causal: query i sees the tokens j <= lens[b] + dropped[b] - q_len[b] + i (the queries are the newest tokens, already
+ *       appended, those that found no room among them: these see all that is held)
  *   ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask, my_transformer.py:566)
  *   bias [B][bias_len] fp32 or NULL, added to the logits of token j < bias_len (the scorer's logits)
  * A query that sees nothing, or only biases of -inf (or so low that bias * log2(e) overflows), gives 0.

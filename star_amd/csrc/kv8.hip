@@ -197,7 +197,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
             if (gridDim.x > 1) *mine = 0;
             if (count(ticket) == (int)gridDim.y - 1) {
                 c.lens[b] = end;
-                if (want > n) c.dropped[b] += want - n;
+                if (a.at) c.dropped[b] = want - n;                  // (what was missing behind `at` is no longer part of the sequence)
+                else if (want > n) c.dropped[b] += want - n;
                 *ticket = 0;
             }
         }
@@ -339,12 +340,13 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
 
     int lim[RT];
     x8 qf[RT][KS];
+    const int64_t came = a.s.causal ? (int64_t)n + max(c.dropped[b], 0) : 0;    // tokens of the sequence, those without room too
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int rho = (rg * RT + rt) * 16 + r16, i = rho / grp, hh = rho % grp;
         const bool real = rho < rows && i < nq;
         int see = n;
-        if (a.s.causal) see = min(see, n - nq + i + 1);
+        if (a.s.causal) see = (int)min((int64_t)see, came - nq + i + 1);
         if (a.s.ilk_diag >= 0) see = (int)min((int64_t)see, (int64_t)i + a.s.ilk_diag + 1);
         lim[rt] = real ? max(see, 0) : 0;
         const T* qr = (const T*)a.q + (int64_t)b * a.s.q_sb + (int64_t)(hk * grp + (rho < rows ? hh : 0)) * a.s.q_sh +

@@ -1930,7 +1930,7 @@ class KVCache8:
     does not depend on how the tokens were split into calls).  kv8_append fills it, kv8_attn reads it.
 
     lens [batch] int32 lives on the device and counts the tokens held; tokens that find no room are dropped and counted
-    (`overflow()`).  An append must be ordered with every other call on the cache (by one stream, or events); reads alone may
+    (`overflow()`), and keep their positions: the tokens that did fit see what they would have seen.  An append must be ordered with every other call on the cache (by one stream, or events); reads alone may
     overlap.  Captured calls replay on the cache as it then is."""
 
     _PARTS = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "lens")
@@ -1997,7 +1997,8 @@ class KVCache8:
         self._dropped[sel] = 0
 
     def overflow(self):
-        """[batch] int32: tokens that found no room.  Non-zero = the sequence's end is missing."""
+        """[batch] int32: tokens that found no room since the last reset or append at given positions.  Non-zero = the
+        sequence's end is missing."""
         return self._dropped
 
     def values(self):
@@ -2080,7 +2081,7 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
              scale: Optional[float] = None):
     """Attention of a few new tokens over an 8-bit cache: q [batch, H, L, hd] in the cache's dtype, H a multiple of the
     cache's heads.  causal: the queries are the newest tokens, already appended -- query i sees the tokens j <=
-    lens[b] - q_len[b] + i; ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask of xattn).  q_len [batch]
+    lens[b] + overflow()[b] - q_len[b] + i; ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask of xattn).  q_len [batch]
     (device integers): queries of every sequence, the rows behind them give 0; default L.  bias [batch, n <= capacity]
     is added to the logits of token j < n.  scale defaults to hd ** -0.5.  A query that sees nothing gives 0.
     Returns [batch, H, L, hd] (memory order [batch, L, H, hd], as xattn).  Inference only: call it under no_grad.

@@ -12,7 +12,7 @@ import weakref
 import pytest
 import torch
 
-from tests.test_self_attention import BF, DEV, by_formula, check, packed, rnd
+from tests.test_self_attention import BF, DEV, FP, by_formula, cached_formula, check, packed, rnd
 
 gpu = pytest.mark.gpu
 
@@ -430,3 +430,66 @@ def test_a_batch_without_keys_or_without_queries_launches_nothing_that_needs_the
 @pytest.mark.parametrize("keys,queries", EMPTY)
 def test_a_batch_without_keys_or_without_queries(ops, keys, queries, padded):
     empty_batch(ops, keys, queries, DEV, padded)
+
+
+# ------------------------------------------------------------------------------------------------------ full caches
+@gpu
+@pytest.mark.parametrize("held,T,L,H,Hkv,hd,dtype", [
+    ([63, 10, 64, 62], 64, 3, 4, 2, 64, BF),
+    ([5055, 5000, 17], 5056, 4, 4, 4, 128, BF),                # cut into parts
+    ([127, 128], 128, 16, 4, 2, 96, FP)])
+def test_tokens_that_found_room_see_themselves_when_others_did_not(ops, held, T, L, H, Hkv, hd, dtype):
+    """An append that fills the cache in the middle of its tokens: query i is the token at held + i and sees everything up to
+    itself that the cache holds."""
+    B = len(held)
+    cache = ops.KVCache8(B, Hkv, T, hd, DEV, dtype)
+    n = torch.tensor(held, device=DEV)
+
+    def fill(at=None):
+        new = (rnd(1, B, Hkv, max(held), hd, dtype=dtype), rnd(2, B, Hkv, max(held), hd, dtype=dtype))
+        ops.kv8_append(cache, *new, counts=n, at=at)
+
+    def attend(counts, first, q_len):
+        q = rnd(5, B, H, L, hd, dtype=dtype)
+        o = ops.kv8_attn(q, cache, q_len=q_len)
+        k, v = cache.values()
+        for i in range(L):
+            see = [max(0, min(T, f + i + 1)) if i < c else 0 for f, c in zip(first, counts)]
+            want, bound = cached_formula(q[:, :, i:i + 1], k, v, see, False, None, -1, None, hd ** -0.5)
+            check(o[:, :, i:i + 1], want, bound, i)
+
+    fill()
+    new = rnd(3, B, Hkv, L, hd, dtype=dtype), rnd(4, B, Hkv, L, hd, dtype=dtype)
+    counts = [L - b % 2 for b in range(B)]
+    c = torch.tensor(counts, device=DEV)
+    ops.kv8_append(cache, *new, counts=c)
+    assert cache.lens.tolist() == [min(T, h + x) for h, x in zip(held, counts)]
+    assert cache.overflow().tolist() == [max(0, h + x - T) for h, x in zip(held, counts)]
+    attend(counts, held, c)
+    first = [h + x for h, x in zip(held, counts)]              # and the next ones, of which none may fit
+    ops.kv8_append(cache, *new)
+    attend([L] * B, first, None)
+    # positions given: what is missing is counted from there
+    fill(at=torch.zeros(B, dtype=torch.int32, device=DEV))
+    assert cache.overflow().tolist() == [0] * B
+    ops.kv8_append(cache, *new, counts=c, at=n)
+    assert cache.overflow().tolist() == [max(0, h + x - T) for h, x in zip(held, counts)]
+    attend(counts, held, c)
+    back = [h // 64 * 64 for h in held]                        # taken back
+    ops.kv8_append(cache, new[0][:, :, :0], new[1][:, :, :0], at=torch.tensor(back, device=DEV))
+    assert cache.overflow().tolist() == [0] * B and cache.lens.tolist() == back
+    attend([L] * B, [x - L for x in back], None)
+
+
+@gpu
+def test_tokens_of_a_module_that_fills_its_cache(ops):
+    from star_amd import NuggetSelfAttention
+    torch.manual_seed(0)
+    m = NuggetSelfAttention(256, 4, kv_heads=2).to(DEV, BF).eval()
+    x = rnd(1, 2, 70, 256)
+    with torch.no_grad():
+        small, large = m.new_cache(2, 64), m.new_cache(2, 128)
+        for cache in (small, large):
+            m(x[:, :62], valid=ops.ValidFrames([62, 61], 62, DEV), cache=cache)
+        a, b = (m(x[:, 62:65], cache=cache) for cache in (small, large))
+    assert torch.equal(a[0, :2], b[0, :2]) and torch.equal(a[1], b[1]) and small.overflow().tolist() == [1, 0]
