@@ -463,6 +463,7 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
  *        positions); a query that sees no key gets o = 0, lse = -inf.  Rows in no sequence are not touched
  *   lse [H][lse_stride] fp32, by row: natural log-sum-exp of the scaled logits, for the backward (NULL: not wanted)
  * Softmax statistics and sums are fp32; the weights P are rounded to dtype for the product with V (as the inputs are).
+ * Logits are fp32: what is smaller than 2^-24 of their size is lost, and from a size of 2^30 on a row's weights mean nothing.
  * Nothing is masked by arithmetic on values: a key after the query never enters its maximum, sum or output, with one
  * exception: V rows of the SAME sequence behind the query but inside a 64-key tile that another query of its 32 sees meet a
  * weight of exactly 0, so an infinite or NaN V reaches up to 94 earlier queries of its own sequence. */

@@ -6,7 +6,8 @@ namespace star {
 
 constexpr float A_LOG2E = 1.4426950408889634f;
 constexpr float A_LN2 = 0.6931471805599453f;
-constexpr float M_NONE = -1.0e30f;       // running maximum before the first visible key (finite: no inf - inf)
+// Running maximum before the first visible key: the lowest finite value (no inf - inf), so that no finite logit is below it
+constexpr float M_NONE = -3.402823466e38f;
 constexpr float M_SLACK = 8.0f;          // log2 units: the running maximum follows only when a tile exceeds it by 2^8
 
 constexpr float M_MOST = 4096.0f;        // largest sum of a lane's weights of a tile against an earlier tile's maximum

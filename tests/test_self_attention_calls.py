@@ -493,3 +493,24 @@ def test_tokens_of_a_module_that_fills_its_cache(ops):
             m(x[:, :62], valid=ops.ValidFrames([62, 61], 62, DEV), cache=cache)
         a, b = (m(x[:, 62:65], cache=cache) for cache in (small, large))
     assert torch.equal(a[0, :2], b[0, :2]) and torch.equal(a[1], b[1]) and small.overflow().tolist() == [1, 0]
+
+
+# ------------------------------------------------------------------------------------------------------ low logits
+@gpu
+@pytest.mark.parametrize("low", [-1e30, -2.3e38])
+@pytest.mark.parametrize("n,T", [(100, 128), (5000, 5056)])
+def test_kv8_attn_rows_whose_every_bias_is_low_give_the_mean(ops, low, n, T):
+    """A finite bias takes a key out only beside higher ones: where every bias is the same, the softmax is that without it
+    (here every other logit is rounded away by it, which leaves the mean)."""
+    hd, H = 64, 4
+    cache = ops.KVCache8(2, 2, T, hd, DEV)
+    k, v = rnd(1, 2, 2, n, hd), rnd(2, 2, 2, n, hd)
+    ops.kv8_append(cache, k, v)
+    q = rnd(3, 2, H, 1, hd)
+    bias = torch.full((2, T), low, device=DEV)
+    bias[1, 5:9] = 0.0
+    o = ops.kv8_attn(q, cache, bias=bias)
+    kk, vv = cache.values()
+    want, bound = cached_formula(torch.stack([torch.zeros_like(q[0]), q[1]]), kk, vv, [n, n], True, None, -1,
+                                 torch.stack([torch.zeros_like(bias[0]), bias[1]]), hd ** -0.5)
+    check(o, want, bound)
