@@ -596,7 +596,7 @@ class NuggetSelfAttention(nn.Module):
         core = qkv.to(torch.bfloat16) if qkv.dtype == torch.float32 else qkv
         out = ops.causal_attn_qkv(core, self.num_heads, self.kv_heads, plan, scale=self.scale)
         if cache is not None:
-            _, k, v = ops._qkv_views(core.detach(), self.num_heads, self.kv_heads, self.head_dim)
+            _, k, v = ops._qkv_views(core.detach().to(cache.dtype), self.num_heads, self.kv_heads, self.head_dim)
             ops.kv8_append(cache, k, v, plan=plan)
         out = out.flatten(1).to(qkv.dtype).view(hidden_states.shape)
         return self.resid_dropout(self.c_proj(out))

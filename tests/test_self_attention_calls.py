@@ -514,3 +514,37 @@ def test_kv8_attn_rows_whose_every_bias_is_low_give_the_mean(ops, low, n, T):
     want, bound = cached_formula(torch.stack([torch.zeros_like(q[0]), q[1]]), kk, vv, [n, n], True, None, -1,
                                  torch.stack([torch.zeros_like(bias[0]), bias[1]]), hd ** -0.5)
     check(o, want, bound)
+
+
+# ------------------------------------------------------------------------------------------------------ types of caches
+@gpu
+@pytest.mark.parametrize("dtype,held", [(FP, BF), (BF, FP), (torch.float32, FP), (torch.float32, BF)])
+def test_a_prompt_and_its_next_part_into_a_cache_of_another_type(ops, dtype, held):
+    """The prompt's own output is that without a cache; what follows, a long next part and single tokens, is the formula's on
+    the values that the cache stands for."""
+    from star_amd import NuggetSelfAttention
+    H, Hkv, hd, lens = 4, 2, 64, [60, 1, 129]
+    torch.manual_seed(0)
+    m = NuggetSelfAttention(H * hd, H, kv_heads=Hkv).to(DEV, dtype).eval()
+    seen = []
+    m.c_attn.register_forward_hook(lambda mod, args, out: seen.append(out))
+    plan, x = ops.PackedSeqs(lens, DEV), rnd(1, sum(lens), H * hd, dtype=dtype)
+    with torch.no_grad():
+        m.c_proj.weight.copy_(torch.eye(H * hd))
+        cache = m.new_cache(3, 350, dtype=held)
+        assert torch.equal(m(x, plan=plan, cache=cache), m(x, plan=plan)) and cache.lens.tolist() == lens
+        core = seen[0].to(BF) if dtype == torch.float32 else seen[0]
+        k = core.to(held).view(-1, H + 2 * Hkv, hd)[:, H:H + Hkv]
+        for b, (first, n) in enumerate(zip((0, 60, 61), lens)):
+            assert torch.equal(cache.k_tail[b, :, :n % 64], k[first + n // 64 * 64:first + n].transpose(0, 1))
+        n = lens
+        for L, counts in ((190, [190, 100, 7]), (1, [1, 1, 1])):
+            xs = rnd(L, 3, L, H * hd, dtype=dtype)
+            seen.clear()
+            y = m(xs, cache=cache, counts=torch.tensor(counts, device=DEV))
+            n = [a + c for a, c in zip(n, counts)]
+            assert cache.lens.tolist() == n
+            q = seen[0].view(3, L, -1, hd)[:, :, :H].transpose(1, 2).to(held)
+            want, bound = cached_formula(q, *cache.values(), n, True, counts, -1, None, hd ** -0.5)
+            u = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2          # (rounded to the module's type once more)
+            check(y.view(3, L, H, hd).transpose(1, 2), want, bound + u * (want.abs() + bound) + 2.0 ** -25, L)
