@@ -2112,7 +2112,7 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
     o = torch.empty_strided((B, H, L, hd), (*o_st, 1), dtype=q.dtype, device=dev)
     if L == 0:
         return o
-    s = KV8Query(H, L, *_row_strides("kv8_attn", "q", q), *o_st, n_bias, 1 if causal else 0, int(ilk_diag),
+    s = KV8Query(H, L, *_row_strides("kv8_attn", "q", q), *o_st, n_bias, 1 if causal else 0, min(max(int(ilk_diag), -1), cache.capacity),
                  hd ** -0.5 if scale is None else float(scale))
     need = cache._workspace.get((H, L))
     if need is None:

@@ -548,3 +548,14 @@ def test_a_prompt_and_its_next_part_into_a_cache_of_another_type(ops, dtype, hel
             want, bound = cached_formula(q, *cache.values(), n, True, counts, -1, None, hd ** -0.5)
             u = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2          # (rounded to the module's type once more)
             check(y.view(3, L, H, hd).transpose(1, 2), want, bound + u * (want.abs() + bound) + 2.0 ** -25, L)
+
+
+@gpu
+def test_kv8_attn_lookback_beyond_32_bits(ops):
+    """A lookback mask as far as any integer hides nothing, one as far back as any integer is none."""
+    cache = ops.KVCache8(1, 2, 128, 64, DEV)
+    k, v, q = rnd(1, 1, 2, 100, 64), rnd(2, 1, 2, 100, 64), rnd(3, 1, 4, 3, 64)
+    ops.kv8_append(cache, k, v)
+    want = ops.kv8_attn(q, cache, causal=False)
+    for far in (100, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 40, -2 ** 32 + 5):
+        assert torch.equal(ops.kv8_attn(q, cache, causal=False, ilk_diag=far), want), far
