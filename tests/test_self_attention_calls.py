@@ -5,6 +5,7 @@ import copy
 import gc
 import io
 import pickle
+import random
 import sys
 import threading
 import weakref
@@ -559,3 +560,34 @@ def test_kv8_attn_lookback_beyond_32_bits(ops):
     want = ops.kv8_attn(q, cache, causal=False)
     for far in (100, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 40, -2 ** 32 + 5):
         assert torch.equal(ops.kv8_attn(q, cache, causal=False, ilk_diag=far), want), far
+
+
+# ------------------------------------------------------------------------------------------------------ workspaces
+def test_every_launch_is_given_the_workspace_that_the_library_asks_for(ops, monkeypatch):
+    """The size is not asked for where launches are never cut: the library agrees on both sides of every border.  (CPU: the
+    launches are recorded, not made.)"""
+    from star_amd import _lib
+    L, given = _lib.lib(), []
+
+    def launch(fn, what, dev, *args):
+        s = next(a for a in args if isinstance(a, ops.CausalShape))
+        size = L.star_causal_fwd_workspace if what == "star_causal_fwd" else L.star_causal_bwd_workspace
+        need = size(s)
+        given.append((what, need > 0))
+        assert args[-1] == need and bool(args[-2]) == (need > 0), (what, args[-1], need, [(n, getattr(s, n)) for n, _ in s._fields_])
+
+    monkeypatch.setattr(ops, "_launch", launch)
+    monkeypatch.setattr(ops, "_rows_like", lambda rows, used, heads, hd, t: torch.empty(hd, dtype=t.dtype))
+    rng = random.Random(0)
+    for _ in range(600):
+        hd, Hkv, g = rng.choice([64, 96, 128]), rng.choice([1, 2, 3, 8]), rng.choice([1, 1, 2, 8])
+        most = rng.choice([32, 33, 255, 256, 257, 319, 320, 321, 384, 385, 448, 449, 832, 833, 1500])
+        keys = [rng.randint(1, most) for _ in range(rng.choice([0, 1, 3, 30, 64, 127]))] + [most]
+        queries = rng.choice([None, [min(n, rng.choice([1, 16, 17, 32, 33])) for n in keys]])
+        plan = ops.PackedSeqs(keys, "cpu", q_lengths=queries)
+        q, k = (torch.empty(hd, dtype=BF).expand(n, h, hd) for n, h in ((plan.q_rows, g * Hkv), (plan.k_rows, Hkv)))
+        s = ops._causal_layout(q, k, k, plan, None)
+        ops._causal_forward(q, k, k, plan, s, False)
+        with torch.no_grad():
+            ops._causal_backward(torch.empty(0, dtype=BF), q, k, k, q, torch.empty(1), plan, s, q, k, k)
+    assert set(given) == {("star_causal_fwd", False), ("star_causal_fwd", True), ("star_causal_bwd", False), ("star_causal_bwd", True)}
