@@ -503,7 +503,7 @@ int star_causal_bwd(const void* q, const void* k, const void* v, const void* o, 
  *   k_codes [B][Hkv][T][hd], k_scales [B][Hkv][T/64]         k_tail [B][Hkv][64][hd]  (row = token % 64)
  *   v_codes [B][Hkv][T/64][hd][64], v_scales [B][Hkv][T/64]  v_tail [B][Hkv][hd][64]  (V is transposed inside a block)
  *   lens [B] tokens held; dropped [B] tokens that found no room (counted, never written), so that a sequence has
- *       lens + dropped positions; a call with `at` counts anew;
+ *       lens + dropped positions (at + count after a call with `at`);
  *   tickets [B * (1 + 2 * Hkv) * STAR_KV8_TICKET_STRIDE]: zero before the first call, zero after every call.  All base addresses multiples of 16 bytes.
  * An append must not overlap any other call on the cache (the stream orders them); attentions alone may. */
 #define STAR_KV8_BLOCK 64

@@ -197,7 +197,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
             if (gridDim.x > 1) *mine = 0;
             if (count(ticket) == (int)gridDim.y - 1) {
                 c.lens[b] = end;
-                if (a.at) c.dropped[b] = want - n;                  // (what was missing behind `at` is no longer part of the sequence)
+                // (with `at` the sequence is at + want tokens long, whatever was missing before)
+                if (a.at) c.dropped[b] = (int)min((int64_t)max(a.at[b], 0) + want - end, (int64_t)0x7fffffff);
                 else if (want > n) c.dropped[b] += want - n;
                 *ticket = 0;
             }

@@ -1930,8 +1930,9 @@ class KVCache8:
     does not depend on how the tokens were split into calls).  kv8_append fills it, kv8_attn reads it.
 
     lens [batch] int32 lives on the device and counts the tokens held; tokens that find no room are dropped and counted
-    (`overflow()`), and keep their positions: the tokens that did fit see what they would have seen.  An append must be ordered with every other call on the cache (by one stream, or events); reads alone may
-    overlap.  Captured calls replay on the cache as it then is."""
+    (`overflow()`), and keep their positions: the tokens that did fit see what they would have seen.  An append must be
+    ordered with every other call on the cache (by one stream, or events); reads alone may overlap.  Captured calls replay
+    on the cache as it then is."""
 
     _PARTS = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "lens")
 
@@ -1987,7 +1988,7 @@ class KVCache8:
         c.dropped, c.tickets = self._dropped.data_ptr(), self._tickets.data_ptr()
 
     def tensors(self):
-        """The cache's own buffers, by name (to save it, or for from_tensors)."""
+        """The cache's own buffers, by name (to save it, or for from_tensors, whose cache counts overflow() from 0)."""
         return {n: getattr(self, n) for n in self._PARTS}
 
     def reset(self, rows=None):
@@ -1997,8 +1998,8 @@ class KVCache8:
         self._dropped[sel] = 0
 
     def overflow(self):
-        """[batch] int32: tokens that found no room since the last reset or append at given positions.  Non-zero = the
-        sequence's end is missing."""
+        """[batch] int32: tokens that found no room; a sequence has lens + overflow() positions.  Non-zero = the sequence's end
+        is missing."""
         return self._dropped
 
     def values(self):
@@ -2081,9 +2082,9 @@ def kv8_attn(q, cache: KVCache8, causal: bool = True, q_len=None, ilk_diag: int 
              scale: Optional[float] = None):
     """Attention of a few new tokens over an 8-bit cache: q [batch, H, L, hd] in the cache's dtype, H a multiple of the
     cache's heads.  causal: the queries are the newest tokens, already appended -- query i sees the tokens j <=
-    lens[b] + overflow()[b] - q_len[b] + i; ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask of xattn).  q_len [batch]
-    (device integers): queries of every sequence, the rows behind them give 0; default L.  bias [batch, n <= capacity]
-    is added to the logits of token j < n.  scale defaults to hd ** -0.5.  A query that sees nothing gives 0.
+    lens[b] + overflow()[b] - q_len[b] + i; ilk_diag >= 0: it sees j <= i + ilk_diag (the infinite-lookback mask of xattn).
+    q_len [batch] (device integers): queries of every sequence, the rows behind them give 0; default L.  bias [batch, n <=
+    capacity] is added to the logits of token j < n.  scale defaults to hd ** -0.5.  A query that sees nothing gives 0.
     Returns [batch, H, L, hd] (memory order [batch, L, H, hd], as xattn).  Inference only: call it under no_grad.
     The values that the cache stands for are used as they are; softmax and sums are fp32, the softmax weights are rounded
     to 16 bits for the product with v.  An infinite or NaN v of a token reaches every query of its sequence in the call as

@@ -483,6 +483,25 @@ def test_tokens_that_found_room_see_themselves_when_others_did_not(ops, held, T,
 
 
 @gpu
+def test_positions_behind_the_capacity_count_what_is_missing(ops):
+    """A program that gives every token's position: overflow() is the part of the sequence that is not held."""
+    cache = ops.KVCache8(3, 1, 64, 64, DEV)
+    k, v, q = rnd(1, 3, 1, 66, 64), rnd(2, 3, 1, 66, 64), rnd(3, 3, 2, 1, 64)
+    at = torch.tensor([60, 62, -5], dtype=torch.int32, device=DEV)
+    ops.kv8_append(cache, k[:, :, :60], v[:, :, :60])
+    ops.kv8_append(cache, k[:, :, 60:62], v[:, :, 60:62], counts=torch.tensor([0, 2, 2], device=DEV))
+    for step in range(6):
+        ops.kv8_append(cache, k[:, :, step:step + 1], v[:, :, step:step + 1], at=at + torch.tensor([step, step, 0], device=DEV))
+        end = [60 + step + 1, 62 + step + 1, 1]
+        assert cache.lens.tolist() == [min(64, n) for n in end]
+        assert cache.overflow().tolist() == [max(0, n - 64) for n in end]
+        want, bound = cached_formula(q, *cache.values(), cache.lens.tolist(), False, None, -1, None, 0.125)
+        check(ops.kv8_attn(q, cache), want, bound, step)
+    ops.kv8_append(cache, k[:, :, :2], v[:, :, :2], at=torch.full((3,), 2 ** 31 - 1, device=DEV))
+    assert cache.lens.tolist() == [64] * 3 and cache.overflow().tolist() == [2 ** 31 - 1 - 62] * 3
+
+
+@gpu
 def test_tokens_of_a_module_that_fills_its_cache(ops):
     from star_amd import NuggetSelfAttention
     torch.manual_seed(0)
