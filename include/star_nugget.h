@@ -456,7 +456,8 @@ int star_xattn_dbias_sum(const float* const* parts_host, int nl, int B, int h, i
  * attention of the semantic encoder over the frames and of the decoder over its own tokens, on sequences that lie one
  * behind the other instead of in a padded batch, with grouped heads (query head h reads key head h / (H / Hkv)).
  *   q [rows,H,hd], k / v [rows,Hkv,hd], o like q: 16-bit values of one type (dtype), hd contiguous, row and head
- *        strides in elements, multiples of 8; base addresses multiples of 16 bytes.  hd in {64, 96, 128}
+ *        strides in elements, multiples of 8; base addresses multiples of 16 bytes, not NULL where there are tiles (also of
+ *        a tensor without rows, which is not read).  hd in {64, 96, 128}
  *   tiles [n_q_tiles][8] int32, every tile of STAR_CAUSAL_TILE queries of every sequence exactly once, in the order in which
  *        they are to start: the sequence's first query row, queries nq, first key row and keys nk, the tile's first query,
  *        and three unused words.  Query i of a sequence sees its keys j <= i + nk - nq (the queries are the newest nq

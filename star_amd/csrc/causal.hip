@@ -954,8 +954,8 @@ __global__ __launch_bounds__(256) void causal_dkv_sum_kernel(const float* __rest
 // anything up to the longest): steps of `per`, so that wgs * (mean / per + 1/2) pieces, which is what such walks come to, fill
 // the 512 places (two a CU) once.  From 320 workgroups on, and from 256 with walks of middle length, a walk in one piece
 // is as good or better: two rounds of pieces and the sums' way through memory cost what the idle CUs did.  Forward
-// and backward, 8 heads of 128: one sequence of 1500 tokens 137 -> 91 us, 3000 tokens 260 -> 170, 5000 tokens (320 workgroups)
-// 460 -> 352; 6 of 800 to 1300 (400) 147 -> 186.
+// and backward, 8 heads of 128: one sequence of 1500 tokens 143 -> 98 us, 3000 tokens 266 -> 178, 5000 tokens (320 workgroups)
+// 467 -> 361; 6 of 800 to 1300 (400) 147 -> 186.
 struct Pieces { int hp, pieces, per; };                            // parts by heads, pieces of the longest walk, steps of a piece
 static Pieces pieces(int hp, int64_t wgs, int64_t longest, int64_t mean, int least) {
     const int64_t room = 512 - wgs / 2;

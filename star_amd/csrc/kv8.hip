@@ -276,7 +276,7 @@ __device__ __forceinline__ f16x8 widen<_Float16>(uint32_t lo, uint32_t hi, float
 template <typename T> struct VHalf { static constexpr float by = 1.f; };
 template <> struct VHalf<_Float16> { static constexpr float by = 0.5f; };
 
-// Codes that one workgroup alone reads pass the caches by (four sequences of up to 131072 tokens, 1.0 GB: 183 -> 161 us)
+// Codes that one workgroup alone reads pass the caches by (four sequences of up to 131072 tokens, 1.0 GB: 178 -> 161 us)
 template <bool ONCE, typename V>
 __device__ __forceinline__ V codes(const V* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
