@@ -606,6 +606,9 @@ class NuggetSelfAttention(nn.Module):
             raise ValueError("NuggetSelfAttention: nothing is differentiated through a cache; call it under torch.no_grad()")
         if hidden_states.dim() != 3:
             raise ValueError(f"NuggetSelfAttention: [B,L,{self.embed_dim}] expected with a cache, got {tuple(hidden_states.shape)}")
+        B, L, _ = hidden_states.shape
+        if B * self.num_heads * L >= ops.KV8_MOST_ROWS:            # (refused before anything is appended)
+            raise ValueError(f"NuggetSelfAttention: {B} sequences x {self.num_heads} heads x {L} tokens at once; give them in parts")
         qkv = self.c_attn(hidden_states)
         core = qkv.to(cache.dtype).unflatten(2, (-1, self.head_dim)).transpose(1, 2)       # [B, heads, L, hd]
         q, k, v = core.split([self.num_heads, self.kv_heads, self.kv_heads], dim=1)

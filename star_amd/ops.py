@@ -1922,6 +1922,7 @@ def _causal_layout(q, k, v, plan, scale):
 
 # ----------------------------------------------------------------------------- 8-bit key/value cache
 KV8_BLOCK, KV8_TICKET_STRIDE = 64, 32        # STAR_KV8_BLOCK, STAR_KV8_TICKET_STRIDE
+KV8_MOST_ROWS = 1 << 24                      # kv8_attn takes fewer queries x heads than this in one call
 
 
 class KVCache8:

@@ -581,6 +581,24 @@ def test_kv8_attn_lookback_beyond_32_bits(ops):
         assert torch.equal(ops.kv8_attn(q, cache, causal=False, ilk_diag=far), want), far
 
 
+def test_more_tokens_than_one_call_takes_are_refused_before_they_are_appended(ops, monkeypatch):
+    from star_amd import _lib
+    appended = []
+    m = recording(monkeypatch, ops, [])
+    monkeypatch.setattr(m.c_attn, "forward", lambda x: torch.empty(1).expand(x.shape[0], x.shape[1], 384))
+    monkeypatch.setattr(ops, "kv8_append", lambda *a, **kw: appended.append(a))
+    cache = type("Cache", (), dict(dtype=torch.bfloat16))()
+    with torch.no_grad(), pytest.raises(ValueError, match="in parts"):
+        m(torch.zeros(1, 1, 128).expand(1, 1 << 23, 128), cache=cache)
+    assert not appended
+    # (the library's own limit)
+    c = _lib.KV8Cache(B=1, Hkv=2, T=128, hd=64, dtype=0)
+    for n in ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "lens", "dropped", "tickets"):
+        setattr(c, n, 16)
+    q = _lib.KV8Query(H=2, L=ops.KV8_MOST_ROWS // 2)
+    assert _lib.lib().star_kv8_attn(c, 16, None, None, q, 16, None, 0, None) == -1 and b"queries" in _lib.lib().star_last_error()
+
+
 # ------------------------------------------------------------------------------------------------------ workspaces
 def test_every_launch_is_given_the_workspace_that_the_library_asks_for(ops, monkeypatch):
     """The size is not asked for where launches are never cut: the library agrees on both sides of every border.  (CPU: the
